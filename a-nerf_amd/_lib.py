@@ -101,6 +101,20 @@ class AnerfTrainLayout(C.Structure):
                 ("gemm_ws_floats", C.c_int64)]
 
 
+MAX_GROUPS, MAX_CHOICES, MAX_RANK = 1024, 64, 1024       # groups of a plan, groups of a row, rank of an adapter
+
+
+class AnerfAdapterIO(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n_adapters", C.c_int32), ("rank", C.c_int32), ("scale", C.c_float),
+                ("n_rows", C.c_int64), ("n_in", C.c_int64), ("n_out", C.c_int64), ("x_stride", C.c_int64),
+                ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("down", C.c_void_p), ("up", C.c_void_p),
+                ("scale_of", C.c_void_p), ("offsets", C.c_void_p), ("order", C.c_void_p), ("y", C.c_void_p), ("h", C.c_void_p)]
+
+
+class AnerfAdapterGradIO(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("g_stride", C.c_int64), ("dx", C.c_void_p), ("ddown", C.c_void_p), ("dup", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/anerf.h declares must be listed here
 SIGNATURES = {
     "anerf_last_error": (C.c_char_p, []),
@@ -195,6 +209,17 @@ SIGNATURES = {
     "anerf_rand_fill_dev": (C.c_int, [C.POINTER(AnerfRandJob), C.c_int32, C.c_void_p, C.c_int32, C.c_void_p]),
     "anerf_adam_step_dev": (C.c_int, [C.c_void_p] * 4 + [C.c_int64, C.c_float, C.c_float, C.c_float, C.c_void_p, C.c_int32, C.c_int32,
                                       C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "anerf_route_rows_workspace_size": (C.c_int64, [C.c_int64, C.c_int32]),
+    "anerf_route_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32] + [C.c_void_p] * 4 + [C.c_int64, C.c_void_p]),
+    "anerf_dispatch_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,
+                                      C.c_void_p]),
+    "anerf_combine_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,
+                                     C.c_void_p]),
+    "anerf_combine_rows_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
+                                              C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "anerf_adapter_linear": (C.c_int, [C.POINTER(AnerfAdapterIO), C.c_void_p]),
+    "anerf_adapter_backward_workspace_size": (C.c_int64, [C.POINTER(AnerfAdapterIO)]),
+    "anerf_adapter_backward": (C.c_int, [C.POINTER(AnerfAdapterIO), C.POINTER(AnerfAdapterGradIO), C.c_void_p, C.c_int64, C.c_void_p]),
 }
 
 _lib = None

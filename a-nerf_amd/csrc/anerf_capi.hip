@@ -7,6 +7,7 @@
 #include <vector>
 #include "anerf_dev.h"
 #include "anerf_gemm.h"
+#include "anerf_rows.h"
 
 namespace anerf {
 
@@ -74,6 +75,13 @@ int mlp_bwd_in_enc_entry(int ld, int code, const float* packed_i, const float* d
                          float tau_v, float tau_d, const float* cut_v, const float* cut_d, int S, float* dY, float* dQ, const float* pnoise,
                          int gate_bones, const float* tau_dev, int n_rays, hipStream_t st);
 int launch_gather_rows3(const float* a, const float* b, const long long* idx, int n, int S, int Ni, float* out, hipStream_t st);
+long long route_workspace(long long n, int G);
+int launch_route(const void* idx, int wide, long long n, int G, int32_t* offsets, int32_t* source, int32_t* slot, void* ws, hipStream_t st);
+int launch_rows(int op, int dtype, const void* a, const void* b, const float* w, const int32_t* slot, const int32_t* end, long long T, int k,
+                long long D, void* out, float* dw, hipStream_t st);
+int launch_adapter_linear(const AnerfAdapterIO& A, hipStream_t st);
+long long adapter_backward_workspace(const AnerfAdapterIO& A);
+int launch_adapter_backward(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, void* ws, hipStream_t st);
 int launch_code_reduce(const float* du, int uw, const float* cam, int n, int S, int n_codes, float* rowsum, float* dcodes,
                        hipStream_t st);
 
@@ -1256,6 +1264,99 @@ int anerf_backward(const AnerfConfig* cfg, const AnerfForwardIO* io, const Anerf
   return pass(0, sc, F(t.fwd.raw), F(t.fwd.z), (int)S, io->noise, hier ? b->g_rgb0 : b->g_rgb, hier ? b->g_acc0 : b->g_acc,
               hier ? b->g_disp0 : b->g_disp, hier ? b->g_alpha0 : b->g_alpha, b->packed_t_c, io->aux_c, b->packed_i_c, &b->grads_c,
               b->g_codes_c, io->pts_noise, coarse_part);
+}
+
+// ---- rows of many groups, adapters -------------------------------------------------------------------------------------------
+static int route_check(int64_t n_pairs, int32_t n_groups) {
+  if (n_pairs < 0 || n_pairs > INT32_MAX) return set_error(ANERF_E_SHAPE, "route_rows: the number of pairs must be 0 .. 2^31 - 1");
+  if (n_groups < 1 || n_groups > ROWS_MAX_GROUPS) return set_error(ANERF_E_SHAPE, "route_rows: n_groups must be 1 .. 1024");
+  return ANERF_OK;
+}
+
+int64_t anerf_route_rows_workspace_size(int64_t n_pairs, int32_t n_groups) {
+  const int rc = route_check(n_pairs, n_groups);
+  return rc ? rc : route_workspace(n_pairs, n_groups);
+}
+
+int anerf_route_rows(const void* groups, int32_t wide, int64_t n_pairs, int32_t n_groups, int32_t* offsets, int32_t* source, int32_t* slot,
+                     void* workspace, int64_t ws_bytes, void* stream) {
+  const int rc = route_check(n_pairs, n_groups);
+  if (rc) return rc;
+  if (!offsets || (n_pairs && (!groups || !source || !slot))) return set_error(ANERF_E_NULL, "route_rows: null pointer");
+  const int64_t need = route_workspace(n_pairs, n_groups);
+  if (ws_bytes < need || (need && !workspace)) return set_error(ANERF_E_WORKSPACE, "route_rows: workspace too small");
+  return launch_route(groups, wide, n_pairs, n_groups, offsets, source, slot, workspace, static_cast<hipStream_t>(stream));
+}
+
+static int rows_check(int32_t dtype, int64_t n_rows, int32_t k, int64_t width) {
+  if (dtype != ANERF_F32 && dtype != ANERF_BF16 && dtype != ANERF_F16) return set_error(ANERF_E_CONFIG, "rows: unknown element type");
+  if (k < 1 || k > ROWS_MAX_CHOICES) return set_error(ANERF_E_SHAPE, "rows: 1 .. 64 groups a row");
+  if (n_rows < 0 || width < 0 || n_rows > INT32_MAX / k) return set_error(ANERF_E_SHAPE, "rows: bad sizes");
+  return ANERF_OK;
+}
+
+int anerf_dispatch_rows(const void* x, int32_t dtype, const float* weights, const int32_t* slot, const int32_t* kept, int64_t n_rows, int32_t k,
+                        int64_t width, void* out, void* stream) {
+  const int rc = rows_check(dtype, n_rows, k, width);
+  if (rc || n_rows == 0 || width == 0) return rc;
+  if (!x || !slot || !kept || !out) return set_error(ANERF_E_NULL, "dispatch_rows: null pointer");
+  return launch_rows(0, dtype, x, nullptr, weights, slot, kept, n_rows, k, width, out, nullptr, static_cast<hipStream_t>(stream));
+}
+
+int anerf_combine_rows(const void* z, int32_t dtype, const float* weights, const int32_t* slot, const int32_t* kept, int64_t n_rows, int32_t k,
+                       int64_t width, void* y, void* stream) {
+  const int rc = rows_check(dtype, n_rows, k, width);
+  if (rc || n_rows == 0 || width == 0) return rc;
+  if (!z || !slot || !kept || !y) return set_error(ANERF_E_NULL, "combine_rows: null pointer");
+  return launch_rows(1, dtype, z, nullptr, weights, slot, kept, n_rows, k, width, y, nullptr, static_cast<hipStream_t>(stream));
+}
+
+int anerf_combine_rows_backward(const void* dy, const void* z, int32_t dtype, const float* weights, const int32_t* slot, const int32_t* kept,
+                                int64_t n_rows, int32_t k, int64_t width, void* dz, float* dweights, void* stream) {
+  const int rc = rows_check(dtype, n_rows, k, width);
+  if (rc || n_rows == 0) return rc;
+  if (!dz && !dweights) return ANERF_OK;
+  if (!slot || !kept || !weights || (width && (!dy || (dweights && !z)))) return set_error(ANERF_E_NULL, "combine_rows_backward: null pointer");
+  return launch_rows(2, dtype, dy, z, weights, slot, kept, n_rows, k, width, dz, dweights, static_cast<hipStream_t>(stream));
+}
+
+static int adapter_check(const AnerfAdapterIO* a) {
+  if (!a) return set_error(ANERF_E_NULL, "adapter: null io");
+  if (a->dtype != ANERF_F32 && a->dtype != ANERF_BF16 && a->dtype != ANERF_F16) return set_error(ANERF_E_CONFIG, "adapter: unknown element type");
+  if (a->n_adapters < 1 || a->n_adapters > ROWS_MAX_GROUPS) return set_error(ANERF_E_SHAPE, "adapter: n_adapters must be 1 .. 1024");
+  if (a->rank < 1 || a->rank > ANERF_MAX_RANK) return set_error(ANERF_E_SHAPE, "adapter: rank must be 1 .. 1024");
+  const int64_t lim = INT64_C(1) << 31, side = INT64_C(1) << 24;      // (tiles, pieces and byte offsets stay inside their integers)
+  if (a->n_in < 1 || a->n_out < 1 || a->n_in > side || a->n_out > side) return set_error(ANERF_E_SHAPE, "adapter: n_in / n_out must be 1 .. 2^24");
+  if (a->n_rows < 0 || a->n_rows >= lim) return set_error(ANERF_E_SHAPE, "adapter: the number of rows must be 0 .. 2^31 - 1");
+  if (((a->n_rows + 63) / 64) * ((a->n_out + 63) / 64) >= lim || ((a->n_rows + 63) / 64) * ((a->n_in + 63) / 64) >= lim)
+    return set_error(ANERF_E_SHAPE, "adapter: too many output tiles for one launch");
+  return ANERF_OK;
+}
+
+int anerf_adapter_linear(const AnerfAdapterIO* a, void* stream) {
+  const int rc = adapter_check(a);
+  if (rc || a->n_rows == 0) return rc;
+  if (!a->x || !a->weight || !a->down || !a->up || !a->offsets || !a->y || !a->h) return set_error(ANERF_E_NULL, "adapter_linear: null pointer");
+  if ((uintptr_t)a->h & 15) return set_error(ANERF_E_SHAPE, "adapter_linear: h must be 16-byte aligned");
+  return launch_adapter_linear(*a, static_cast<hipStream_t>(stream));
+}
+
+int64_t anerf_adapter_backward_workspace_size(const AnerfAdapterIO* a) {
+  const int rc = adapter_check(a);
+  return rc ? rc : adapter_backward_workspace(*a);
+}
+
+int anerf_adapter_backward(const AnerfAdapterIO* a, const AnerfAdapterGradIO* g, void* workspace, int64_t ws_bytes, void* stream) {
+  const int rc = adapter_check(a);
+  if (rc) return rc;
+  if (!g) return set_error(ANERF_E_NULL, "adapter_backward: null gradients");
+  if (!g->dx && !g->ddown && !g->dup) return ANERF_OK;
+  if (a->n_rows == 0 && !g->ddown && !g->dup) return ANERF_OK;
+  if (!a->weight || !a->down || !a->up || !a->offsets || (a->n_rows && (!g->g || !a->h || (g->ddown && !a->x))))
+    return set_error(ANERF_E_NULL, "adapter_backward: null pointer");
+  if (!workspace || ws_bytes < adapter_backward_workspace(*a)) return set_error(ANERF_E_WORKSPACE, "adapter_backward: workspace too small");
+  if (((uintptr_t)workspace & 255) || ((uintptr_t)a->h & 15)) return set_error(ANERF_E_SHAPE, "adapter_backward: workspace (256 bytes) or h (16) misaligned");
+  return launch_adapter_backward(*a, *g, workspace, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -192,8 +192,19 @@ class NeRF(nn.Module):
             return None, None
         return self.framecodes.table_for(cam_idx, self.training)
 
-    def forward(self, x):
-        """x [..., input_ch+input_ch_bones+input_ch_views(+1)] -> [..., 4]   (nerf.py:133-148)."""
+    def set_adapters(self, adapters):
+        """adapters.NetAdapters of this network (or None): forward(x, subject_idxs=...) then gives every row its subject's adapter.  Not a
+        child module: the network's state_dict keeps the reference's keys."""
+        self.__dict__["_adapters"] = adapters
+        return self
+
+    def forward(self, x, subject_idxs=None, subject_weights=None):
+        """x [..., input_ch+input_ch_bones+input_ch_views(+1)] -> [..., 4]   (nerf.py:133-148).
+        subject_idxs [...] or [..., k]: the subject(s) of every row, with attached adapters (set_adapters)."""
+        if subject_idxs is not None:
+            if self.__dict__.get("_adapters") is None:
+                raise ValueError("NeRF.forward: subject_idxs without adapters (NeRF.set_adapters)")
+            return self._adapters(self, x, subject_idxs, subject_weights)
         stream, aux = self.packed(fold=False)
         codes = self.framecodes.codes.weight if self.use_framecode else None
         if self.use_framecode and not self.training:

@@ -905,3 +905,191 @@ def backward(state, g, packed_t_c, packed_t_f, perm, shapes_c, shapes_f, packed_
         elif passes in (2, 4, 32) and after_coarse_params is not None:
             after_coarse_params()
     return grads_c, grads_f, g_skts, g_codes_c, g_codes_f
+
+
+# ---- rows of many groups (subjects, experts): in order of their group and back; a shared projection with an adapter per row --------
+# Tensor level, no autograd: adapters.py holds the differentiable calls.
+
+ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class on_device:
+    """make `dev` the current device for the launches inside (the library launches on the current device's current stream)"""
+
+    def __init__(self, dev):
+        self.ctx = torch.cuda.device(dev) if dev.index is not None and dev.index != torch._C._cuda_getDevice() else None
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *a):
+        if self.ctx is not None:
+            self.ctx.__exit__(*a)
+
+
+def _rows_like(t, name, dev=None, dtype=None):
+    """a CUDA(ROCm) tensor of a row type (and of `dev` / `dtype` if given)"""
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if not t.is_cuda or t.dtype not in ROW_DTYPES:
+        raise TypeError(f"{name}: expected a float32 / bfloat16 / float16 CUDA(ROCm) tensor, got {t.dtype} on {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype} like the rows, got {t.dtype}")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{name}: on {t.device}, the rows are on {dev}")
+    return t
+
+
+class RowPlan:
+    """Rows in order of their group (anerf_route_rows).  The pairs (t, j) -- row t's j-th group -- sorted by group, stable, the
+    dropped ones (group outside 0 .. n_groups-1) last:
+      offsets [n_groups + 1] int32   first position of every group; the last entry counts the kept pairs
+      source  [n_rows * k]   int32   position -> pair t * k + j
+      slot    [n_rows, k] or [n_rows] int32   pair -> position (shape of the groups it was made from)"""
+
+    def __init__(self, offsets, source, slot, n_rows, k, n_groups):
+        self.offsets, self.source, self.slot = offsets, source, slot
+        self.n_rows, self.k, self.n_groups = n_rows, k, n_groups
+
+    @property
+    def device(self):
+        return self.offsets.device
+
+    def sorted(self):
+        """the plan of the DISPATCHED rows: n_rows * k of them, lying in group order already"""
+        return SortedRows(self.offsets, self.n_rows * self.k, self.n_groups)
+
+
+class SortedRows:
+    """rows that lie in group order: group g owns rows offsets[g] .. offsets[g+1]-1, the rows behind offsets[n_groups] have none"""
+
+    def __init__(self, offsets, n_rows, n_groups):
+        self.offsets, self.n_rows, self.n_groups = offsets, n_rows, n_groups
+
+    @property
+    def device(self):
+        return self.offsets.device
+
+
+def route_rows(groups, n_groups):
+    """groups [T] or [T, k] int32 / int64 (k <= 64) -> RowPlan; a value outside 0 .. n_groups-1 drops the pair.  Two launches at most, no
+    host sync."""
+    if not torch.is_tensor(groups) or not groups.is_cuda or groups.dtype not in (torch.int32, torch.int64):
+        raise TypeError("route_rows: groups must be an int32 / int64 CUDA(ROCm) tensor")
+    if groups.dim() not in (1, 2):
+        raise ValueError(f"route_rows: groups must be [rows] or [rows, k], got {tuple(groups.shape)}")
+    T, k = groups.shape[0], groups.shape[1] if groups.dim() == 2 else 1
+    if not 1 <= k <= _lib.MAX_CHOICES:
+        raise ValueError(f"route_rows: 1 .. {_lib.MAX_CHOICES} groups a row, got {k}")
+    n_groups = int(n_groups)
+    if not 1 <= n_groups <= _lib.MAX_GROUPS:
+        raise ValueError(f"route_rows: n_groups must be 1 .. {_lib.MAX_GROUPS}, got {n_groups}")
+    groups = groups.contiguous()
+    n, dev, lib = T * k, groups.device, _lib.load()
+    need = lib.anerf_route_rows_workspace_size(n, n_groups)
+    if need < 0:
+        _lib.check(int(need), "anerf_route_rows_workspace_size")
+    # one allocation: offsets | source | slot | workspace (every part starts on 16 bytes)
+    no, ns = (n_groups + 4) // 4 * 4, (n + 3) // 4 * 4
+    buf = torch.empty(no + 2 * ns + (need + 3) // 4, dtype=torch.int32, device=dev)
+    offsets, source, slot, ws = buf[:n_groups + 1], buf[no:no + n], buf[no + ns:no + ns + n], buf[no + 2 * ns:]
+    with on_device(dev):
+        _lib.check(lib.anerf_route_rows(_p(groups), int(groups.dtype == torch.int64), n, n_groups, _p(offsets), _p(source), _p(slot), _p(ws), need,
+                                        _stream()), "anerf_route_rows")
+    return RowPlan(offsets, source, slot.view(groups.shape), T, k, n_groups)
+
+
+def _row_weights(weights, plan):
+    if weights is None:
+        return None
+    if not torch.is_tensor(weights) or weights.dtype != torch.float32 or weights.device != plan.device:
+        raise TypeError(f"weights: expected a float32 tensor on {plan.device}")
+    if weights.numel() != plan.n_rows * plan.k or (weights.dim() > 1 and weights.shape[0] != plan.n_rows):
+        raise ValueError(f"weights: {tuple(weights.shape)} for {plan.n_rows} rows of {plan.k} groups")
+    return weights.contiguous()
+
+
+def _rows_2d(t, n, name, dev):
+    t = _rows_like(t, name, dev)
+    if t.dim() < 1 or t.shape[0] != n:
+        raise ValueError(f"{name}: {tuple(t.shape)} for a plan of {n} rows")
+    width = 1
+    for d in t.shape[1:]:
+        width *= d
+    return t.contiguous(), width
+
+
+def dispatch_rows(x, plan, weights=None):
+    """x [T, ...] -> [T * k, ...] in group order (times weights [T, k] if given); zero rows behind the kept ones"""
+    x, width = _rows_2d(x, plan.n_rows, "dispatch_rows", plan.device)
+    weights = _row_weights(weights, plan)
+    out = torch.empty((plan.n_rows * plan.k,) + tuple(x.shape[1:]), dtype=x.dtype, device=x.device)
+    with on_device(x.device):
+        _lib.check(_lib.load().anerf_dispatch_rows(_p(x), ROW_DTYPES[x.dtype], _p(weights), _p(plan.slot), _p(plan.offsets[-1:]), plan.n_rows, plan.k,
+                                                   width, _p(out), _stream()), "anerf_dispatch_rows")
+    return out
+
+
+def combine_rows(z, plan, weights=None):
+    """z [T * k, ...] in group order -> [T, ...]: the sum of every row's kept entries (times weights [T, k] if given)"""
+    z, width = _rows_2d(z, plan.n_rows * plan.k, "combine_rows", plan.device)
+    weights = _row_weights(weights, plan)
+    y = torch.empty((plan.n_rows,) + tuple(z.shape[1:]), dtype=z.dtype, device=z.device)
+    with on_device(z.device):
+        _lib.check(_lib.load().anerf_combine_rows(_p(z), ROW_DTYPES[z.dtype], _p(weights), _p(plan.slot), _p(plan.offsets[-1:]), plan.n_rows, plan.k,
+                                                  width, _p(y), _stream()), "anerf_combine_rows")
+    return y
+
+
+def combine_rows_backward(dy, z, plan, weights, want_dz=True, want_dw=True):
+    """gradients of combine_rows with weights -> (dz [T * k, ...] or None, dweights like weights or None)"""
+    dy, width = _rows_2d(dy, plan.n_rows, "combine_rows_backward", plan.device)
+    z = z.contiguous() if want_dw else None
+    w = _row_weights(weights, plan)
+    dz = torch.empty((plan.n_rows * plan.k,) + tuple(dy.shape[1:]), dtype=dy.dtype, device=dy.device) if want_dz else None
+    dw = torch.empty(weights.shape, dtype=torch.float32, device=dy.device) if want_dw else None
+    with on_device(dy.device):
+        _lib.check(_lib.load().anerf_combine_rows_backward(_p(dy), _p(z), ROW_DTYPES[dy.dtype], _p(w), _p(plan.slot), _p(plan.offsets[-1:]), plan.n_rows,
+                                                           plan.k, width, _p(dz), _p(dw), _stream()), "anerf_combine_rows_backward")
+    return dz, dw
+
+
+def _adapter_io(x, weight, down, up, rows, bias, scale, scale_of):
+    """AnerfAdapterIO of 2-D rows x (any row stride) + the tensors whose pointers it holds"""
+    io = _lib.AnerfAdapterIO()
+    io.dtype, io.n_adapters, io.rank, io.scale = ROW_DTYPES[x.dtype], down.shape[0], down.shape[1], float(scale)
+    io.n_rows, io.n_in, io.n_out, io.x_stride = x.shape[0], weight.shape[1], weight.shape[0], x.stride(0)
+    order = rows.source if isinstance(rows, RowPlan) else None
+    keep = [x, weight, down, up, bias, scale_of, rows.offsets, order]
+    for name, t in zip(("x", "weight", "down", "up", "bias", "scale_of", "offsets", "order"), keep):
+        setattr(io, name, None if t is None else t.data_ptr())
+    return io, keep
+
+
+def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=None):
+    """x [M, K] W^T + bias + s_i (x A_i^T) B_i^T (anerf_adapter_linear) -> (y [M, N], h): h is what the backward needs.  weight [N, K],
+    down [L, R, K] (A), up [L, N, R] (B), rows: RowPlan (k = 1) or SortedRows of the M rows over the L adapters."""
+    io, keep = _adapter_io(x, weight, down, up, rows, bias, scale, scale_of)
+    y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=x.device)
+    h = torch.empty(x.shape[0], (down.shape[1] + 15) // 16 * 16, dtype=torch.float32, device=x.device)
+    io.y, io.h = y.data_ptr(), h.data_ptr()
+    with on_device(x.device):
+        _lib.check(_lib.load().anerf_adapter_linear(C.byref(io), _stream()), "anerf_adapter_linear")
+    return y, h
+
+
+def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, want_dx=True, want_ddown=True, want_dup=True):
+    """gradients of adapter_linear with weight and bias frozen (anerf_adapter_backward) -> (dx, ddown, dup), None where not wanted"""
+    io, keep = _adapter_io(x, weight, down, up, rows, None, scale, scale_of)
+    io.h = h.data_ptr()
+    dx = torch.empty(x.shape[0], weight.shape[1], dtype=x.dtype, device=x.device) if want_dx else None
+    ddown = torch.empty_like(down) if want_ddown else None
+    dup = torch.empty_like(up) if want_dup else None
+    go = _lib.AnerfAdapterGradIO(g.data_ptr(), g.stride(0), None if dx is None else dx.data_ptr(), None if ddown is None else ddown.data_ptr(),
+                                 None if dup is None else dup.data_ptr())
+    lib = _lib.load()
+    with on_device(x.device):
+        ws, nbytes = _workspace(lib.anerf_adapter_backward_workspace_size, "anerf_adapter_backward_workspace_size", x.device, C.byref(io))
+        _lib.check(lib.anerf_adapter_backward(C.byref(io), C.byref(go), _p(ws), nbytes, _stream()), "anerf_adapter_backward")
+    return dx, ddown, dup

@@ -552,6 +552,63 @@ int anerf_make_ray_batch(const float* rays_o, const float* rays_d, int32_t n_ray
 int anerf_cyl_bbox(const double* cyls, const double* c2ws, const double* hwf, const int32_t* off, const double* circle,
                    int32_t n_frames, int32_t* bbox, void* stream);
 
+/* ---- rows of many groups: sorted by group and back, and a shared projection with a low-rank adapter per row ----------------
+ * One set of shared weights serves many subjects: a batch holds rows of several of them, each subject owning a thin pair of matrices
+ * (A_i, B_i) beside every shared projection.  Element types of the calls below: */
+#define ANERF_F32 0
+#define ANERF_BF16 1
+#define ANERF_F16 2
+
+/* Plan of n_rows rows with k groups each (k = 1: one group a row; a mixture of experts: k > 1).  groups [n_rows * k] int64
+ * (wide != 0) or int32; a value outside 0 .. n_groups-1 drops the pair.  Stable: pairs of a group keep their order; the dropped pairs
+ * come last, in order.  Outputs: offsets [n_groups + 1] (offsets[g] = first position of group g, offsets[n_groups] = pairs kept),
+ * source [n_rows * k] (position -> pair), slot [n_rows * k] (pair -> position).  n_groups <= 1024, k <= 64, n_rows * k < 2^31.
+ * workspace: anerf_route_rows_workspace_size bytes (may be 0), 16-byte aligned. */
+int64_t anerf_route_rows_workspace_size(int64_t n_pairs, int32_t n_groups);
+int anerf_route_rows(const void* groups, int32_t wide, int64_t n_pairs, int32_t n_groups, int32_t* offsets, int32_t* source, int32_t* slot,
+                     void* workspace, int64_t ws_bytes, void* stream);
+/* out [n_rows * k][width]: out[slot[t][j]] = x[t] (times weights[t][j] if given), zero at the positions of dropped pairs.
+ * kept: DEVICE pointer to the number of kept pairs (offsets + n_groups).  weights [n_rows][k] float or NULL. */
+int anerf_dispatch_rows(const void* x, int32_t dtype, const float* weights, const int32_t* slot, const int32_t* kept, int64_t n_rows, int32_t k,
+                        int64_t width, void* out, void* stream);
+/* y [n_rows][width] = sum over the kept pairs of row t, in the order of j, of z[slot[t][j]] (times weights[t][j]): summed in fp32,
+ * rounded once.  A row with no kept pair gets zeros. */
+int anerf_combine_rows(const void* z, int32_t dtype, const float* weights, const int32_t* slot, const int32_t* kept, int64_t n_rows, int32_t k,
+                       int64_t width, void* y, void* stream);
+/* Gradients of anerf_combine_rows with weights: dz [n_rows * k][width] (weights[t][j] * dy[t] at the pair's position, zero at dropped
+ * positions) and dweights [n_rows][k] (<dy[t], z[slot[t][j]]> in fp32, zero for dropped pairs); either may be NULL.  The gradient of
+ * anerf_dispatch_rows is anerf_combine_rows, that of anerf_combine_rows without weights is anerf_dispatch_rows. */
+int anerf_combine_rows_backward(const void* dy, const void* z, int32_t dtype, const float* weights, const int32_t* slot, const int32_t* kept,
+                                int64_t n_rows, int32_t k, int64_t width, void* dz, float* dweights, void* stream);
+
+/* y[r] = x[r] W^T + bias + s_i (x[r] A_i^T) B_i^T, i = adapter of row r.  Positions 0 .. n_rows-1 are the rows in the order of their
+ * adapter: adapter i owns positions offsets[i] .. offsets[i+1]-1, positions from offsets[n_adapters] on have none (shared projection
+ * alone); order [n_rows] maps a position to its row, NULL = the rows lie in that order.  s_i = scale * scale_of[i] (scale_of NULL: scale).
+ *   x [n_rows][n_in] rows x_stride elements apart, weight [n_out][n_in], bias [n_out] or NULL, down [n_adapters][rank][n_in] (A),
+ *   up [n_adapters][n_out][rank] (B), y [n_rows][n_out]; h [n_rows][rank rounded up to 16] fp32, 16-byte aligned, written: x A_i^T by position
+ *   (kept for the backward).  All of dtype but h and scale_of.  Sums in fp32, one rounding at the end. */
+typedef struct AnerfAdapterIO {
+  int32_t dtype, n_adapters, rank;
+  float scale;
+  int64_t n_rows, n_in, n_out, x_stride;
+  const void *x, *weight, *bias, *down, *up;
+  const float* scale_of;
+  const int32_t *offsets, *order;
+  void* y;
+  float* h;
+} AnerfAdapterIO;
+int anerf_adapter_linear(const AnerfAdapterIO* io, void* stream);
+/* Gradients with weight and bias frozen, from g = d loss / d y ([n_rows][n_out], rows g_stride apart) and the forward's io (its h as
+ * the forward left it; y and bias are not read): dx [n_rows][n_in], ddown / dup shaped as down / up; each may be NULL.  Every element is
+ * written (adapters without rows: zeros), every sum has one order.  workspace: anerf_adapter_backward_workspace_size bytes, 256-byte aligned. */
+typedef struct AnerfAdapterGradIO {
+  const void* g;
+  int64_t g_stride;
+  void *dx, *ddown, *dup;
+} AnerfAdapterGradIO;
+int64_t anerf_adapter_backward_workspace_size(const AnerfAdapterIO* io);
+int anerf_adapter_backward(const AnerfAdapterIO* io, const AnerfAdapterGradIO* grad, void* workspace, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
