@@ -308,59 +308,99 @@ __global__ void __launch_bounds__(MN_THREADS) k_main(MainArgs P) {
 }
 
 // ---------------------------------------------------------------------------------------------------------- gradients of A and B
-// part[piece][j][c] = sum over the piece's positions p of Z[order[p]][c] * V[p][j]       (Z = x, V = u: dA;  Z = g, V = h: dB)
-// A thread owns 4 columns of Z and 16 ranks; V's row is the same for the whole workgroup and comes through the scalar cache.
-constexpr int TG_THREADS = 256, TG_COLS = 4, TG_RANKS = 16;
+// part[piece] = sum over the piece's positions p of Z[order[p]][c] * V[p][j]        (Z = x, V = u: dA;  Z = g, V = h: dB)
+// The contraction runs over rows, so that v_mfma_f32_16x16x4_f32 takes its operands as they lie in memory: lane (i, q) loads
+// columns 4i .. 4i+3 of row q of a group of four, element e being its operand for the block of columns 4i + e, and V[p][16n + i].
+// Values of 16-bit types become fp32 on the way (h and u stay whole): up to rank 32 the loads of Z are what bounds it, not the MFMAs.
+// A workgroup owns 64 columns x 16*NJ ranks of a piece; its four waves take every fourth group of rows and are added through LDS.
+// BY_RANK: part [piece][Rp][C] (operand order Z, V), else [piece][C][Rp] (V, Z): a lane ends with four values that lie together.
+constexpr int TG_WAVES = 4, TG_COLS = 64, TG_DEPTH = 4;
 
-template <int DT>
-__global__ void __launch_bounds__(TG_THREADS) k_thin_grad(const typename Elem<DT>::T* __restrict__ Z, long long ldz, const int32_t* __restrict__ order,
-                                                          const float* __restrict__ V, const int32_t* __restrict__ offsets, int L, long long C,
-                                                          int Rp, int rows, float* __restrict__ part) {
+template <int DT, int NJ, bool BY_RANK>
+__global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(const typename Elem<DT>::T* __restrict__ Z, long long ldz, const int32_t* __restrict__ order,
+                                                             const float* __restrict__ V, const int32_t* __restrict__ offsets, int L, long long C,
+                                                             int Rp, int rows, float* __restrict__ part) {
   typedef typename Elem<DT>::T E;
-  typedef E vec __attribute__((ext_vector_type(TG_COLS)));
+  typedef E vec __attribute__((ext_vector_type(4)));
+  __shared__ f32x4 red[TG_WAVES - 1][4 * NJ][64];
   int a, p0, p1;
   if (!find_piece(offsets, L, rows, blockIdx.y, a, p0, p1)) return;
-  p0 = __builtin_amdgcn_readfirstlane(p0);
-  p1 = __builtin_amdgcn_readfirstlane(p1);
-  const long long c = ((long long)blockIdx.x * TG_THREADS + threadIdx.x) * TG_COLS;
-  const int j0 = blockIdx.z * TG_RANKS;
-  if (c >= C) return;
-  const bool whole = c + TG_COLS <= C;
-  float acc[TG_COLS][TG_RANKS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+  const long long c = (long long)blockIdx.x * TG_COLS + 4 * i;
+  const int j0 = blockIdx.z * 16 * NJ;
+  const bool whole = c + 4 <= C;
+  f32x4 acc[4][NJ];
 #pragma unroll
-  for (int e = 0; e < TG_COLS; ++e)
+  for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int j = 0; j < TG_RANKS; ++j) acc[e][j] = 0.f;
-  for (int p = p0; p < p1; ++p) {
-    const E* zr = Z + (long long)(order ? order[p] : p) * ldz + c;
-    float z[TG_COLS];
-    if (whole) {
-      vec v;
-      __builtin_memcpy(&v, zr, sizeof(v));
+    for (int n = 0; n < NJ; ++n) acc[e][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int b = p0 + 4 * wave; b < p1; b += 4 * TG_WAVES * TG_DEPTH) {
+    f32x4 z[TG_DEPTH];
+    float v[TG_DEPTH][NJ];
 #pragma unroll
-      for (int e = 0; e < TG_COLS; ++e) z[e] = (float)v[e];
-    } else {
+    for (int d = 0; d < TG_DEPTH; ++d) {
+      const int p = b + 4 * TG_WAVES * d + q;
+      const bool on = p < p1;
+      z[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < TG_COLS; ++e) z[e] = c + e < C ? (float)zr[e] : 0.f;
+      for (int n = 0; n < NJ; ++n) v[d][n] = on && j0 + 16 * n < Rp ? V[(long long)p * Rp + j0 + 16 * n + i] : 0.f;
+      if (on) {
+        const E* zr = Z + (long long)(order ? order[p] : p) * ldz + c;
+        if (whole) {
+          vec w;
+          __builtin_memcpy(&w, zr, sizeof(w));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[d][e] = (float)w[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < C) z[d][e] = (float)zr[e];
+        }
+      }
     }
-    const float* vr = V + (long long)p * Rp + j0;
 #pragma unroll
-    for (int j = 0; j < TG_RANKS; ++j) {
-      const float f = vr[j];
+    for (int d = 0; d < TG_DEPTH; ++d)
 #pragma unroll
-      for (int e = 0; e < TG_COLS; ++e) acc[e][j] = fmaf(z[e], f, acc[e][j]);
-    }
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n)
+          acc[e][n] = BY_RANK ? __builtin_amdgcn_mfma_f32_16x16x4f32(z[d][e], v[d][n], acc[e][n], 0, 0, 0)
+                              : __builtin_amdgcn_mfma_f32_16x16x4f32(v[d][n], z[d][e], acc[e][n], 0, 0, 0);
   }
+  if (wave) {
 #pragma unroll
-  for (int j = 0; j < TG_RANKS; ++j) {
-    float* o = part + ((long long)blockIdx.y * Rp + j0 + j) * C + c;
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int e = 0; e < TG_COLS; ++e)
-      if (c + e < C) o[e] = acc[e][j];
+      for (int n = 0; n < NJ; ++n) red[wave - 1][e * NJ + n][lane] = acc[e][n];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 0; w < TG_WAVES - 1; ++w)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) acc[e][n] += red[w][e * NJ + n][lane];
+  const long long base = (long long)blockIdx.y * Rp * C, c0 = (long long)blockIdx.x * TG_COLS;
+#pragma unroll
+  for (int n = 0; n < NJ; ++n) {
+    if (j0 + 16 * n >= Rp) break;
+    if (BY_RANK) {      // block e, register r: column 16q + 4r + e of rank 16n + i
+      float* o = part + base + (long long)(j0 + 16 * n + i) * C + c0 + 16 * q;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c0 + 16 * q + 4 * r + e < C) o[4 * r + e] = acc[e][n][r];
+    } else {            // block e, register r: rank 16n + 4q + r of column 4i + e
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < C) *reinterpret_cast<f32x4*>(part + base + (c + e) * Rp + j0 + 16 * n + 4 * q) = acc[e][n];
+    }
   }
 }
 
-// adds an adapter's pieces in their order, times s_i; BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
+// adds an adapter's pieces in their order, times s_i.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
 template <int DT, bool BY_RANK>
 __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__ part, const int32_t* __restrict__ offsets, int L, long long C, int R,
                                                        int Rp, int rows, const float* __restrict__ scale_of, float scale,
@@ -373,12 +413,13 @@ __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__
   for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
   const int n = (offsets[a + 1] - offsets[a] + rows - 1) / rows;
   const float s = scale_of ? scale * scale_of[a] : scale;
-  const long long all = C * R;
+  const long long all = C * R, stride = C * Rp;
   for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
-    const long long j = e / C, c = e % C;
+    const float* src = part + first * stride + (BY_RANK ? e : e / R * Rp + e % R);
     float v = 0.f;
-    for (int q = 0; q < n; ++q) v += part[((long long)(first + q) * Rp + j) * C + c];
-    out[(long long)a * all + (BY_RANK ? j * C + c : c * R + j)] = (E)(v * s);
+#pragma unroll 8
+    for (int q = 0; q < n; ++q) v += src[q * stride];
+    out[(long long)a * all + e] = (E)(v * s);
   }
 }
 
@@ -403,11 +444,9 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   U* out = static_cast<U*>(T.out) + b / T.tiles * T.rows * T.cols;
   const long long r0 = b % T.tiles / T.tiles_c * 64, c0 = b % T.tiles % T.tiles_c * 64;
   const int cx = threadIdx.x & 63, ry = threadIdx.x >> 6;
-#pragma unroll
   for (int r = ry; r < 64; r += 4)
     if (r0 + r < T.rows && c0 + cx < T.cols) t[r][cx] = in[(r0 + r) * T.cols + c0 + cx];
   __syncthreads();
-#pragma unroll
   for (int c = ry; c < 64; c += 4)
     if (c0 + c < T.cols && r0 + cx < T.rows) out[(c0 + c) * T.rows + r0 + cx] = t[cx][c];
 }
@@ -450,13 +489,13 @@ int launch_adapter_linear(const AnerfAdapterIO& A, hipStream_t st) {
   }
 }
 
-// rows of a piece of k_thin_grad: enough pieces to fill the chip, as few as that allows (each writes C x Rp floats)
+// rows of a piece of k_thin_grad: about 1024 workgroups (a chip full of them twice over), but 64 rows at least (a piece writes C x Rp floats)
+static int grad_ranks(int Rp) { return Rp <= 16 ? 1 : Rp <= 32 ? 2 : 4; }
 static int grad_rows(long long M, long long C, int Rp) {
-  const long long blocks_c = (C + TG_THREADS * TG_COLS - 1) / (TG_THREADS * TG_COLS) * (Rp / TG_RANKS);
-  long long pieces = (1024 + blocks_c - 1) / blocks_c;
-  long long rows = (M + pieces - 1) / pieces;
-  rows = (rows + 31) / 32 * 32;
-  return (int)(rows < 32 ? 32 : rows);
+  const long long blocks = (C + TG_COLS - 1) / TG_COLS * ((Rp + 16 * grad_ranks(Rp) - 1) / (16 * grad_ranks(Rp)));
+  const long long pieces = (1024 + blocks - 1) / blocks;
+  const long long rows = ((M + pieces - 1) / pieces + 63) / 64 * 64;
+  return (int)(rows < 64 ? 64 : rows);
 }
 
 static long long part_floats(long long M, int L, long long C, int Rp) {
@@ -491,8 +530,12 @@ static int thin_grad_t(const void* Z, long long ldz, const int32_t* order, const
   const int Rp = (A.rank + 15) / 16 * 16, rows = grad_rows(A.n_rows, C, Rp);
   const long long pieces = pieces_bound(A.n_rows, A.n_adapters, rows);
   if (pieces > 0) {
-    const dim3 grid((unsigned)((C + TG_THREADS * TG_COLS - 1) / (TG_THREADS * TG_COLS)), (unsigned)pieces, Rp / TG_RANKS);
-    k_thin_grad<DT><<<grid, TG_THREADS, 0, st>>>(static_cast<const E*>(Z), ldz, order, V, A.offsets, A.n_adapters, C, Rp, rows, part);
+    const int nj = grad_ranks(Rp);
+    const dim3 grid((unsigned)((C + TG_COLS - 1) / TG_COLS), (unsigned)pieces, (Rp + 16 * nj - 1) / (16 * nj));
+    auto run = [&](auto kernel) { kernel<<<grid, TG_WAVES * 64, 0, st>>>(static_cast<const E*>(Z), ldz, order, V, A.offsets, A.n_adapters, C, Rp, rows, part); };
+    if (nj == 1) run(k_thin_grad<DT, 1, BY_RANK>);
+    else if (nj == 2) run(k_thin_grad<DT, 2, BY_RANK>);
+    else run(k_thin_grad<DT, 4, BY_RANK>);
     const int rc = check_launch("k_thin_grad");
     if (rc) return rc;
   }
