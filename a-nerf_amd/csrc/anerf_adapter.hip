@@ -15,7 +15,8 @@ namespace anerf {
 // ---------------------------------------------------------------------------------------------------------------- h = x A^T
 // HBM-bound on x.  The four waves split the contraction (every fourth 64-byte step), each holding all 32 rows x 16*NJ ranks of the
 // piece in MFMA accumulators, fed straight from memory: a row of A serves 32 rows of x, and nothing is read twice from HBM.
-constexpr int TH_ROWS = 32, TH_WAVES = 4;
+constexpr int TH_ROWS = 32, TH_WAVES = 4, TH_DEPTH = 4;
+template <int V> struct Const { static constexpr int value = V; };
 
 template <int DT, int NJ>
 __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const int32_t* __restrict__ order,
@@ -44,19 +45,27 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
 #pragma unroll
     for (int n = 0; n < NJ; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   const long long steps = K / STEP;
-#pragma unroll 4
-  for (long long s = wave; s < steps; s += TH_WAVES) {
-    const long long k = s * STEP + q * EPC;
-    u32x4 xv[2], av[NJ];
+  auto walk = [&](long long s0, auto depth) {       // `depth` steps of this wave, all their loads in front of the products
+    constexpr int D = decltype(depth)::value;
+    u32x4 xv[D][2], av[D][NJ];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) xv[m] = load16(xr[m] + k);
+    for (int d = 0; d < D; ++d) {
+      const long long k = (s0 + d * TH_WAVES) * STEP + q * EPC;
 #pragma unroll
-    for (int n = 0; n < NJ; ++n) av[n] = load16(ar[n] + k);
+      for (int m = 0; m < 2; ++m) xv[d][m] = load16(xr[m] + k);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+      for (int n = 0; n < NJ; ++n) av[d][n] = load16(ar[n] + k);
+    }
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) acc[m][n] = Elem<DT>::mma(av[n], xv[m], acc[m][n]);
-  }
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) acc[m][n] = Elem<DT>::mma(av[d][n], xv[d][m], acc[m][n]);
+  };
+  long long s = wave;
+  for (; s + (TH_DEPTH - 1) * TH_WAVES < steps; s += TH_DEPTH * TH_WAVES) walk(s, Const<TH_DEPTH>());
+  for (; s < steps; s += TH_WAVES) walk(s, Const<1>());
   if (steps * STEP < K && wave == (int)(steps % TH_WAVES)) {
     const long long k = steps * STEP + q * EPC;
     u32x4 xv[2], av[NJ];
@@ -103,7 +112,7 @@ __device__ __forceinline__ u32x4 h_operand(const float* __restrict__ hr, int c, 
     const float* s = hr + 16 * c + 8 * (q & 1);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float f = s[e] * down_scale;
+      const float f = DT == ANERF_F16 ? s[e] * down_scale : s[e];
       const E hi = (E)f;
       const float rest = f - (float)hi;
       v[e] = q < 2 ? hi : (E)(__builtin_isfinite(f) && __builtin_isfinite((float)hi) ? rest : 0.f);
@@ -119,13 +128,15 @@ __device__ __forceinline__ u32x4 b_operand(const typename Elem<DT>::T* __restric
 }
 
 // ------------------------------------------------------------------------------------------------------------------ y = x W^T ...
-// BM positions x BN outputs a workgroup, 2 x 2 waves, 16x16 MFMA blocks with W's rows as the first operand, so that a lane ends
+// BM positions x BN outputs a workgroup of WM x WN waves, 16x16 MFMA blocks with W's rows as the first operand, so that a lane ends
 // with four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, double-buffered; 16-byte
-// chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.
-// The low-rank term comes first: for every adapter with positions in the tile, h B_i^T is formed in accumulators of its own and taken
-// over by that adapter's rows alone (a NaN in one adapter stays with its rows), and multiplied by s_i in fp32.
-constexpr int MN_THREADS = 256;
-
+// chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.  DIRECT: global_load_lds_dwordx4, eight rows
+// an instruction, the lanes fetching the chunks in the order they have to lie in LDS (16-byte aligned rows); otherwise through registers,
+// at any alignment.
+// The low-rank term comes first, behind the first stage's loads: for every adapter with positions in the tile h B_i^T is formed from
+// zero and added to that adapter's rows alone (a NaN in one adapter stays with its rows), times s_i in fp32.
+// fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set, so that no chain of
+// additions is longer than 8 * FOLD + K / (32 * FOLD).
 struct MainArgs {
   const void *x, *w, *bias, *up;
   const float* scale_of;       // per adapter, or NULL
@@ -138,62 +149,88 @@ struct MainArgs {
   float scale;
 };
 
-template <int DT, int BM, int BN>
-__global__ void __launch_bounds__(MN_THREADS) k_main(MainArgs P) {
+constexpr int FOLD = 8;
+
+template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_main(MainArgs P) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, KB = 8 * EPC;        // elements of a 128-byte row piece
-  constexpr int MI = BM / 32, NI = BN / 32;               // 16-row / 16-output blocks of a wave
-  constexpr int XL = BM / 32, WL = BN / 32;               // 16-byte loads of a thread and stage
-  __shared__ u32x4 lds[2][(BM + BN) * 8];
+  constexpr int NW = WM * WN;
+  constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
+  constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;       // 16-byte loads of a lane and stage
+  constexpr int STAGE = (BM + BN) * 8;                    // 16-byte units
+  extern __shared__ u32x4 lds[];                          // [2][STAGE]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
-  const int wm = wave & 1, wn = wave >> 1;
-  const long long tiles_n = (P.N + BN - 1) / BN;
-  const long long m0 = (long long)blockIdx.x / tiles_n * BM, n0 = (long long)blockIdx.x % tiles_n * BN;
+  const int wm = wave % WM, wn = wave / WM;
+  // workgroups go round-robin to the 8 XCDs: each XCD gets a contiguous range of the tile order, in which 4 row tiles share a column of W
+  long long m0, n0;
+  {
+    const long long tm = (P.M + BM - 1) / BM, tn = (P.N + BN - 1) / BN, all = tm * tn;
+    const long long xcd = blockIdx.x & 7, t = xcd * (all >> 3) + (xcd < (all & 7) ? xcd : (all & 7)) + (blockIdx.x >> 3);
+    const long long g = t / (4 * tn), in = t % (4 * tn);
+    const long long rows = tm - 4 * g < 4 ? tm - 4 * g : 4;
+    m0 = (4 * g + in % rows) * BM;
+    n0 = in / rows * BN;
+  }
   const E* X = static_cast<const E*>(P.x);
   const E* W = static_cast<const E*>(P.w);
-  const int ch = tid & 7;
+  // a lane's part of every stage: row r = 8 * (wave + NW * l) + lane / 8, the chunk that has to lie at position lane % 8
+  const int sub = lane >> 3, ch = (lane & 7) ^ sub;
   const E* xrow[XL];
   const E* wrow[WL];
 #pragma unroll
   for (int l = 0; l < XL; ++l) {
-    long long p = m0 + (tid >> 3) + 32 * l;
+    long long p = m0 + 8 * (wave + NW * l) + sub;
     if (p >= P.M) p = P.M - 1;
-    xrow[l] = X + (P.order ? (long long)P.order[p] : p) * P.ldx;
+    xrow[l] = X + (P.order ? (long long)P.order[p] : p) * P.ldx + ch * EPC;
   }
 #pragma unroll
   for (int l = 0; l < WL; ++l) {
-    long long n = n0 + (tid >> 3) + 32 * l;
+    long long n = n0 + 8 * (wave + NW * l) + sub;
     if (n >= P.N) n = P.N - 1;
-    wrow[l] = W + n * P.K;
+    wrow[l] = W + n * P.K + ch * EPC;
   }
   u32x4 rx[XL], rw[WL];
-  auto fetch = [&](long long s) {
-    const long long k = s * KB + ch * EPC;
-    if (k + EPC <= P.K) {
+  auto at = [&](int buf, int row8) { return buf * STAGE + row8 * 64; };      // eight rows of 128 bytes
+  auto dma = [&](const E* src, int to) {
+    const unsigned l = (unsigned)reinterpret_cast<size_t>((lds_ptr_t)(lds + to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(src) : "memory", "m0");
+  };
+  auto fetch_regs = [&](long long s) {
+    const long long k = s * KB, left = P.K - k - ch * EPC;
+    if (left >= EPC) {
 #pragma unroll
       for (int l = 0; l < XL; ++l) rx[l] = load16(xrow[l] + k);
 #pragma unroll
       for (int l = 0; l < WL; ++l) rw[l] = load16(wrow[l] + k);
     } else {
 #pragma unroll
-      for (int l = 0; l < XL; ++l) rx[l] = load_tail<DT>(xrow[l], k, P.K);
+      for (int l = 0; l < XL; ++l) rx[l] = load_tail<DT>(xrow[l] + k, 0, left);
 #pragma unroll
-      for (int l = 0; l < WL; ++l) rw[l] = load_tail<DT>(wrow[l], k, P.K);
+      for (int l = 0; l < WL; ++l) rw[l] = load_tail<DT>(wrow[l] + k, 0, left);
     }
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int l = 0; l < XL; ++l) {
-      const int r = (tid >> 3) + 32 * l;
-      lds[buf][r * 8 + (ch ^ (r & 7))] = rx[l];
-    }
+    for (int l = 0; l < XL; ++l) lds[at(buf, wave + NW * l) + lane] = rx[l];
 #pragma unroll
-    for (int l = 0; l < WL; ++l) {
-      const int r = (tid >> 3) + 32 * l;
-      lds[buf][(BM + r) * 8 + (ch ^ (r & 7))] = rw[l];
+    for (int l = 0; l < WL; ++l) lds[at(buf, BM / 8 + wave + NW * l) + lane] = rw[l];
+  };
+  const long long stages = (P.K + KB - 1) / KB, full = P.K / KB;
+  // starts stage s; DIRECT: into LDS (the last, partial one through registers), otherwise into registers
+  auto start = [&](long long s, int buf) {
+    if (DIRECT && s < full) {
+      const long long k = s * KB;
+#pragma unroll
+      for (int l = 0; l < XL; ++l) dma(xrow[l] + k, at(buf, wave + NW * l));
+#pragma unroll
+      for (int l = 0; l < WL; ++l) dma(wrow[l] + k, at(buf, BM / 8 + wave + NW * l));
+    } else {
+      fetch_regs(s);
+      if (DIRECT) put(buf);
     }
   };
-  fetch(0);
+  start(0, 0);
   f32x4 acc[MI][NI];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
@@ -205,89 +242,127 @@ __global__ void __launch_bounds__(MN_THREADS) k_main(MainArgs P) {
   const int kept = P.offsets[P.L];
   if (m0 < kept) {
     if (tile_end > kept) tile_end = kept;
-    int lo = 0, hi = P.L;                    // first adapter that ends behind m0
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (P.offsets[mid + 1] > m0) hi = mid; else lo = mid + 1;
+    int first = 0;                           // first adapter that ends behind m0, 64 at a time
+    for (int a0 = 0; a0 < P.L; a0 += 64) {
+      const int a = a0 + lane;
+      const unsigned long long past = __ballot(a < P.L && P.offsets[a < P.L ? a + 1 : 0] > m0);
+      if (past) {
+        first = a0 + __builtin_ctzll(past);
+        break;
+      }
     }
     const int chunks = P.Rp / 16;
-    for (int a = lo; a < P.L; ++a) {
+    for (int a = first; a < P.L; ++a) {
       const int a0 = P.offsets[a], a1 = P.offsets[a + 1];
       if (a0 >= tile_end) break;
       if (a1 <= a0) continue;
-      const E* B = static_cast<const E*>(P.up) + (long long)a * P.N * P.R;
       const float s = P.scale_of ? P.scale * P.scale_of[a] : P.scale;
+      bool mine[MI];
+      const float* hr[MI];
+      float ds[MI], us[MI];
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
-        const long long p = m0 + wm * (BM / 2) + 16 * m + i;
-        const bool mine = p >= a0 && p < a1;
-        if (!__ballot(mine)) continue;
-        const float* hr = P.h + (mine ? p : (long long)a0) * P.Rp;
-        float ds = 1.f, us = s;
+        const long long p = m0 + wm * TM + 16 * m + i;
+        mine[m] = p >= a0 && p < a1;
+        hr[m] = P.h + (mine[m] ? p : (long long)a0) * P.Rp;
+        ds[m] = 1.f;
+        us[m] = s;
         if constexpr (DT == ANERF_F16) {     // largest |h| of the row -> [1, 2)
           float big = 0.f;
           for (int j = 0; j < P.Rp; j += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(hr + j);
+            const f32x4 v = *reinterpret_cast<const f32x4*>(hr[m] + j);
             big = fmaxf(fmaxf(big, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
           }
           if (big > 0.f && __builtin_isfinite(big)) {
             const int e = min(max(ilogbf(big), -100), 100);
-            ds = ldexpf(1.f, -e);
-            us = s * ldexpf(1.f, e);
+            ds[m] = ldexpf(1.f, -e);
+            us[m] = s * ldexpf(1.f, e);
           }
         }
+      }
+      const E* br[NI];
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-          const long long col = n0 + wn * (BN / 2) + 16 * n + i;
-          const E* br = B + (col < P.N ? col : P.N - 1) * P.R;
-          f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
-          for (int c = 0; c < chunks; ++c) t = Elem<DT>::mma(b_operand<DT>(br, c, q, P.R), h_operand<DT>(hr, c, q, ds), t);
-          if (mine) acc[m][n] = t * us;
-        }
+      for (int n = 0; n < NI; ++n) {
+        const long long col = n0 + wn * TN + 16 * n + i;
+        br[n] = static_cast<const E*>(P.up) + ((long long)a * P.N + (col < P.N ? col : P.N - 1)) * P.R;
+      }
+      for (int c = 0; c < chunks; ++c) {
+        u32x4 bf[NI], hf[MI];
+#pragma unroll
+        for (int n = 0; n < NI; ++n) bf[n] = b_operand<DT>(br[n], c, q, P.R);
+#pragma unroll
+        for (int m = 0; m < MI; ++m) hf[m] = h_operand<DT>(hr[m], c, q, ds[m]);
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            const f32x4 t = Elem<DT>::mma(bf[n], hf[m], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[m][n][e] = mine[m] ? fmaf(t[e], us[m], acc[m][n][e]) : acc[m][n][e];
+          }
       }
     }
   }
 
   // ---- x W^T
-  const long long stages = (P.K + KB - 1) / KB;
-  put(0);
-  __syncthreads();
+  constexpr bool TWO = DT == ANERF_F32;
+  f32x4 sum[TWO ? MI : 1][TWO ? NI : 1];
+  if constexpr (TWO) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n) sum[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (!DIRECT) put(0);
   for (long long s = 0; s < stages; ++s) {
     const int buf = (int)(s & 1);
-    if (s + 1 < stages) fetch(s + 1);
+    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                         // stage s is in LDS, and every wave is done with the other buffer
+    if (s + 1 < stages) start(s + 1, buf ^ 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       u32x4 xf[MI], wf[NI];
 #pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const int r = wm * (BM / 2) + 16 * m + i;
-        xf[m] = lds[buf][r * 8 + ((4 * h + q) ^ (r & 7))];
+      for (int n = 0; n < NI; ++n) {
+        const int r = BM + wn * TN + 16 * n + i;
+        wf[n] = lds[buf * STAGE + r * 8 + ((4 * h + q) ^ (r & 7))];
       }
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int r = wn * (BN / 2) + 16 * n + i;
-        wf[n] = lds[buf][(BM + r) * 8 + ((4 * h + q) ^ (r & 7))];
+      for (int m = 0; m < MI; ++m) {
+        const int r = wm * TM + 16 * m + i;
+        xf[m] = lds[buf * STAGE + r * 8 + ((4 * h + q) ^ (r & 7))];
       }
 #pragma unroll
       for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] = Elem<DT>::mma(wf[n], xf[m], acc[m][n]);
     }
-    if (s + 1 < stages) put(buf ^ 1);
-    __syncthreads();
+    if constexpr (TWO) {
+      if (s % FOLD == FOLD - 1) {
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            sum[m][n] += acc[m][n];
+            acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+          }
+      }
+    }
+    if (!DIRECT && s + 1 < stages) put(buf ^ 1);
   }
 
   // ---- bias, rounding, store: lane (i, q) holds outputs 4q .. 4q+3 of its row in every 16x16 block
   const E* bias = static_cast<const E*>(P.bias);
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
-    const long long p = m0 + wm * (BM / 2) + 16 * m + i;
+    const long long p = m0 + wm * TM + 16 * m + i;
     if (p >= P.M) continue;
     E* yr = static_cast<E*>(P.y) + (P.order ? (long long)P.order[p] : p) * P.N;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
-      const long long col = n0 + wn * (BN / 2) + 16 * n + 4 * q;
+      const long long col = n0 + wn * TN + 16 * n + 4 * q;
       f32x4 v = acc[m][n];
+      if constexpr (TWO) v += sum[m][n];
       typedef E out4 __attribute__((ext_vector_type(4)));
       if (col + 4 <= P.N) {
         if (bias) {
@@ -400,7 +475,7 @@ __global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(const typename Elem
   }
 }
 
-// adds an adapter's pieces in their order, times s_i.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
+// adds an adapter's pieces, wave w those of q = w mod 4 in order, then the four sums; times s_i.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
 template <int DT, bool BY_RANK>
 __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__ part, const int32_t* __restrict__ offsets, int L, long long C, int R,
                                                        int Rp, int rows, const float* __restrict__ scale_of, float scale,
@@ -414,12 +489,20 @@ __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__
   const int n = (offsets[a + 1] - offsets[a] + rows - 1) / rows;
   const float s = scale_of ? scale * scale_of[a] : scale;
   const long long all = C * R, stride = C * Rp;
-  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
-    const float* src = part + first * stride + (BY_RANK ? e : e / R * Rp + e % R);
+  __shared__ float red[4][64];
+  const int w = threadIdx.x >> 6;
+  for (long long e0 = (long long)blockIdx.x * 64; e0 < all; e0 += (long long)gridDim.x * 64) {
+    const long long e = e0 + lane;
     float v = 0.f;
-#pragma unroll 8
-    for (int q = 0; q < n; ++q) v += src[q * stride];
-    out[(long long)a * all + e] = (E)(v * s);
+    if (e < all) {
+      const float* src = part + first * stride + (BY_RANK ? e : e / R * Rp + e % R);
+#pragma unroll 4
+      for (int q = w; q < n; q += 4) v += src[q * stride];
+    }
+    __syncthreads();
+    red[w][lane] = v;
+    __syncthreads();
+    if (w == 0 && e < all) out[(long long)a * all + e] = (E)((red[0][lane] + red[1][lane] + (red[2][lane] + red[3][lane])) * s);
   }
 }
 
@@ -452,6 +535,40 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- launchers
+template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
+static int run_main(const MainArgs& P, hipStream_t st) {
+  static unsigned long long done = 0;
+  constexpr int bytes = 2 * (BM + BN) * 128;
+  const auto kernel = k_main<DT, BM, BN, WM, WN, DIRECT>;
+  ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes, &done);
+  kernel<<<(unsigned)((P.M + BM - 1) / BM * ((P.N + BN - 1) / BN)), WM * WN * 64, bytes, st>>>(P);
+  return check_launch("k_main");
+}
+
+// Tile: the larger, the fewer LDS reads a product (a 256 x 256 tile's waves read 3/8 of what a 64 x 64 tile's do) and the fewer tiles
+// there are to fill 256 CUs with: the time is rounds of the chip x what a tile costs.
+template <int DT>
+static int launch_main(const MainArgs& P, hipStream_t st) {
+  const bool direct = (((uintptr_t)P.x | (uintptr_t)P.w) & 15) == 0 && P.K % Elem<DT>::EPC == 0 && P.ldx % Elem<DT>::EPC == 0;
+  auto cost = [&](int bm, int bn, int at_once, double rate) {     // CU rounds x relative time of what a CU holds at once
+    const double tiles = (double)((P.M + bm - 1) / bm) * (double)((P.N + bn - 1) / bn);
+    const double rounds = (double)(long long)((tiles + 256.0 * at_once - 1) / (256.0 * at_once));
+    const double share = tiles < 256.0 * at_once ? (tiles + 255) / 256 : at_once;      // tiles that the busiest CU runs side by side
+    return rounds * (double)(long long)share * bm * bn / rate;
+  };
+  const double c64 = cost(64, 64, 4, 0.5), c128 = cost(128, 128, 2, 0.75), cbig = DT == ANERF_F32 ? cost(128, 256, 1, 0.8) : cost(256, 256, 1, 1.0);
+  const double cmid = cost(256, 128, 1, 0.85);
+  if (!direct) return c64 < c128 ? run_main<DT, 64, 64, 2, 2, false>(P, st) : run_main<DT, 128, 128, 2, 2, false>(P, st);
+  if (cbig <= c64 && cbig <= c128 && (DT == ANERF_F32 || cbig <= cmid)) {
+    if constexpr (DT == ANERF_F32) return run_main<DT, 128, 256, 2, 4, true>(P, st);
+    else return run_main<DT, 256, 256, 2, 4, true>(P, st);
+  }
+  if constexpr (DT != ANERF_F32) {
+    if (cmid <= c64 && cmid <= c128) return run_main<DT, 256, 128, 4, 2, true>(P, st);
+  }
+  return c64 < c128 ? run_main<DT, 64, 64, 2, 2, true>(P, st) : run_main<DT, 128, 128, 2, 2, true>(P, st);
+}
+
 template <int DT>
 static int linear_t(const AnerfAdapterIO& A, hipStream_t st) {
   typedef typename Elem<DT>::T E;
@@ -470,15 +587,7 @@ static int linear_t(const AnerfAdapterIO& A, hipStream_t st) {
   if (rc || !A.y) return rc;       // (the gradient of A alone needs h only)
   MainArgs P = {A.x, A.weight, A.bias, A.up, A.scale_of, A.offsets, A.order, A.h, A.y, A.x_stride, A.n_in, A.n_out, A.n_rows, A.n_adapters,
                 A.rank, Rp, A.scale};
-  // 128 x 128 tiles read each operand half as often as 64 x 64 ones; below one workgroup a CU the smaller ones fill more of the chip
-  const long long big = (A.n_rows + 127) / 128 * ((A.n_out + 127) / 128);
-  if (big >= 256) {
-    k_main<DT, 128, 128><<<(unsigned)big, MN_THREADS, 0, st>>>(P);
-  } else {
-    const long long tiles = (A.n_rows + 63) / 64 * ((A.n_out + 63) / 64);
-    k_main<DT, 64, 64><<<(unsigned)tiles, MN_THREADS, 0, st>>>(P);
-  }
-  return check_launch("k_main");
+  return launch_main<DT>(P, st);
 }
 
 int launch_adapter_linear(const AnerfAdapterIO& A, hipStream_t st) {
@@ -539,7 +648,7 @@ static int thin_grad_t(const void* Z, long long ldz, const int32_t* order, const
     const int rc = check_launch("k_thin_grad");
     if (rc) return rc;
   }
-  const long long all = C * A.rank, bx = (all + 255) / 256;
+  const long long all = C * A.rank, bx = (all + 63) / 64;
   k_thin_grad_sum<DT, BY_RANK><<<dim3((unsigned)(bx < 4096 ? bx : 4096), A.n_adapters), 256, 0, st>>>(part, A.offsets, A.n_adapters, C, A.rank, Rp, rows,
                                                                                                    A.scale_of, A.scale, static_cast<E*>(out));
   return check_launch("k_thin_grad_sum");
