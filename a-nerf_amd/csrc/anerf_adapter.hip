@@ -17,6 +17,8 @@ namespace anerf {
 // piece in MFMA accumulators, fed straight from memory: a row of A serves 32 rows of x, and nothing is read twice from HBM.
 constexpr int TH_ROWS = 32, TH_WAVES = 4, TH_DEPTH = 4;
 template <int V> struct Const { static constexpr int value = V; };
+template <bool C, typename A, typename B> struct Pick { typedef A T; };
+template <typename A, typename B> struct Pick<false, A, B> { typedef B T; };
 
 template <int DT, int NJ>
 __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const int32_t* __restrict__ order,
@@ -61,7 +63,9 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int n = 0; n < NJ; ++n) acc[m][n] = Elem<DT>::mma(av[d][n], xv[d][m], acc[m][n]);
+        for (int n = 0; n < NJ; ++n)
+#pragma unroll
+          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(av[d][n], xv[d][m], acc[m][n], e);
   };
   long long s = wave;
   for (; s + (TH_DEPTH - 1) * TH_WAVES < steps; s += TH_DEPTH * TH_WAVES) walk(s, Const<TH_DEPTH>());
@@ -76,7 +80,9 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) acc[m][n] = Elem<DT>::mma(av[n], xv[m], acc[m][n]);
+      for (int n = 0; n < NJ; ++n)
+#pragma unroll
+        for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(av[n], xv[m], acc[m][n], e);
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -97,39 +103,39 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   }
 }
 
-// ------------------------------------------------------------------------------------------------- one h operand of the low-rank term
-// Lane (i, q) wants 16 bytes of its row's h against chunk c of B.  fp32: elements 16c + 4q ...  16-bit types: h is split into the
-// nearest value hi and the rest lo, [hi of 16 ranks | lo of the same 16] making one 32-wide step against [B | B], so that h keeps
-// 16 (bf16) or 21 (fp16) of its bits; fp16's range does not hold every h, so a row of h is first divided by a power of two.
-template <int DT>
-__device__ __forceinline__ u32x4 h_operand(const float* __restrict__ hr, int c, int q, float down_scale) {
+// ------------------------------------------------------------------------------------- operands of the low-rank term, 16 ranks a time
+// fp32: BS / 16 steps u of 64 / BS x 4 ranks.  16-bit types: h is split into the nearest value hi and the rest lo, and [hi of 16 ranks | lo of
+// the same 16] meets [B | B] -- one 32-wide step of 16 x 16 blocks, two 16-wide ones of 32 x 32 -- so that h keeps 16 (bf16) or 21 (fp16) of
+// its bits; fp16's range does not hold every h, so a row of h is first divided by a power of two.
+template <int DT, int BS>
+__device__ __forceinline__ int rank_of(int c, int u, int q) {
+  return 16 * c + (DT == ANERF_F32 ? 64 / BS * 4 * u + 4 * q : 8 * (q & 1));
+}
+
+template <int DT, int BS>
+__device__ __forceinline__ u32x4 h_operand(const float* __restrict__ hr, int c, int u, int q, float down_scale) {
+  const float* s = hr + rank_of<DT, BS>(c, u, q);
   if constexpr (DT == ANERF_F32) {
-    return __builtin_bit_cast(u32x4, *reinterpret_cast<const f32x4*>(hr + 16 * c + 4 * q));
+    return __builtin_bit_cast(u32x4, *reinterpret_cast<const f32x4*>(s));
   } else {
     typedef typename Elem<DT>::T E;
     typedef E vec __attribute__((ext_vector_type(8)));
+    const bool low = BS == 16 ? q >= 2 : u == 1;
     vec v;
-    const float* s = hr + 16 * c + 8 * (q & 1);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float f = DT == ANERF_F16 ? s[e] * down_scale : s[e];
       const E hi = (E)f;
       const float rest = f - (float)hi;
-      v[e] = q < 2 ? hi : (E)(__builtin_isfinite(f) && __builtin_isfinite((float)hi) ? rest : 0.f);
+      v[e] = !low ? hi : (E)(__builtin_isfinite(f) && __builtin_isfinite((float)hi) ? rest : 0.f);
     }
     return __builtin_bit_cast(u32x4, v);
   }
 }
 
-template <int DT>
-__device__ __forceinline__ u32x4 b_operand(const typename Elem<DT>::T* __restrict__ br, int c, int q, int R) {
-  const int j = 16 * c + (DT == ANERF_F32 ? 4 * q : 8 * (q & 1));
-  return load_tail<DT>(br, j, R);
-}
-
 // ------------------------------------------------------------------------------------------------------------------ y = x W^T ...
-// BM positions x BN outputs a workgroup of WM x WN waves, 16x16 MFMA blocks with W's rows as the first operand, so that a lane ends
-// with four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, double-buffered; 16-byte
+// BM positions x BN outputs a workgroup of WM x WN waves, BS x BS MFMA blocks with W's rows as the first operand, so that a lane ends
+// with groups of four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, double-buffered; 16-byte
 // chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.  DIRECT: global_load_lds_dwordx4, eight rows
 // an instruction, the lanes fetching the chunks in the order they have to lie in LDS (16-byte aligned rows); otherwise through registers,
 // at any alignment.
@@ -149,18 +155,20 @@ struct MainArgs {
   float scale;
 };
 
-constexpr int FOLD = 8;
+constexpr int FOLD = 16;
 
-template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
-__global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_main(MainArgs P) {
+template <int DT, int BS, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) k_main(MainArgs P) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, KB = 8 * EPC;        // elements of a 128-byte row piece
   constexpr int NW = WM * WN;
-  constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
+  constexpr int TM = BM / WM, TN = BN / WN, MI = TM / BS, NI = TN / BS;
+  constexpr int NV = BS * BS / 64, QB = 64 / BS;          // accumulators of a lane and block, lane groups of a step
+  typedef typename Block<BS>::Acc Acc;
   constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;       // 16-byte loads of a lane and stage
   constexpr int STAGE = (BM + BN) * 8;                    // 16-byte units
   extern __shared__ u32x4 lds[];                          // [2][STAGE]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane % BS, q = lane / BS;
   const int wm = wave % WM, wn = wave / WM;
   // workgroups go round-robin to the 8 XCDs: each XCD gets a contiguous range of the tile order, in which 4 row tiles share a column of W
   long long m0, n0;
@@ -172,42 +180,44 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_ma
     m0 = (4 * g + in % rows) * BM;
     n0 = in / rows * BN;
   }
-  const E* X = static_cast<const E*>(P.x);
-  const E* W = static_cast<const E*>(P.w);
-  // a lane's part of every stage: row r = 8 * (wave + NW * l) + lane / 8, the chunk that has to lie at position lane % 8
+  // a lane's part of every stage: row r = 8 * (wave + NW * l) + lane / 8, the chunk that has to lie at position lane % 8.  DIRECT: byte
+  // offsets of 32 bits against a scalar base that moves with the stage (a vector instruction in the fp32 loop costs matrix time)
   const int sub = lane >> 3, ch = (lane & 7) ^ sub;
-  const E* xrow[XL];
-  const E* wrow[WL];
+  typedef typename Pick<DIRECT, unsigned, long long>::T Off;
+  Off xo[XL], wo[WL];
 #pragma unroll
   for (int l = 0; l < XL; ++l) {
     long long p = m0 + 8 * (wave + NW * l) + sub;
     if (p >= P.M) p = P.M - 1;
-    xrow[l] = X + (P.order ? (long long)P.order[p] : p) * P.ldx + ch * EPC;
+    xo[l] = (Off)(((P.order ? (long long)P.order[p] : p) * P.ldx + ch * EPC) * (long long)sizeof(E));
   }
 #pragma unroll
   for (int l = 0; l < WL; ++l) {
     long long n = n0 + 8 * (wave + NW * l) + sub;
     if (n >= P.N) n = P.N - 1;
-    wrow[l] = W + n * P.K + ch * EPC;
+    wo[l] = (Off)((n * P.K + ch * EPC) * (long long)sizeof(E));
   }
   u32x4 rx[XL], rw[WL];
   auto at = [&](int buf, int row8) { return buf * STAGE + row8 * 64; };      // eight rows of 128 bytes
-  auto dma = [&](const E* src, int to) {
+  auto dma = [&](const void* base, unsigned off, int to) {
     const unsigned l = (unsigned)reinterpret_cast<size_t>((lds_ptr_t)(lds + to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(off), "s"(base) : "memory", "m0");
   };
-  auto fetch_regs = [&](long long s) {
-    const long long k = s * KB, left = P.K - k - ch * EPC;
+  const int K = (int)P.K;
+  auto fetch_regs = [&](int s) {
+    const int k = s * KB, left = K - k - ch * EPC;
+    const char* xb = static_cast<const char*>(P.x) + (long long)k * sizeof(E);
+    const char* wb = static_cast<const char*>(P.w) + (long long)k * sizeof(E);
     if (left >= EPC) {
 #pragma unroll
-      for (int l = 0; l < XL; ++l) rx[l] = load16(xrow[l] + k);
+      for (int l = 0; l < XL; ++l) rx[l] = load16(xb + xo[l]);
 #pragma unroll
-      for (int l = 0; l < WL; ++l) rw[l] = load16(wrow[l] + k);
+      for (int l = 0; l < WL; ++l) rw[l] = load16(wb + wo[l]);
     } else {
 #pragma unroll
-      for (int l = 0; l < XL; ++l) rx[l] = load_tail<DT>(xrow[l] + k, 0, left);
+      for (int l = 0; l < XL; ++l) rx[l] = load_tail<DT>(reinterpret_cast<const E*>(xb + xo[l]), 0, left);
 #pragma unroll
-      for (int l = 0; l < WL; ++l) rw[l] = load_tail<DT>(wrow[l] + k, 0, left);
+      for (int l = 0; l < WL; ++l) rw[l] = load_tail<DT>(reinterpret_cast<const E*>(wb + wo[l]), 0, left);
     }
   };
   auto put = [&](int buf) {
@@ -216,26 +226,28 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_ma
 #pragma unroll
     for (int l = 0; l < WL; ++l) lds[at(buf, BM / 8 + wave + NW * l) + lane] = rw[l];
   };
-  const long long stages = (P.K + KB - 1) / KB, full = P.K / KB;
-  // starts stage s; DIRECT: into LDS (the last, partial one through registers), otherwise into registers
-  auto start = [&](long long s, int buf) {
-    if (DIRECT && s < full) {
-      const long long k = s * KB;
+  const int stages = (K + KB - 1) / KB, full = K / KB;
+  // starts stage s; DIRECT: into LDS, otherwise into registers.  In a last, partial stage the chunks behind the row are not there: DIRECT
+  // lanes fetch the stage's first chunk in their place, and the products take zeros for them
+  auto start = [&](int s, int buf) {
+    if constexpr (DIRECT) {
+      const char* xb = static_cast<const char*>(P.x) + (long long)s * 128;
+      const char* wb = static_cast<const char*>(P.w) + (long long)s * 128;
+      const unsigned back = s < full || s * KB + ch * EPC < K ? 0u : ch * 16u;
 #pragma unroll
-      for (int l = 0; l < XL; ++l) dma(xrow[l] + k, at(buf, wave + NW * l));
+      for (int l = 0; l < XL; ++l) dma(xb, xo[l] - back, at(buf, wave + NW * l));
 #pragma unroll
-      for (int l = 0; l < WL; ++l) dma(wrow[l] + k, at(buf, BM / 8 + wave + NW * l));
+      for (int l = 0; l < WL; ++l) dma(wb, wo[l] - back, at(buf, BM / 8 + wave + NW * l));
     } else {
       fetch_regs(s);
-      if (DIRECT) put(buf);
     }
   };
   start(0, 0);
-  f32x4 acc[MI][NI];
+  Acc acc[MI][NI];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
 #pragma unroll
-    for (int n = 0; n < NI; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NI; ++n) acc[m][n] = Acc{};
 
   // ---- low-rank term
   long long tile_end = m0 + BM < P.M ? m0 + BM : P.M;
@@ -262,7 +274,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_ma
       float ds[MI], us[MI];
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
-        const long long p = m0 + wm * TM + 16 * m + i;
+        const long long p = m0 + wm * TM + BS * m + i;
         mine[m] = p >= a0 && p < a1;
         hr[m] = P.h + (mine[m] ? p : (long long)a0) * P.Rp;
         ds[m] = 1.f;
@@ -283,102 +295,161 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_ma
       const E* br[NI];
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const long long col = n0 + wn * TN + 16 * n + i;
+        const long long col = n0 + wn * TN + BS * n + i;
         br[n] = static_cast<const E*>(P.up) + ((long long)a * P.N + (col < P.N ? col : P.N - 1)) * P.R;
       }
       for (int c = 0; c < chunks; ++c) {
-        u32x4 bf[NI], hf[MI];
+        constexpr int US = BS / 16;
+        u32x4 bf[NI][US];
 #pragma unroll
-        for (int n = 0; n < NI; ++n) bf[n] = b_operand<DT>(br[n], c, q, P.R);
+        for (int n = 0; n < NI; ++n)
 #pragma unroll
-        for (int m = 0; m < MI; ++m) hf[m] = h_operand<DT>(hr[m], c, q, ds[m]);
+          for (int u = 0; u < US; ++u)
+            bf[n][u] = DT != ANERF_F32 && u ? bf[n][0] : load_tail<DT>(br[n], rank_of<DT, BS>(c, u, q), P.R);
 #pragma unroll
-        for (int m = 0; m < MI; ++m)
+        for (int m = 0; m < MI; ++m) {
+          u32x4 hf[US];
+#pragma unroll
+          for (int u = 0; u < US; ++u) hf[u] = h_operand<DT, BS>(hr[m], c, u, q, ds[m]);
 #pragma unroll
           for (int n = 0; n < NI; ++n) {
-            const f32x4 t = Elem<DT>::mma(bf[n], hf[m], f32x4{0.f, 0.f, 0.f, 0.f});
+            Acc t = Acc{};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][n][e] = mine[m] ? fmaf(t[e], us[m], acc[m][n][e]) : acc[m][n][e];
+            for (int u = 0; u < US; ++u)
+#pragma unroll
+              for (int e = 0; e < Elem<DT>::INSTR; ++e) t = Elem<DT>::template mma<BS>(bf[n][u], hf[u], t, e);
+#pragma unroll
+            for (int e = 0; e < NV; ++e) acc[m][n][e] = mine[m] ? fmaf(t[e], us[m], acc[m][n][e]) : acc[m][n][e];
           }
+        }
       }
     }
   }
 
   // ---- x W^T
   constexpr bool TWO = DT == ANERF_F32;
-  f32x4 sum[TWO ? MI : 1][TWO ? NI : 1];
+  Acc sum[TWO ? MI : 1][TWO ? NI : 1];
   if constexpr (TWO) {
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
-      for (int n = 0; n < NI; ++n) sum[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NI; ++n) sum[m][n] = Acc{};
   }
-  if (!DIRECT) put(0);
-  for (long long s = 0; s < stages; ++s) {
-    const int buf = (int)(s & 1);
+  // A half stage's rows of x are taken in two groups, and every group's fragments are read from LDS while the products of the group
+  // before it run (two sets of W's fragments, one of each group of x's), so that the matrix units need not wait for LDS.  The one barrier
+  // of a stage lies before its last group's products: there every wave has read the last of stage s, whose buffer stage s + 2 may then
+  // overwrite, and every wave's loads of stage s + 1 have arrived.
+  constexpr int MG = MI / 2;
+  static_assert(8 / QB == 2 && MI % 2 == 0, "two halves a stage, two groups a half");
+  u32x4 wf[2][NI], xf[2][MG];
+  // fragment addresses: row i of a block has r & 7 = i & 7, the halves' chunks differ in bit 2
+  const int px = (wm * TM + i) * 8, pw = (BM + wn * TN + i) * 8, c0 = q ^ (i & 7);
+  auto read_w = [&](int buf, int h) {
+    const u32x4* f = lds + buf * STAGE + pw + (c0 ^ (4 * h));
+#pragma unroll
+    for (int n = 0; n < NI; ++n) wf[h][n] = f[n * BS * 8];
+  };
+  auto read_x = [&](int buf, int h, int g) {
+    const u32x4* f = lds + buf * STAGE + px + (c0 ^ (4 * h));
+#pragma unroll
+    for (int m = 0; m < MG; ++m) xf[g][m] = f[(g * MG + m) * BS * 8];
+  };
+  auto products = [&](int h, int g) {
+#pragma unroll
+    for (int m = 0; m < MG; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[g * MG + m][n] = Elem<DT>::template mma<BS>(wf[h][n], xf[g][m], acc[g * MG + m][n], e);
+  };
+  auto arrive = [&]() {
     if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                         // stage s is in LDS, and every wave is done with the other buffer
-    if (s + 1 < stages) start(s + 1, buf ^ 1);
+    __syncthreads();
+  };
+  if (!DIRECT) put(0);
+  arrive();
+  if (stages > 1) start(1, 1);
+  read_w(0, 0);
+  read_x(0, 0, 0);
+  auto zero_behind = [&](u32x4* f, int n, int h) {      // fragments of the partial stage: chunks behind the row
+    const bool there = full * KB + (QB * h + q) * EPC < K;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 xf[MI], wf[NI];
-#pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const int r = BM + wn * TN + 16 * n + i;
-        wf[n] = lds[buf * STAGE + r * 8 + ((4 * h + q) ^ (r & 7))];
-      }
-#pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const int r = wm * TM + 16 * m + i;
-        xf[m] = lds[buf * STAGE + r * 8 + ((4 * h + q) ^ (r & 7))];
-      }
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NI; ++n) acc[m][n] = Elem<DT>::mma(wf[n], xf[m], acc[m][n]);
+    for (int e = 0; e < n; ++e) f[e] = there ? f[e] : u32x4{0, 0, 0, 0};
+  };
+  auto stage = [&](int s, int buf, auto partial) {
+    constexpr bool PART = decltype(partial)::value != 0;
+    read_x(buf, 0, 1);
+    if (PART) zero_behind(wf[0], NI, 0), zero_behind(xf[0], MG, 0), zero_behind(xf[1], MG, 0);
+    products(0, 0);
+    read_w(buf, 1);
+    read_x(buf, 1, 0);
+    if (PART) zero_behind(wf[1], NI, 1), zero_behind(xf[0], MG, 1);
+    products(0, 1);
+    read_x(buf, 1, 1);
+    if (PART) zero_behind(xf[1], MG, 1);
+    products(1, 0);
+    if (s + 1 < stages) {
+      if (!DIRECT) put(buf ^ 1);
+      arrive();
+      if (s + 2 < stages) start(s + 2, buf);
+      read_w(buf ^ 1, 0);
+      read_x(buf ^ 1, 0, 0);
     }
+    products(1, 1);
+  };
+  // the buffer is a constant of the loop's code: two stages a turn
+  const int whole = DIRECT ? full : stages;
+  for (int s = 0; s < whole; s += 2) {
+    stage(s, 0, Const<0>());
+    if (s + 1 < whole) stage(s + 1, 1, Const<0>());
     if constexpr (TWO) {
-      if (s % FOLD == FOLD - 1) {
+      if (s % FOLD == FOLD - 2) {
 #pragma unroll
         for (int m = 0; m < MI; ++m)
 #pragma unroll
           for (int n = 0; n < NI; ++n) {
             sum[m][n] += acc[m][n];
-            acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            acc[m][n] = Acc{};
           }
       }
     }
-    if (!DIRECT && s + 1 < stages) put(buf ^ 1);
   }
+  if (DIRECT && full < stages) stage(full, full & 1, Const<1>());
 
-  // ---- bias, rounding, store: lane (i, q) holds outputs 4q .. 4q+3 of its row in every 16x16 block
+  // ---- bias, rounding, store: lane (i, q) holds outputs 8g + 4q .. +3 of its row, a group g of four registers of every block
   const E* bias = static_cast<const E*>(P.bias);
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
-    const long long p = m0 + wm * TM + 16 * m + i;
+    const long long p = m0 + wm * TM + BS * m + i;
     if (p >= P.M) continue;
     E* yr = static_cast<E*>(P.y) + (P.order ? (long long)P.order[p] : p) * P.N;
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      const long long col = n0 + wn * TN + 16 * n + 4 * q;
-      f32x4 v = acc[m][n];
-      if constexpr (TWO) v += sum[m][n];
-      typedef E out4 __attribute__((ext_vector_type(4)));
-      if (col + 4 <= P.N) {
-        if (bias) {
+    for (int n = 0; n < NI; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += (float)bias[col + e];
+      for (int g = 0; g < NV / 4; ++g) {
+        const long long col = n0 + wn * TN + BS * n + 8 * g + 4 * q;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[m][n][4 * g + e];
+          if constexpr (TWO) v[e] += sum[m][n][4 * g + e];
         }
-        out4 o;
+        typedef E out4 __attribute__((ext_vector_type(4)));
+        if (col + 4 <= P.N) {
+          if (bias) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (E)v[e];
-        __builtin_memcpy(yr + col, &o, sizeof(o));
-      } else {
+            for (int e = 0; e < 4; ++e) v[e] += (float)bias[col + e];
+          }
+          out4 o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < P.N) yr[col + e] = (E)(bias ? v[e] + (float)bias[col + e] : v[e]);
+          for (int e = 0; e < 4; ++e) o[e] = (E)v[e];
+          __builtin_memcpy(yr + col, &o, sizeof(o));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < P.N) yr[col + e] = (E)(bias ? v[e] + (float)bias[col + e] : v[e]);
+        }
       }
-    }
   }
 }
 
@@ -539,7 +610,7 @@ template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
 static int run_main(const MainArgs& P, hipStream_t st) {
   static unsigned long long done = 0;
   constexpr int bytes = 2 * (BM + BN) * 128;
-  const auto kernel = k_main<DT, BM, BN, WM, WN, DIRECT>;
+  const auto kernel = k_main<DT, 16, BM, BN, WM, WN, DIRECT>;
   ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes, &done);
   kernel<<<(unsigned)((P.M + BM - 1) / BM * ((P.N + BN - 1) / BN)), WM * WN * 64, bytes, st>>>(P);
   return check_launch("k_main");
@@ -549,7 +620,8 @@ static int run_main(const MainArgs& P, hipStream_t st) {
 // there are to fill 256 CUs with: the time is rounds of the chip x what a tile costs.
 template <int DT>
 static int launch_main(const MainArgs& P, hipStream_t st) {
-  const bool direct = (((uintptr_t)P.x | (uintptr_t)P.w) & 15) == 0 && P.K % Elem<DT>::EPC == 0 && P.ldx % Elem<DT>::EPC == 0;
+  const bool direct = (((uintptr_t)P.x | (uintptr_t)P.w) & 15) == 0 && P.K % Elem<DT>::EPC == 0 && P.ldx % Elem<DT>::EPC == 0 &&
+                      P.M * P.ldx * (long long)sizeof(typename Elem<DT>::T) < (1ll << 32) && P.N * P.K * (long long)sizeof(typename Elem<DT>::T) < (1ll << 32);
   auto cost = [&](int bm, int bn, int at_once, double rate) {     // CU rounds x relative time of what a CU holds at once
     const double tiles = (double)((P.M + bm - 1) / bm) * (double)((P.N + bn - 1) / bn);
     const double rounds = (double)(long long)((tiles + 256.0 * at_once - 1) / (256.0 * at_once));
@@ -558,6 +630,15 @@ static int launch_main(const MainArgs& P, hipStream_t st) {
   };
   const double c64 = cost(64, 64, 4, 0.5), c128 = cost(128, 128, 2, 0.75), cbig = DT == ANERF_F32 ? cost(128, 256, 1, 0.8) : cost(256, 256, 1, 1.0);
   const double cmid = cost(256, 128, 1, 0.85);
+#ifdef EXP_BIG4
+  if constexpr (DT != ANERF_F32) { if (cbig <= cmid) return run_main<DT, 256, 256, 2, 2, true>(P, st); }
+#endif
+#ifdef EXP_TILE
+  if (EXP_TILE == 64) return run_main<DT, 64, 64, 2, 2, true>(P, st);
+  if (EXP_TILE == 128) return run_main<DT, 128, 128, 2, 2, true>(P, st);
+  if (EXP_TILE == 256) return run_main<DT, 128, 256, 2, 4, true>(P, st);
+  if (EXP_TILE == 12864) return run_main<DT, 128, 64, 2, 2, true>(P, st);
+#endif
   if (!direct) return c64 < c128 ? run_main<DT, 64, 64, 2, 2, false>(P, st) : run_main<DT, 128, 128, 2, 2, false>(P, st);
   if (cbig <= c64 && cbig <= c128 && (DT == ANERF_F32 || cbig <= cmid)) {
     if constexpr (DT == ANERF_F32) return run_main<DT, 128, 256, 2, 4, true>(P, st);
