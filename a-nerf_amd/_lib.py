@@ -217,6 +217,7 @@ SIGNATURES = {
                                      C.c_void_p]),
     "anerf_combine_rows_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                               C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "anerf_adapter_h_size": (C.c_int64, [C.POINTER(AnerfAdapterIO)]),
     "anerf_adapter_linear": (C.c_int, [C.POINTER(AnerfAdapterIO), C.c_void_p]),
     "anerf_adapter_backward_workspace_size": (C.c_int64, [C.POINTER(AnerfAdapterIO)]),
     "anerf_adapter_backward": (C.c_int, [C.POINTER(AnerfAdapterIO), C.POINTER(AnerfAdapterGradIO), C.c_void_p, C.c_int64, C.c_void_p]),

@@ -1,10 +1,10 @@
 // anerf_adapter.hip -- a shared projection with a low-rank adapter of its own for every row (gfx950):
 //     y[r] = x[r] W^T + b + s_i (x[r] A_i^T) B_i^T          i = the row's adapter, none: the shared projection alone
 // and its gradients with W and b frozen:
-//     u[r] = g[r] B_i,  dx = g W + s_i u A_i,  dA_i = s_i sum_r u[r]^T x[r],  dB_i = s_i sum_r g[r]^T h[r],  h[r] = x[r] A_i^T
+//     h[r] = s_i x[r] A_i^T,  u[r] = s_i g[r] B_i,  dx = g W + u A_i,  dA_i = sum_r u[r]^T x[r],  dB_i = sum_r g[r]^T h[r]
 // Rows are walked in the order of their adapter (positions p; order[p] = row, NULL = rows lie in that order already), adapter i
 // owning positions offsets[i] .. offsets[i+1]-1; the rows behind offsets[L] have no adapter.
-//   k_thin       h[p] = x[order[p]] A_i^T: one workgroup a piece of 32 positions of one adapter
+//   k_thin       h[p] = s_i x[order[p]] A_i^T: one workgroup a piece of 32 positions of one adapter
 //   k_main       x W^T tile by tile; a tile starts with the low-rank term of the adapters whose positions it holds
 //   k_thin_grad  dA_i / dB_i as sums over pieces of an adapter's positions, k_thin_grad_sum adds the pieces in order
 //   k_transpose  W, A, B with their last two axes swapped: dx is then the forward product of (g, W^T, B^T, A^T)
@@ -12,9 +12,24 @@
 
 namespace anerf {
 
-// ---------------------------------------------------------------------------------------------------------------- h = x A^T
+// ------------------------------------------------------------------------------------------------------------ h = s_i x A_i^T
 // HBM-bound on x.  The four waves split the contraction (every fourth 64-byte step), each holding all 32 rows x 16*NJ ranks of the
 // piece in MFMA accumulators, fed straight from memory: a row of A serves 32 rows of x, and nothing is read twice from HBM.
+// Kept as [position][Rp] fp32 (Rp = rank rounded up to 16, zeros behind the rank) for the gradient of B, and, for the 16-bit types, as what
+// k_main multiplies with: the nearest value hi and the rest lo, [hi of 16 ranks | lo of the same 16] per 16 ranks, which meet [B | B]
+// there -- h keeps 16 (bf16) or 21 (fp16) of its bits.  fp16's range does not hold every h: k_split_rows scales its rows first.
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+template <typename E, typename V4>
+__device__ __forceinline__ void split4(f32x4 v, V4& hi, V4& lo) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = (E)v[e];
+    const float rest = v[e] - (float)hi[e];
+    lo[e] = __builtin_isfinite((float)hi[e]) ? (E)rest : (E)0.f;       // (infinity and NaN are carried by hi alone)
+  }
+}
+
 constexpr int TH_ROWS = 32, TH_WAVES = 4, TH_DEPTH = 4;
 template <int V> struct Const { static constexpr int value = V; };
 template <bool C, typename A, typename B> struct Pick { typedef A T; };
@@ -23,7 +38,8 @@ template <typename A, typename B> struct Pick<false, A, B> { typedef B T; };
 template <int DT, int NJ>
 __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const int32_t* __restrict__ order,
                                                         const typename Elem<DT>::T* __restrict__ down, const int32_t* __restrict__ offsets,
-                                                        int L, long long K, int R, int Rp, float* __restrict__ h) {
+                                                        int L, long long K, int R, int Rp, const float* __restrict__ scale_of, float scale,
+                                                        float* __restrict__ h, typename Elem<DT>::T* __restrict__ split) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
   __shared__ f32x4 red[TH_WAVES][2 * NJ][64];
@@ -31,6 +47,7 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   if (!find_piece(offsets, L, TH_ROWS, blockIdx.x, a, p0, p1)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
   const int j0 = blockIdx.y * 16 * NJ;
+  const float s_a = scale_of ? scale * scale_of[a] : scale;
   const E* A = down + (long long)a * R * K;
   const E* xr[2];
   const E* ar[NJ];
@@ -96,40 +113,40 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
     const int p = p0 + 16 * (f / NJ) + i, j = j0 + 16 * (f % NJ) + 4 * q;
     if (p < p1 && j < Rp) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e >= R) v[e] = 0.f;                   // ranks of the padding: zero
+      for (int e = 0; e < 4; ++e) v[e] = j + e < R ? v[e] * s_a : 0.f;      // ranks of the padding: zero
       *reinterpret_cast<f32x4*>(h + (long long)p * Rp + j) = v;
+      if constexpr (DT == ANERF_BF16) {
+        bf16x4 hi, lo;
+        split4<E, bf16x4>(v, hi, lo);
+        E* o = split + (long long)p * 2 * Rp + 2 * (j & ~15) + (j & 15);
+        *reinterpret_cast<bf16x4*>(o) = hi;
+        *reinterpret_cast<bf16x4*>(o + 16) = lo;
+      }
     }
   }
 }
 
-// ------------------------------------------------------------------------------------- operands of the low-rank term, 16 ranks a time
-// fp32: BS / 16 steps u of 64 / BS x 4 ranks.  16-bit types: h is split into the nearest value hi and the rest lo, and [hi of 16 ranks | lo of
-// the same 16] meets [B | B] -- one 32-wide step of 16 x 16 blocks, two 16-wide ones of 32 x 32 -- so that h keeps 16 (bf16) or 21 (fp16) of
-// its bits; fp16's range does not hold every h, so a row of h is first divided by a power of two.
-template <int DT, int BS>
-__device__ __forceinline__ int rank_of(int c, int u, int q) {
-  return 16 * c + (DT == ANERF_F32 ? 64 / BS * 4 * u + 4 * q : 8 * (q & 1));
-}
-
-template <int DT, int BS>
-__device__ __forceinline__ u32x4 h_operand(const float* __restrict__ hr, int c, int u, int q, float down_scale) {
-  const float* s = hr + rank_of<DT, BS>(c, u, q);
-  if constexpr (DT == ANERF_F32) {
-    return __builtin_bit_cast(u32x4, *reinterpret_cast<const f32x4*>(s));
-  } else {
-    typedef typename Elem<DT>::T E;
-    typedef E vec __attribute__((ext_vector_type(8)));
-    const bool low = BS == 16 ? q >= 2 : u == 1;
-    vec v;
+// fp16: a row of h is divided by the power of two that brings its largest value into [1, 2) before it is split
+__global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h, const int32_t* __restrict__ kept, int Rp, _Float16* __restrict__ split,
+                                                    float* __restrict__ factor) {
+  const int p = blockIdx.x * 16 + (threadIdx.x >> 4), i = threadIdx.x & 15;
+  if (p >= *kept) return;
+  const float* r = h + (long long)p * Rp;
+  float big = 0.f;
+  for (int j = i; j < Rp; j += 16) big = fmaxf(big, fabsf(r[j]));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float f = DT == ANERF_F16 ? s[e] * down_scale : s[e];
-      const E hi = (E)f;
-      const float rest = f - (float)hi;
-      v[e] = !low ? hi : (E)(__builtin_isfinite(f) && __builtin_isfinite((float)hi) ? rest : 0.f);
-    }
-    return __builtin_bit_cast(u32x4, v);
+  for (int d = 8; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d));
+  int e = 0;
+  if (big > 0.f && __builtin_isfinite(big)) e = min(max(ilogbf(big), -100), 100);
+  if (i == 0) factor[p] = ldexpf(1.f, e);
+  const float down = ldexpf(1.f, -e);
+  for (int j = 4 * i; j < Rp; j += 64) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(r + j) * down;
+    f16x4 hi, lo;
+    split4<_Float16, f16x4>(v, hi, lo);
+    _Float16* o = split + (long long)p * 2 * Rp + 2 * (j & ~15) + (j & 15);
+    *reinterpret_cast<f16x4*>(o) = hi;
+    *reinterpret_cast<f16x4*>(o + 16) = lo;
   }
 }
 
@@ -139,20 +156,19 @@ __device__ __forceinline__ u32x4 h_operand(const float* __restrict__ hr, int c, 
 // chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.  DIRECT: global_load_lds_dwordx4, eight rows
 // an instruction, the lanes fetching the chunks in the order they have to lie in LDS (16-byte aligned rows); otherwise through registers,
 // at any alignment.
-// The low-rank term comes first, behind the first stage's loads: for every adapter with positions in the tile h B_i^T is formed from
-// zero and added to that adapter's rows alone (a NaN in one adapter stays with its rows), times s_i in fp32.
+// The low-rank term comes first, behind the first stage's loads: for every adapter with positions in the tile h B_i^T is added to the
+// blocks of its rows; a block that two adapters share takes it by row (a NaN in one adapter stays with its rows).
 // fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set, so that no chain of
 // additions is longer than 8 * FOLD + K / (32 * FOLD).
 struct MainArgs {
   const void *x, *w, *bias, *up;
-  const float* scale_of;       // per adapter, or NULL
   const int32_t *offsets, *order;
-  const float* h;
+  const void* h;               // operand form of h: [M][Rp] fp32, [M][2 Rp] 16-bit
+  const float* factor;         // fp16: power of two of every row of h
   void* y;
   long long ldx, K, N;
   long long M;
   int L, R, Rp;
-  float scale;
 };
 
 constexpr int FOLD = 16;
@@ -168,7 +184,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;       // 16-byte loads of a lane and stage
   constexpr int STAGE = (BM + BN) * 8;                    // 16-byte units
   extern __shared__ u32x4 lds[];                          // [2][STAGE]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane % BS, q = lane / BS;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane % BS, q = lane / BS;
   const int wm = wave % WM, wn = wave / WM;
   // workgroups go round-robin to the 8 XCDs: each XCD gets a contiguous range of the tile order, in which 4 row tiles share a column of W
   long long m0, n0;
@@ -199,9 +215,9 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   }
   u32x4 rx[XL], rw[WL];
   auto at = [&](int buf, int row8) { return buf * STAGE + row8 * 64; };      // eight rows of 128 bytes
-  auto dma = [&](const void* base, unsigned off, int to) {
-    const unsigned l = (unsigned)reinterpret_cast<size_t>((lds_ptr_t)(lds + to));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(off), "s"(base) : "memory", "m0");
+  const unsigned lds0 = (unsigned)reinterpret_cast<size_t>((lds_ptr_t)lds) + wave * 1024;
+  auto dma = [&](const void* base, unsigned off, int to) {                   // `to`: 16-byte units behind the wave's eight rows
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + to * 16), "v"(off), "s"(base) : "memory", "m0");
   };
   const int K = (int)P.K;
   auto fetch_regs = [&](int s) {
@@ -233,11 +249,18 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     if constexpr (DIRECT) {
       const char* xb = static_cast<const char*>(P.x) + (long long)s * 128;
       const char* wb = static_cast<const char*>(P.w) + (long long)s * 128;
-      const unsigned back = s < full || s * KB + ch * EPC < K ? 0u : ch * 16u;
+      if (s < full) {
 #pragma unroll
-      for (int l = 0; l < XL; ++l) dma(xb, xo[l] - back, at(buf, wave + NW * l));
+        for (int l = 0; l < XL; ++l) dma(xb, xo[l], at(buf, NW * l));
 #pragma unroll
-      for (int l = 0; l < WL; ++l) dma(wb, wo[l] - back, at(buf, BM / 8 + wave + NW * l));
+        for (int l = 0; l < WL; ++l) dma(wb, wo[l], at(buf, BM / 8 + NW * l));
+      } else {
+        const unsigned back = s * KB + ch * EPC < K ? 0u : ch * 16u;
+#pragma unroll
+        for (int l = 0; l < XL; ++l) dma(xb, xo[l] - back, at(buf, NW * l));
+#pragma unroll
+        for (int l = 0; l < WL; ++l) dma(wb, wo[l] - back, at(buf, BM / 8 + NW * l));
+      }
     } else {
       fetch_regs(s);
     }
@@ -250,78 +273,66 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     for (int n = 0; n < NI; ++n) acc[m][n] = Acc{};
 
   // ---- low-rank term
-  long long tile_end = m0 + BM < P.M ? m0 + BM : P.M;
   const int kept = P.offsets[P.L];
   if (m0 < kept) {
-    if (tile_end > kept) tile_end = kept;
-    int first = 0;                           // first adapter that ends behind m0, 64 at a time
-    for (int a0 = 0; a0 < P.L; a0 += 64) {
-      const int a = a0 + lane;
-      const unsigned long long past = __ballot(a < P.L && P.offsets[a < P.L ? a + 1 : 0] > m0);
-      if (past) {
-        first = a0 + __builtin_ctzll(past);
-        break;
+    const int t0 = (int)m0, t1 = min((int)(m0 + BM < P.M ? m0 + BM : P.M), kept);
+    const int w0 = t0 + wm * TM;                               // the wave's first position and output
+    const long long c0 = n0 + wn * TN;
+    const int last_col = (int)(P.N - 1 - c0 < TN ? P.N - 1 - c0 : TN);
+    const int chunks = P.Rp / 16, row_bytes = P.Rp * 4;        // (two 16-bit values or one fp32 a rank)
+    const char* hw = static_cast<const char*>(P.h) + (long long)w0 * row_bytes + 16 * q;
+    // the adapters 64 at a time; those that own positions of the tile
+    for (int b0 = 0; b0 < P.L; b0 += 64) {
+      const int ab = b0 + lane;
+      const int lo = ab < P.L ? P.offsets[ab] : 0, hi = ab < P.L ? P.offsets[ab + 1] : 0;
+      unsigned long long owners = __ballot(hi > lo && hi > t0 && lo < t1);
+      while (owners) {
+        const int l = __builtin_ctzll(owners);
+        owners &= owners - 1;
+        const int r0 = max(__builtin_amdgcn_readlane(lo, l) - w0, 0), r1 = min(__builtin_amdgcn_readlane(hi, l) - w0, TM);
+        if (r0 >= r1) continue;                                // none of this wave's
+        const E* bw = static_cast<const E*>(P.up) + ((long long)(b0 + l) * P.N + c0) * P.R;
+        for (int c = 0; c < chunks; ++c) {
+          const int j = 16 * c + (DT == ANERF_F32 ? 4 * q : 8 * (q & 1));
+          u32x4 bf[NI], hf[MI];
+#pragma unroll
+          for (int n = 0; n < NI; ++n) bf[n] = load_tail<DT>(bw + min(BS * n + i, last_col) * P.R, j, P.R);
+#pragma unroll
+          for (int m = 0; m < MI; ++m) {
+            const int r = min(max(BS * m + i, r0), r1 - 1);
+            hf[m] = *reinterpret_cast<const u32x4*>(hw + r * row_bytes + 64 * c);
+          }
+#pragma unroll
+          for (int m = 0; m < MI; ++m) {
+            if (BS * m >= r1 || BS * m + BS <= r0) continue;
+            if (BS * m >= r0 && BS * m + BS <= r1) {
+#pragma unroll
+              for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<BS>(bf[n], hf[m], acc[m][n], e);
+            } else {
+              const bool mine = BS * m + i >= r0 && BS * m + i < r1;
+#pragma unroll
+              for (int n = 0; n < NI; ++n) {
+                Acc t = Acc{};
+#pragma unroll
+                for (int e = 0; e < Elem<DT>::INSTR; ++e) t = Elem<DT>::template mma<BS>(bf[n], hf[m], t, e);
+#pragma unroll
+                for (int e = 0; e < NV; ++e) acc[m][n][e] = mine ? acc[m][n][e] + t[e] : acc[m][n][e];
+              }
+            }
+          }
+        }
       }
+      if (__builtin_amdgcn_readlane(hi, 63) >= t1) break;
     }
-    const int chunks = P.Rp / 16;
-    for (int a = first; a < P.L; ++a) {
-      const int a0 = P.offsets[a], a1 = P.offsets[a + 1];
-      if (a0 >= tile_end) break;
-      if (a1 <= a0) continue;
-      const float s = P.scale_of ? P.scale * P.scale_of[a] : P.scale;
-      bool mine[MI];
-      const float* hr[MI];
-      float ds[MI], us[MI];
+    if constexpr (DT == ANERF_F16) {
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
-        const long long p = m0 + wm * TM + BS * m + i;
-        mine[m] = p >= a0 && p < a1;
-        hr[m] = P.h + (mine[m] ? p : (long long)a0) * P.Rp;
-        ds[m] = 1.f;
-        us[m] = s;
-        if constexpr (DT == ANERF_F16) {     // largest |h| of the row -> [1, 2)
-          float big = 0.f;
-          for (int j = 0; j < P.Rp; j += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(hr[m] + j);
-            big = fmaxf(fmaxf(big, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
-          }
-          if (big > 0.f && __builtin_isfinite(big)) {
-            const int e = min(max(ilogbf(big), -100), 100);
-            ds[m] = ldexpf(1.f, -e);
-            us[m] = s * ldexpf(1.f, e);
-          }
-        }
-      }
-      const E* br[NI];
+        const int p = w0 + BS * m + i;
+        const float f = p < kept ? P.factor[p] : 1.f;
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const long long col = n0 + wn * TN + BS * n + i;
-        br[n] = static_cast<const E*>(P.up) + ((long long)a * P.N + (col < P.N ? col : P.N - 1)) * P.R;
-      }
-      for (int c = 0; c < chunks; ++c) {
-        constexpr int US = BS / 16;
-        u32x4 bf[NI][US];
-#pragma unroll
-        for (int n = 0; n < NI; ++n)
-#pragma unroll
-          for (int u = 0; u < US; ++u)
-            bf[n][u] = DT != ANERF_F32 && u ? bf[n][0] : load_tail<DT>(br[n], rank_of<DT, BS>(c, u, q), P.R);
-#pragma unroll
-        for (int m = 0; m < MI; ++m) {
-          u32x4 hf[US];
-#pragma unroll
-          for (int u = 0; u < US; ++u) hf[u] = h_operand<DT, BS>(hr[m], c, u, q, ds[m]);
-#pragma unroll
-          for (int n = 0; n < NI; ++n) {
-            Acc t = Acc{};
-#pragma unroll
-            for (int u = 0; u < US; ++u)
-#pragma unroll
-              for (int e = 0; e < Elem<DT>::INSTR; ++e) t = Elem<DT>::template mma<BS>(bf[n][u], hf[u], t, e);
-#pragma unroll
-            for (int e = 0; e < NV; ++e) acc[m][n][e] = mine[m] ? fmaf(t[e], us[m], acc[m][n][e]) : acc[m][n][e];
-          }
-        }
+        for (int n = 0; n < NI; ++n) acc[m][n] *= f;
       }
     }
   }
@@ -343,14 +354,14 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   static_assert(8 / QB == 2 && MI % 2 == 0, "two halves a stage, two groups a half");
   u32x4 wf[2][NI], xf[2][MG];
   // fragment addresses: row i of a block has r & 7 = i & 7, the halves' chunks differ in bit 2
-  const int px = (wm * TM + i) * 8, pw = (BM + wn * TN + i) * 8, c0 = q ^ (i & 7);
+  const int px = (wm * TM + i) * 8, pw = (BM + wn * TN + i) * 8, ch0 = q ^ (i & 7);
   auto read_w = [&](int buf, int h) {
-    const u32x4* f = lds + buf * STAGE + pw + (c0 ^ (4 * h));
+    const u32x4* f = lds + buf * STAGE + pw + (ch0 ^ (4 * h));
 #pragma unroll
     for (int n = 0; n < NI; ++n) wf[h][n] = f[n * BS * 8];
   };
   auto read_x = [&](int buf, int h, int g) {
-    const u32x4* f = lds + buf * STAGE + px + (c0 ^ (4 * h));
+    const u32x4* f = lds + buf * STAGE + px + (ch0 ^ (4 * h));
 #pragma unroll
     for (int m = 0; m < MG; ++m) xf[g][m] = f[(g * MG + m) * BS * 8];
   };
@@ -546,11 +557,10 @@ __global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(const typename Elem
   }
 }
 
-// adds an adapter's pieces, wave w those of q = w mod 4 in order, then the four sums; times s_i.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
+// adds an adapter's pieces, wave w those of q = w mod 4 in order, then the four sums.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
 template <int DT, bool BY_RANK>
 __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__ part, const int32_t* __restrict__ offsets, int L, long long C, int R,
-                                                       int Rp, int rows, const float* __restrict__ scale_of, float scale,
-                                                       typename Elem<DT>::T* __restrict__ out) {
+                                                       int Rp, int rows, typename Elem<DT>::T* __restrict__ out) {
   typedef typename Elem<DT>::T E;
   const int a = blockIdx.y, lane = threadIdx.x & 63;
   int first = 0;
@@ -558,7 +568,6 @@ __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__
 #pragma unroll
   for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
   const int n = (offsets[a + 1] - offsets[a] + rows - 1) / rows;
-  const float s = scale_of ? scale * scale_of[a] : scale;
   const long long all = C * R, stride = C * Rp;
   __shared__ float red[4][64];
   const int w = threadIdx.x >> 6;
@@ -573,7 +582,7 @@ __global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__
     __syncthreads();
     red[w][lane] = v;
     __syncthreads();
-    if (w == 0 && e < all) out[(long long)a * all + e] = (E)((red[0][lane] + red[1][lane] + (red[2][lane] + red[3][lane])) * s);
+    if (w == 0 && e < all) out[(long long)a * all + e] = (E)(red[0][lane] + red[1][lane] + (red[2][lane] + red[3][lane]));
   }
 }
 
@@ -630,9 +639,6 @@ static int launch_main(const MainArgs& P, hipStream_t st) {
   };
   const double c64 = cost(64, 64, 4, 0.5), c128 = cost(128, 128, 2, 0.75), cbig = DT == ANERF_F32 ? cost(128, 256, 1, 0.8) : cost(256, 256, 1, 1.0);
   const double cmid = cost(256, 128, 1, 0.85);
-#ifdef EXP_BIG4
-  if constexpr (DT != ANERF_F32) { if (cbig <= cmid) return run_main<DT, 256, 256, 2, 2, true>(P, st); }
-#endif
 #ifdef EXP_TILE
   if (EXP_TILE == 64) return run_main<DT, 64, 64, 2, 2, true>(P, st);
   if (EXP_TILE == 128) return run_main<DT, 128, 128, 2, 2, true>(P, st);
@@ -650,24 +656,46 @@ static int launch_main(const MainArgs& P, hipStream_t st) {
   return c64 < c128 ? run_main<DT, 64, 64, 2, 2, true>(P, st) : run_main<DT, 128, 128, 2, 2, true>(P, st);
 }
 
+// what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][2 Rp] (16-bit types) | factor [n_rows] (fp16); byte offsets
+struct HLayout {
+  int Rp;
+  long long split, factor, bytes;
+};
+static HLayout h_layout(const AnerfAdapterIO& A) {
+  HLayout H;
+  H.Rp = (A.rank + 15) / 16 * 16;
+  const long long part = A.n_rows * H.Rp * 4;
+  H.split = part;
+  H.factor = A.dtype == ANERF_F32 ? part : 2 * part;
+  H.bytes = H.factor + (A.dtype == ANERF_F16 ? (A.n_rows + 3) / 4 * 16 : 0);
+  return H;
+}
+long long adapter_h_bytes(const AnerfAdapterIO& A) { return h_layout(A).bytes; }
+
 template <int DT>
 static int linear_t(const AnerfAdapterIO& A, hipStream_t st) {
   typedef typename Elem<DT>::T E;
-  const int Rp = (A.rank + 15) / 16 * 16;
+  const HLayout H = h_layout(A);
   const long long pieces = pieces_bound(A.n_rows, A.n_adapters, TH_ROWS);
-  const E* x = static_cast<const E*>(A.x);
-  const E* down = static_cast<const E*>(A.down);
-  if (Rp <= 16)
-    k_thin<DT, 1><<<dim3((unsigned)pieces, 1), TH_WAVES * 64, 0, st>>>(x, A.x_stride, A.order, down, A.offsets, A.n_adapters, A.n_in, A.rank, Rp, A.h);
-  else if (Rp <= 32)
-    k_thin<DT, 2><<<dim3((unsigned)pieces, 1), TH_WAVES * 64, 0, st>>>(x, A.x_stride, A.order, down, A.offsets, A.n_adapters, A.n_in, A.rank, Rp, A.h);
-  else
-    k_thin<DT, 4><<<dim3((unsigned)pieces, (Rp + 63) / 64), TH_WAVES * 64, 0, st>>>(x, A.x_stride, A.order, down, A.offsets, A.n_adapters, A.n_in,
-                                                                                     A.rank, Rp, A.h);
-  int rc = check_launch("k_thin");
+  const int Rp = H.Rp;
+  float* h = reinterpret_cast<float*>(A.h);
+  E* split = reinterpret_cast<E*>(static_cast<char*>(A.h) + H.split);
+  float* factor = reinterpret_cast<float*>(static_cast<char*>(A.h) + H.factor);
+  auto thin = [&](auto kernel, int parts) {
+    kernel<<<dim3((unsigned)pieces, parts), TH_WAVES * 64, 0, st>>>(static_cast<const E*>(A.x), A.x_stride, A.order, static_cast<const E*>(A.down), A.offsets,
+                                                                  A.n_adapters, A.n_in, A.rank, Rp, A.scale_of, A.scale, h, split);
+  };
+  if (Rp <= 16) thin(k_thin<DT, 1>, 1);
+  else if (Rp <= 32) thin(k_thin<DT, 2>, 1);
+  else thin(k_thin<DT, 4>, (Rp + 63) / 64);
+  if constexpr (DT == ANERF_F16) {
+    if (A.y) k_split_rows<<<(unsigned)((A.n_rows + 15) / 16), 256, 0, st>>>(h, A.offsets + A.n_adapters, Rp, split, factor);
+  }
+  const int rc = check_launch("k_thin");
   if (rc || !A.y) return rc;       // (the gradient of A alone needs h only)
-  MainArgs P = {A.x, A.weight, A.bias, A.up, A.scale_of, A.offsets, A.order, A.h, A.y, A.x_stride, A.n_in, A.n_out, A.n_rows, A.n_adapters,
-                A.rank, Rp, A.scale};
+  const void* operand = split;
+  if constexpr (DT == ANERF_F32) operand = h;
+  const MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, A.y, A.x_stride, A.n_in, A.n_out, A.n_rows, A.n_adapters, A.rank, Rp};
   return launch_main<DT>(P, st);
 }
 
@@ -705,7 +733,7 @@ static BackwardPlan backward_plan(const AnerfAdapterIO& A) {
   B.wt = at, at += up16(A.n_in * A.n_out * es);
   B.dt = at, at += up16((long long)A.n_adapters * A.rank * A.n_in * es);
   B.ut = at, at += up16((long long)A.n_adapters * A.rank * A.n_out * es);
-  B.u = at, at += up16(A.n_rows * Rp * 4);
+  B.u = at, at += up16(h_layout(A).bytes);
   const long long pa = part_floats(A.n_rows, A.n_adapters, A.n_in, Rp), pb = part_floats(A.n_rows, A.n_adapters, A.n_out, Rp);
   B.part = at, at += up16((pa > pb ? pa : pb) * 4);
   B.bytes = at;
@@ -731,7 +759,7 @@ static int thin_grad_t(const void* Z, long long ldz, const int32_t* order, const
   }
   const long long all = C * A.rank, bx = (all + 63) / 64;
   k_thin_grad_sum<DT, BY_RANK><<<dim3((unsigned)(bx < 4096 ? bx : 4096), A.n_adapters), 256, 0, st>>>(part, A.offsets, A.n_adapters, C, A.rank, Rp, rows,
-                                                                                                   A.scale_of, A.scale, static_cast<E*>(out));
+                                                                                                   static_cast<E*>(out));
   return check_launch("k_thin_grad_sum");
 }
 
@@ -759,7 +787,7 @@ static int backward_t(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, char
     if (rc) return rc;
     AnerfAdapterIO T = A;
     T.x = G.g, T.x_stride = G.g_stride, T.weight = ws + B.wt, T.bias = nullptr, T.down = ws + B.ut, T.up = ws + B.dt;
-    T.n_in = A.n_out, T.n_out = A.n_in, T.y = G.dx, T.h = u;
+    T.n_in = A.n_out, T.n_out = A.n_in, T.y = G.dx, T.h = ws + B.u;
     rc = linear_t<DT>(T, st);
     if (rc) return rc;
   }
@@ -768,7 +796,7 @@ static int backward_t(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, char
     if (rc) return rc;
   }
   if (G.dup) {
-    const int rc = thin_grad_t<DT, false>(G.g, G.g_stride, A.order, A.h, A, A.n_out, part, G.dup, st);
+    const int rc = thin_grad_t<DT, false>(G.g, G.g_stride, A.order, static_cast<const float*>(A.h), A, A.n_out, part, G.dup, st);
     if (rc) return rc;
   }
   return ANERF_OK;

@@ -80,6 +80,7 @@ int launch_route(const void* idx, int wide, long long n, int G, int32_t* offsets
 int launch_rows(int op, int dtype, const void* a, const void* b, const float* w, const int32_t* slot, const int32_t* end, long long T, int k,
                 long long D, void* out, float* dw, hipStream_t st);
 int launch_adapter_linear(const AnerfAdapterIO& A, hipStream_t st);
+long long adapter_h_bytes(const AnerfAdapterIO& A);
 long long adapter_backward_workspace(const AnerfAdapterIO& A);
 int launch_adapter_backward(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, void* ws, hipStream_t st);
 int launch_code_reduce(const float* du, int uw, const float* cam, int n, int S, int n_codes, float* rowsum, float* dcodes,
@@ -1331,6 +1332,11 @@ static int adapter_check(const AnerfAdapterIO* a) {
   if (((a->n_rows + 63) / 64) * ((a->n_out + 63) / 64) >= lim || ((a->n_rows + 63) / 64) * ((a->n_in + 63) / 64) >= lim)
     return set_error(ANERF_E_SHAPE, "adapter: too many output tiles for one launch");
   return ANERF_OK;
+}
+
+int64_t anerf_adapter_h_size(const AnerfAdapterIO* a) {
+  const int rc = adapter_check(a);
+  return rc ? rc : adapter_h_bytes(*a);
 }
 
 int anerf_adapter_linear(const AnerfAdapterIO* a, void* stream) {

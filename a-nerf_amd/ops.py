@@ -1072,10 +1072,11 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=Non
     down [L, R, K] (A), up [L, N, R] (B), rows: RowPlan (k = 1) or SortedRows of the M rows over the L adapters."""
     io, keep = _adapter_io(x, weight, down, up, rows, bias, scale, scale_of)
     y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape[0], (down.shape[1] + 15) // 16 * 16, dtype=torch.float32, device=x.device)
+    lib = _lib.load()
+    h, _ = _workspace(lib.anerf_adapter_h_size, "anerf_adapter_h_size", x.device, C.byref(io))
     io.y, io.h = y.data_ptr(), h.data_ptr()
     with on_device(x.device):
-        _lib.check(_lib.load().anerf_adapter_linear(C.byref(io), _stream()), "anerf_adapter_linear")
+        _lib.check(lib.anerf_adapter_linear(C.byref(io), _stream()), "anerf_adapter_linear")
     return y, h
 
 

@@ -585,8 +585,9 @@ int anerf_combine_rows_backward(const void* dy, const void* z, int32_t dtype, co
  * adapter: adapter i owns positions offsets[i] .. offsets[i+1]-1, positions from offsets[n_adapters] on have none (shared projection
  * alone); order [n_rows] maps a position to its row, NULL = the rows lie in that order.  s_i = scale * scale_of[i] (scale_of NULL: scale).
  *   x [n_rows][n_in] rows x_stride elements apart, weight [n_out][n_in], bias [n_out] or NULL, down [n_adapters][rank][n_in] (A),
- *   up [n_adapters][n_out][rank] (B), y [n_rows][n_out]; h [n_rows][rank rounded up to 16] fp32, 16-byte aligned, written: x A_i^T by position
- *   (kept for the backward).  All of dtype but h and scale_of.  Sums in fp32, one rounding at the end. */
+ *   up [n_adapters][n_out][rank] (B), y [n_rows][n_out], all of dtype; h: anerf_adapter_h_size bytes, 16-byte aligned, written: s_i x A_i^T
+ *   by position in fp32 [n_rows][rank rounded up to 16], and behind it the forms the products use (kept for the backward).  Sums in fp32, one
+ *   rounding at the end. */
 typedef struct AnerfAdapterIO {
   int32_t dtype, n_adapters, rank;
   float scale;
@@ -595,8 +596,9 @@ typedef struct AnerfAdapterIO {
   const float* scale_of;
   const int32_t *offsets, *order;
   void* y;
-  float* h;
+  void* h;
 } AnerfAdapterIO;
+int64_t anerf_adapter_h_size(const AnerfAdapterIO* io);
 int anerf_adapter_linear(const AnerfAdapterIO* io, void* stream);
 /* Gradients with weight and bias frozen, from g = d loss / d y ([n_rows][n_out], rows g_stride apart) and the forward's io (its h as
  * the forward left it; y and bias are not read): dx [n_rows][n_in], ddown / dup shaped as down / up; each may be NULL.  Every element is
