@@ -102,6 +102,7 @@ class AnerfTrainLayout(C.Structure):
 
 
 MAX_GROUPS, MAX_CHOICES, MAX_RANK = 1024, 64, 1024       # groups of a plan, groups of a row, rank of an adapter
+FEW_ROWS = 64                                            # ANERF_FEW_ROWS
 
 
 class AnerfAdapterIO(C.Structure):
@@ -218,7 +219,9 @@ SIGNATURES = {
     "anerf_combine_rows_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                               C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
     "anerf_adapter_h_size": (C.c_int64, [C.POINTER(AnerfAdapterIO)]),
-    "anerf_adapter_linear": (C.c_int, [C.POINTER(AnerfAdapterIO), C.c_void_p]),
+    "anerf_adapter_workspace_size": (C.c_int64, [C.POINTER(AnerfAdapterIO)]),
+    "anerf_adapter_linear": (C.c_int, [C.POINTER(AnerfAdapterIO), C.c_void_p, C.c_int64, C.c_void_p]),
+    "anerf_adapter_linear_few": (C.c_int, [C.POINTER(AnerfAdapterIO), C.c_void_p, C.c_int32, C.c_void_p]),
     "anerf_adapter_backward_workspace_size": (C.c_int64, [C.POINTER(AnerfAdapterIO)]),
     "anerf_adapter_backward": (C.c_int, [C.POINTER(AnerfAdapterIO), C.POINTER(AnerfAdapterGradIO), C.c_void_p, C.c_int64, C.c_void_p]),
 }

@@ -173,6 +173,13 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
             raise ValueError(f"adapter_linear: {tuple(rows.shape)} adapter indices for rows {tuple(lead)}")
         if rows.device != dev:
             raise ValueError(f"adapter_linear: indices on {rows.device}, rows on {dev}")
+        if rows.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"adapter_linear: adapter indices must be int32 / int64, got {rows.dtype}")
+        grad = torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad)
+        if M <= ops._lib.FEW_ROWS and not grad:      # a decoding step: no plan, W streams through once
+            flat = flat if flat.stride(1) == 1 and flat.stride(0) >= K else flat.contiguous()
+            return ops.adapter_linear_few(flat, weight.contiguous(), down.contiguous(), up.contiguous(), rows.reshape(-1).contiguous(),
+                                          None if bias is None else bias.contiguous(), float(scale), scale_of).reshape(lead + (N,))
         rows = route_rows(rows.reshape(-1), L)
     elif not isinstance(rows, (RowPlan, SortedRows)):
         raise TypeError(f"adapter_linear: rows must be indices, a RowPlan or its sorted(), got {type(rows).__name__}")

@@ -7,7 +7,10 @@
 //   k_thin       h[p] = s_i x[order[p]] A_i^T: one workgroup a piece of 32 positions of one adapter
 //   k_main       x W^T tile by tile; a tile starts with the low-rank term of the adapters whose positions it holds
 //   k_thin_grad  dA_i / dB_i as sums over pieces of an adapter's positions, k_thin_grad_sum adds the pieces in order
+//   k_few        up to 64 rows with an adapter index each, in any order
 //   k_transpose  W, A, B with their last two axes swapped: dx is then the forward product of (g, W^T, B^T, A^T)
+#include <math.h>
+#include <algorithm>
 #include "anerf_rows.h"
 
 namespace anerf {
@@ -156,6 +159,7 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 // chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.  DIRECT: global_load_lds_dwordx4, eight rows
 // an instruction, the lanes fetching the chunks in the order they have to lie in LDS (16-byte aligned rows); otherwise through registers,
 // at any alignment.
+// Few tiles: `splits` workgroups share one, each with a contiguous part of the stages, and k_sum_parts adds their fp32 tiles.
 // The low-rank term comes first, behind the first stage's loads: for every adapter with positions in the tile h B_i^T is added to the
 // blocks of its rows; a block that two adapters share takes it by row (a NaN in one adapter stays with its rows).
 // fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set, so that no chain of
@@ -166,9 +170,10 @@ struct MainArgs {
   const void* h;               // operand form of h: [M][Rp] fp32, [M][2 Rp] 16-bit
   const float* factor;         // fp16: power of two of every row of h
   void* y;
+  float* part;                 // splits > 1: fp32 [splits][M][N]
   long long ldx, K, N;
   long long M;
-  int L, R, Rp;
+  int L, R, Rp, splits;
 };
 
 constexpr int FOLD = 16;
@@ -190,7 +195,8 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   long long m0, n0;
   {
     const long long tm = (P.M + BM - 1) / BM, tn = (P.N + BN - 1) / BN, all = tm * tn;
-    const long long xcd = blockIdx.x & 7, t = xcd * (all >> 3) + (xcd < (all & 7) ? xcd : (all & 7)) + (blockIdx.x >> 3);
+    const unsigned b = P.splits > 1 ? blockIdx.x / P.splits : blockIdx.x;
+    const long long xcd = b & 7, t = xcd * (all >> 3) + (xcd < (all & 7) ? xcd : (all & 7)) + (b >> 3);
     const long long g = t / (4 * tn), in = t % (4 * tn);
     const long long rows = tm - 4 * g < 4 ? tm - 4 * g : 4;
     m0 = (4 * g + in % rows) * BM;
@@ -242,7 +248,10 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
     for (int l = 0; l < WL; ++l) lds[at(buf, BM / 8 + wave + NW * l) + lane] = rw[l];
   };
-  const int stages = (K + KB - 1) / KB, full = K / KB;
+  const int all_stages = (K + KB - 1) / KB, full = K / KB;
+  const int part = P.splits > 1 ? blockIdx.x % P.splits : 0;
+  const int first = P.splits > 1 ? (int)((long long)all_stages * part / P.splits) : 0;
+  const int stages = P.splits > 1 ? (int)((long long)all_stages * (part + 1) / P.splits) : all_stages;      // end of this workgroup's
   // starts stage s; DIRECT: into LDS, otherwise into registers.  In a last, partial stage the chunks behind the row are not there: DIRECT
   // lanes fetch the stage's first chunk in their place, and the products take zeros for them
   auto start = [&](int s, int buf) {
@@ -265,7 +274,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       fetch_regs(s);
     }
   };
-  start(0, 0);
+  start(first, 0);
   Acc acc[MI][NI];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
@@ -274,7 +283,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 
   // ---- low-rank term
   const int kept = P.offsets[P.L];
-  if (m0 < kept) {
+  if (m0 < kept && part == 0) {
     const int t0 = (int)m0, t1 = min((int)(m0 + BM < P.M ? m0 + BM : P.M), kept);
     const int w0 = t0 + wm * TM;                               // the wave's first position and output
     const long long c0 = n0 + wn * TN;
@@ -379,7 +388,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   };
   if (!DIRECT) put(0);
   arrive();
-  if (stages > 1) start(1, 1);
+  if (first + 1 < stages) start(first + 1, 1);
   read_w(0, 0);
   read_x(0, 0, 0);
   auto zero_behind = [&](u32x4* f, int n, int h) {      // fragments of the partial stage: chunks behind the row
@@ -409,12 +418,12 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     products(1, 1);
   };
   // the buffer is a constant of the loop's code: two stages a turn
-  const int whole = DIRECT ? full : stages;
-  for (int s = 0; s < whole; s += 2) {
+  const int whole = DIRECT && full < stages ? full : stages;
+  for (int s = first; s < whole; s += 2) {
     stage(s, 0, Const<0>());
     if (s + 1 < whole) stage(s + 1, 1, Const<0>());
     if constexpr (TWO) {
-      if (s % FOLD == FOLD - 2) {
+      if ((s - first) % FOLD == FOLD - 2) {
 #pragma unroll
         for (int m = 0; m < MI; ++m)
 #pragma unroll
@@ -425,7 +434,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       }
     }
   }
-  if (DIRECT && full < stages) stage(full, full & 1, Const<1>());
+  if (DIRECT && full < stages) stage(full, (full - first) & 1, Const<1>());
 
   // ---- bias, rounding, store: lane (i, q) holds outputs 8g + 4q .. +3 of its row, a group g of four registers of every block
   const E* bias = static_cast<const E*>(P.bias);
@@ -433,7 +442,9 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   for (int m = 0; m < MI; ++m) {
     const long long p = m0 + wm * TM + BS * m + i;
     if (p >= P.M) continue;
-    E* yr = static_cast<E*>(P.y) + (P.order ? (long long)P.order[p] : p) * P.N;
+    const long long row = P.order ? (long long)P.order[p] : p;
+    E* yr = static_cast<E*>(P.y) + row * P.N;
+    float* pr = P.part + (part * P.M + row) * P.N;
 #pragma unroll
     for (int n = 0; n < NI; ++n)
 #pragma unroll
@@ -446,7 +457,11 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
           if constexpr (TWO) v[e] += sum[m][n][4 * g + e];
         }
         typedef E out4 __attribute__((ext_vector_type(4)));
-        if (col + 4 <= P.N) {
+        if (P.splits > 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < P.N) pr[col + e] = v[e];
+        } else if (col + 4 <= P.N) {
           if (bias) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += (float)bias[col + e];
@@ -461,6 +476,189 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
             if (col + e < P.N) yr[col + e] = (E)(bias ? v[e] + (float)bias[col + e] : v[e]);
         }
       }
+  }
+}
+
+// y = the parts' sum in order + bias; [M][N] as one row of values
+template <int DT>
+__global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ part, int splits, long long all, long long N, const typename Elem<DT>::T* __restrict__ bias,
+                                                   typename Elem<DT>::T* __restrict__ y) {
+  typedef typename Elem<DT>::T E;
+  typedef E out4 __attribute__((ext_vector_type(4)));
+  const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= all) return;
+  if (e + 4 <= all) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      f32x4 w;
+      __builtin_memcpy(&w, part + s * all + e, 16);
+      v += w;
+    }
+    out4 o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = (E)(bias ? v[k] + (float)bias[(e + k) % N] : v[k]);
+    __builtin_memcpy(y + e, &o, sizeof(o));
+  } else {
+    for (int k = 0; e + k < all; ++k) {
+      float v = 0.f;
+      for (int s = 0; s < splits; ++s) v += part[s * all + e + k];
+      y[e + k] = (E)(bias ? v + (float)bias[(e + k) % N] : v);
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------- few rows (a decoding step)
+// Up to 64 rows, each with an adapter index of its own, no plan: the time is what the shared weight takes to arrive.
+//   k_few_thin  h[r][j] = s_i <x[r], A_i[j]>: one wave a value
+//   k_few       a workgroup owns 16*NT outputs of all rows; its eight waves take every eighth 64-byte step of W's rows straight into MFMA
+//               operands (W is read once, no LDS on its way), x comes from L2, and the waves' sums are added through LDS.  The low-rank term of
+//               an output is a dot of `rank` values in fp32, read in front of the loop, so that B's latency hides behind W's.
+constexpr int FEW_WAVES = 8;
+static_assert(ANERF_FEW_ROWS == 64, "four blocks of 16 rows");
+
+template <typename I>
+__device__ __forceinline__ int adapter_of(const void* groups, int r, int L) {
+  const I v = static_cast<const I*>(groups)[r];
+  return v >= 0 && v < (I)L ? (int)v : -1;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) k_few_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const typename Elem<DT>::T* __restrict__ down,
+                                                  const void* __restrict__ groups, int wide, int L, long long K, int R, const float* __restrict__ scale_of,
+                                                  float scale, float* __restrict__ h) {
+  typedef typename Elem<DT>::T E;
+  constexpr int EPC = Elem<DT>::EPC;
+  typedef E vec __attribute__((ext_vector_type(EPC)));
+  const int r = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int a = wide ? adapter_of<long long>(groups, r, L) : adapter_of<int>(groups, r, L);
+  if (a < 0 || j >= R) return;
+  const E* xr = x + r * ldx;
+  const E* ar = down + ((long long)a * R + j) * K;
+  float sum = 0.f;
+  const long long whole = K / EPC;
+#pragma unroll 4
+  for (long long c = lane; c < whole; c += 64) {
+    const vec xv = __builtin_bit_cast(vec, load16(xr + c * EPC)), av = __builtin_bit_cast(vec, load16(ar + c * EPC));
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) s = fmaf((float)xv[e], (float)av[e], s);
+    sum += s;
+  }
+  const long long c = whole * EPC + lane;
+  if (c < K) sum = fmaf((float)xr[c], (float)ar[c], sum);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) h[r * R + j] = sum * (scale_of ? scale * scale_of[a] : scale);
+}
+
+template <int DT, int MT, int NT>
+__global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>::T* __restrict__ x, long long ldx, const typename Elem<DT>::T* __restrict__ w,
+                                                        const typename Elem<DT>::T* __restrict__ bias, const typename Elem<DT>::T* __restrict__ up,
+                                                        const void* __restrict__ groups, int wide, int L, int M, long long K, long long N, int R,
+                                                        const float* __restrict__ h, typename Elem<DT>::T* __restrict__ y) {
+  typedef typename Elem<DT>::T E;
+  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, DEPTH = MT * NT >= 4 ? 2 : 4;
+  typedef E vec __attribute__((ext_vector_type(EPC)));
+  constexpr int OUT = 16 * NT, VALUES = OUT * 16 * MT, MINE = (VALUES + FEW_WAVES * 64 - 1) / (FEW_WAVES * 64);
+  __shared__ f32x4 red[FEW_WAVES / 2][MT * NT][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, q = lane >> 4;
+  const long long n0 = (long long)blockIdx.x * OUT;
+  // the low-rank term of this thread's outputs: row v / OUT, output n0 + v % OUT
+  float thin[MINE];
+#pragma unroll
+  for (int t = 0; t < MINE; ++t) {
+    thin[t] = 0.f;
+    const int v = tid + t * FEW_WAVES * 64, r = v / OUT;
+    const long long n = n0 + v % OUT;
+    if (v >= VALUES || r >= M || n >= N) continue;
+    const int a = wide ? adapter_of<long long>(groups, r, L) : adapter_of<int>(groups, r, L);
+    if (a < 0) continue;
+    const E* br = up + ((long long)a * N + n) * R;
+    const float* hr = h + r * R;
+    int j = 0;
+    for (; j + EPC <= R; j += EPC) {
+      const vec b = __builtin_bit_cast(vec, load16(br + j));
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) thin[t] = fmaf(hr[j + e], (float)b[e], thin[t]);
+    }
+    for (; j < R; ++j) thin[t] = fmaf(hr[j], (float)br[j], thin[t]);
+  }
+  const E* wr[NT];
+  const E* xr[MT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const long long o = n0 + 16 * n + i;
+    wr[n] = w + (o < N ? o : N - 1) * K;
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xr[m] = x + min(16 * m + i, M - 1) * ldx;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto walk = [&](long long s0, auto depth, auto tail) {
+    constexpr int D = decltype(depth)::value;
+    u32x4 wv[D][NT], xv[D][MT];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const long long k = (s0 + d * FEW_WAVES) * STEP + q * EPC;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) wv[d][n] = decltype(tail)::value ? load_tail<DT>(wr[n], k, K) : load16(wr[n] + k);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xv[d][m] = decltype(tail)::value ? load_tail<DT>(xr[m], k, K) : load16(xr[m] + k);
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(wv[d][n], xv[d][m], acc[m][n], e);
+  };
+  const long long steps = K / STEP;
+  long long s = wave;
+  for (; s + (DEPTH - 1) * FEW_WAVES < steps; s += DEPTH * FEW_WAVES) walk(s, Const<DEPTH>(), Const<0>());
+  for (; s < steps; s += FEW_WAVES) walk(s, Const<1>(), Const<0>());
+  if (steps * STEP < K && wave == (int)(steps % FEW_WAVES)) walk(steps, Const<1>(), Const<1>());
+  // 8 -> 4 -> 2 -> 1 waves
+#pragma unroll
+  for (int half = FEW_WAVES / 2; half; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) red[wave - half][m * NT + n][lane] = acc[m][n];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] += red[wave][m * NT + n][lane];
+    }
+    __syncthreads();
+  }
+  float* out = reinterpret_cast<float*>(red);      // [16 MT rows][OUT + 4]
+  constexpr int LD = OUT + 4;
+  static_assert(16 * MT * LD * 4 <= sizeof(red), "the sums fit where the waves' parts were");
+  if (wave == 0) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(out + (16 * m + i) * LD + 16 * n + 4 * q) = acc[m][n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < MINE; ++t) {
+    const int v = tid + t * FEW_WAVES * 64, r = v / OUT;
+    const long long n = n0 + v % OUT;
+    if (v >= VALUES || r >= M || n >= N) continue;
+    float f = out[r * LD + v % OUT] + thin[t];
+    if (bias) f += (float)bias[n];
+    y[r * N + n] = (E)f;
   }
 }
 
@@ -621,39 +819,53 @@ static int run_main(const MainArgs& P, hipStream_t st) {
   constexpr int bytes = 2 * (BM + BN) * 128;
   const auto kernel = k_main<DT, 16, BM, BN, WM, WN, DIRECT>;
   ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes, &done);
-  kernel<<<(unsigned)((P.M + BM - 1) / BM * ((P.N + BN - 1) / BN)), WM * WN * 64, bytes, st>>>(P);
-  return check_launch("k_main");
+  kernel<<<(unsigned)((P.M + BM - 1) / BM * ((P.N + BN - 1) / BN) * P.splits), WM * WN * 64, bytes, st>>>(P);
+  const int rc = check_launch("k_main");
+  if (rc || P.splits == 1) return rc;
+  typedef typename Elem<DT>::T E;
+  const long long all = P.M * P.N;
+  k_sum_parts<DT><<<(unsigned)((all + 1023) / 1024), 256, 0, st>>>(P.part, P.splits, all, P.N, static_cast<const E*>(P.bias), static_cast<E*>(P.y));
+  return check_launch("k_sum_parts");
 }
 
-// Tile: the larger, the fewer LDS reads a product (a 256 x 256 tile's waves read 3/8 of what a 64 x 64 tile's do) and the fewer tiles
-// there are to fill 256 CUs with: the time is rounds of the chip x what a tile costs.
+// Less than one 64 x 64 tile a CU leaves CUs idle and their few waves waiting: the contraction is split until there are 512 workgroups,
+// eight stages each at least (128 x 4096 x 4096 bf16: 128 tiles 48 us, 512 workgroups and the sum 35; 256 tiles and more do not gain)
+static int split_of(int dtype, long long M, long long K, long long N) {
+  const long long tiles = (M + 63) / 64 * ((N + 63) / 64), stages = (K + (dtype == ANERF_F32 ? 31 : 63)) / (dtype == ANERF_F32 ? 32 : 64);
+  if (tiles == 0 || tiles >= 256) return 1;
+  const long long s = 512 / tiles < stages / 8 ? 512 / tiles : stages / 8;
+  return s < 2 ? 1 : s > 16 ? 16 : (int)s;
+}
+
+// Tile: the larger, the fewer LDS reads a product (a 256 x 256 tile's waves read 3/8 of what a 64 x 64 tile's do), but the tiles of one CU
+// run one after the other, and what the last round leaves idle grows.  Cost: tiles of the busiest CU x size / rate; the rates are
+// what the tiles reach where there are many of them, relative to 256 x 256 (bf16, 8192 x 4096 x 4096: 256 x 256 274 us, 128 x 128 318, 128 x 64
+// 368, 64 x 64 446).  fp32 is bound by its products, and one size is as fast as the other (1941 .. 2009 us).
 template <int DT>
 static int launch_main(const MainArgs& P, hipStream_t st) {
+  constexpr long long es = sizeof(typename Elem<DT>::T), span = 1ll << 32;      // DIRECT's offsets have 32 bits
   const bool direct = (((uintptr_t)P.x | (uintptr_t)P.w) & 15) == 0 && P.K % Elem<DT>::EPC == 0 && P.ldx % Elem<DT>::EPC == 0 &&
-                      P.M * P.ldx * (long long)sizeof(typename Elem<DT>::T) < (1ll << 32) && P.N * P.K * (long long)sizeof(typename Elem<DT>::T) < (1ll << 32);
-  auto cost = [&](int bm, int bn, int at_once, double rate) {     // CU rounds x relative time of what a CU holds at once
-    const double tiles = (double)((P.M + bm - 1) / bm) * (double)((P.N + bn - 1) / bn);
-    const double rounds = (double)(long long)((tiles + 256.0 * at_once - 1) / (256.0 * at_once));
-    const double share = tiles < 256.0 * at_once ? (tiles + 255) / 256 : at_once;      // tiles that the busiest CU runs side by side
-    return rounds * (double)(long long)share * bm * bn / rate;
+                      P.M * P.ldx * es < span && P.N * P.K * es < span;
+  auto cost = [&](int bm, int bn, double rate, bool few_waves) {
+    const long long tiles = (P.M + bm - 1) / bm * ((P.N + bn - 1) / bn), mine = (tiles + 255) / 256;
+    return (double)mine * bm * bn / (few_waves && mine == 1 ? 0.85 * rate : rate);      // (one wave a SIMD does not hide its own waits)
   };
-  const double c64 = cost(64, 64, 4, 0.5), c128 = cost(128, 128, 2, 0.75), cbig = DT == ANERF_F32 ? cost(128, 256, 1, 0.8) : cost(256, 256, 1, 1.0);
-  const double cmid = cost(256, 128, 1, 0.85);
-#ifdef EXP_TILE
-  if (EXP_TILE == 64) return run_main<DT, 64, 64, 2, 2, true>(P, st);
-  if (EXP_TILE == 128) return run_main<DT, 128, 128, 2, 2, true>(P, st);
-  if (EXP_TILE == 256) return run_main<DT, 128, 256, 2, 4, true>(P, st);
-  if (EXP_TILE == 12864) return run_main<DT, 128, 64, 2, 2, true>(P, st);
-#endif
-  if (!direct) return c64 < c128 ? run_main<DT, 64, 64, 2, 2, false>(P, st) : run_main<DT, 128, 128, 2, 2, false>(P, st);
-  if (cbig <= c64 && cbig <= c128 && (DT == ANERF_F32 || cbig <= cmid)) {
-    if constexpr (DT == ANERF_F32) return run_main<DT, 128, 256, 2, 4, true>(P, st);
-    else return run_main<DT, 256, 256, 2, 4, true>(P, st);
+  constexpr bool F32 = DT == ANERF_F32;
+  const double c64 = cost(64, 64, F32 ? 0.97 : 0.6, true), c128 = cost(128, 128, F32 ? 1.0 : 0.87, true);
+  if (P.splits > 1 || !direct || F32) {
+    const bool small = P.splits > 1 || c64 <= c128;
+    if (direct) return small ? run_main<DT, 64, 64, 2, 2, true>(P, st) : run_main<DT, 128, 128, 2, 2, true>(P, st);
+    return small ? run_main<DT, 64, 64, 2, 2, false>(P, st) : run_main<DT, 128, 128, 2, 2, false>(P, st);
   }
-  if constexpr (DT != ANERF_F32) {
-    if (cmid <= c64 && cmid <= c128) return run_main<DT, 256, 128, 4, 2, true>(P, st);
+  if constexpr (!F32) {
+    const double c96 = cost(128, 64, 0.75, true), c192 = cost(256, 128, 0.97, false), c256 = cost(256, 256, 1.05, false);
+    const double least = fmin(fmin(fmin(c64, c128), c96), fmin(c192, c256));
+    if (c256 == least) return run_main<DT, 256, 256, 2, 4, true>(P, st);
+    if (c192 == least) return run_main<DT, 256, 128, 4, 2, true>(P, st);
+    if (c128 == least) return run_main<DT, 128, 128, 2, 2, true>(P, st);
+    if (c96 == least) return run_main<DT, 128, 64, 2, 2, true>(P, st);
   }
-  return c64 < c128 ? run_main<DT, 64, 64, 2, 2, true>(P, st) : run_main<DT, 128, 128, 2, 2, true>(P, st);
+  return run_main<DT, 64, 64, 2, 2, true>(P, st);
 }
 
 // what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][2 Rp] (16-bit types) | factor [n_rows] (fp16); byte offsets
@@ -671,9 +883,13 @@ static HLayout h_layout(const AnerfAdapterIO& A) {
   return H;
 }
 long long adapter_h_bytes(const AnerfAdapterIO& A) { return h_layout(A).bytes; }
+long long adapter_workspace(const AnerfAdapterIO& A) {
+  const int splits = split_of(A.dtype, A.n_rows, A.n_in, A.n_out);
+  return splits > 1 ? splits * A.n_rows * A.n_out * 4 : 0;
+}
 
 template <int DT>
-static int linear_t(const AnerfAdapterIO& A, hipStream_t st) {
+static int linear_t(const AnerfAdapterIO& A, void* ws, hipStream_t st) {
   typedef typename Elem<DT>::T E;
   const HLayout H = h_layout(A);
   const long long pieces = pieces_bound(A.n_rows, A.n_adapters, TH_ROWS);
@@ -695,15 +911,47 @@ static int linear_t(const AnerfAdapterIO& A, hipStream_t st) {
   if (rc || !A.y) return rc;       // (the gradient of A alone needs h only)
   const void* operand = split;
   if constexpr (DT == ANERF_F32) operand = h;
-  const MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, A.y, A.x_stride, A.n_in, A.n_out, A.n_rows, A.n_adapters, A.rank, Rp};
+  const MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, A.y, static_cast<float*>(ws),
+                      A.x_stride, A.n_in, A.n_out, A.n_rows, A.n_adapters, A.rank, Rp, split_of(DT, A.n_rows, A.n_in, A.n_out)};
   return launch_main<DT>(P, st);
 }
 
-int launch_adapter_linear(const AnerfAdapterIO& A, hipStream_t st) {
+int launch_adapter_linear(const AnerfAdapterIO& A, void* ws, hipStream_t st) {
   switch (A.dtype) {
-    case ANERF_F32: return linear_t<ANERF_F32>(A, st);
-    case ANERF_BF16: return linear_t<ANERF_BF16>(A, st);
-    default: return linear_t<ANERF_F16>(A, st);
+    case ANERF_F32: return linear_t<ANERF_F32>(A, ws, st);
+    case ANERF_BF16: return linear_t<ANERF_BF16>(A, ws, st);
+    default: return linear_t<ANERF_F16>(A, ws, st);
+  }
+}
+
+template <int DT>
+static int few_t(const AnerfAdapterIO& A, const void* groups, int wide, hipStream_t st) {
+  typedef typename Elem<DT>::T E;
+  const E* x = static_cast<const E*>(A.x);
+  const int M = (int)A.n_rows;
+  float* h = static_cast<float*>(A.h);
+  k_few_thin<DT><<<dim3(M, (A.rank + 3) / 4), 256, 0, st>>>(x, A.x_stride, static_cast<const E*>(A.down), groups, wide, A.n_adapters, A.n_in, A.rank,
+                                                           A.scale_of, A.scale, h);
+  int rc = check_launch("k_few_thin");
+  if (rc) return rc;
+  auto run = [&](auto kernel, int out) {
+    kernel<<<(unsigned)((A.n_out + out - 1) / out), FEW_WAVES * 64, 0, st>>>(x, A.x_stride, static_cast<const E*>(A.weight), static_cast<const E*>(A.bias),
+                                                                          static_cast<const E*>(A.up), groups, wide, A.n_adapters, M, A.n_in, A.n_out,
+                                                                          A.rank, h, static_cast<E*>(A.y));
+  };
+  // 32 outputs a workgroup halve what x costs in L2 traffic, where they still fill the chip
+  const bool wide_out = A.n_out >= 8192;
+  if (M <= 16) wide_out ? run(k_few<DT, 1, 2>, 32) : run(k_few<DT, 1, 1>, 16);
+  else if (M <= 32) wide_out ? run(k_few<DT, 2, 2>, 32) : run(k_few<DT, 2, 1>, 16);
+  else wide_out ? run(k_few<DT, 4, 2>, 32) : run(k_few<DT, 4, 1>, 16);
+  return check_launch("k_few");
+}
+
+int launch_adapter_few(const AnerfAdapterIO& A, const void* groups, int wide, hipStream_t st) {
+  switch (A.dtype) {
+    case ANERF_F32: return few_t<ANERF_F32>(A, groups, wide, st);
+    case ANERF_BF16: return few_t<ANERF_BF16>(A, groups, wide, st);
+    default: return few_t<ANERF_F16>(A, groups, wide, st);
   }
 }
 
@@ -721,8 +969,13 @@ static long long part_floats(long long M, int L, long long C, int Rp) {
   return pieces_bound(M, L, rows) * Rp * C;
 }
 
+static AnerfAdapterIO swapped(const AnerfAdapterIO& A) {      // sizes of the product that dx is
+  AnerfAdapterIO T = A;
+  T.n_in = A.n_out, T.n_out = A.n_in;
+  return T;
+}
 struct BackwardPlan {
-  long long wt, dt, ut, u, part, bytes;     // byte offsets in the workspace
+  long long wt, dt, ut, u, part, bytes;     // byte offsets in the workspace; the parts of dx's product and those of dA, dB share `part`
 };
 static BackwardPlan backward_plan(const AnerfAdapterIO& A) {
   const long long es = A.dtype == ANERF_F32 ? 4 : 2;
@@ -735,7 +988,8 @@ static BackwardPlan backward_plan(const AnerfAdapterIO& A) {
   B.ut = at, at += up16((long long)A.n_adapters * A.rank * A.n_out * es);
   B.u = at, at += up16(h_layout(A).bytes);
   const long long pa = part_floats(A.n_rows, A.n_adapters, A.n_in, Rp), pb = part_floats(A.n_rows, A.n_adapters, A.n_out, Rp);
-  B.part = at, at += up16((pa > pb ? pa : pb) * 4);
+  const long long pd = adapter_workspace(swapped(A));
+  B.part = at, at += up16(std::max(std::max(pa, pb) * 4, pd));
   B.bytes = at;
   return B;
 }
@@ -785,10 +1039,10 @@ static int backward_t(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, char
     else k_transpose<uint16_t><<<(unsigned)blocks, 256, 0, st>>>(J);
     int rc = check_launch("k_transpose");
     if (rc) return rc;
-    AnerfAdapterIO T = A;
+    AnerfAdapterIO T = swapped(A);
     T.x = G.g, T.x_stride = G.g_stride, T.weight = ws + B.wt, T.bias = nullptr, T.down = ws + B.ut, T.up = ws + B.dt;
-    T.n_in = A.n_out, T.n_out = A.n_in, T.y = G.dx, T.h = ws + B.u;
-    rc = linear_t<DT>(T, st);
+    T.y = G.dx, T.h = ws + B.u;
+    rc = linear_t<DT>(T, ws + B.part, st);
     if (rc) return rc;
   }
   if (G.ddown) {

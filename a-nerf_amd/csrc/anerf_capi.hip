@@ -79,8 +79,10 @@ long long route_workspace(long long n, int G);
 int launch_route(const void* idx, int wide, long long n, int G, int32_t* offsets, int32_t* source, int32_t* slot, void* ws, hipStream_t st);
 int launch_rows(int op, int dtype, const void* a, const void* b, const float* w, const int32_t* slot, const int32_t* end, long long T, int k,
                 long long D, void* out, float* dw, hipStream_t st);
-int launch_adapter_linear(const AnerfAdapterIO& A, hipStream_t st);
+long long adapter_workspace(const AnerfAdapterIO& A);
+int launch_adapter_linear(const AnerfAdapterIO& A, void* ws, hipStream_t st);
 long long adapter_h_bytes(const AnerfAdapterIO& A);
+int launch_adapter_few(const AnerfAdapterIO& A, const void* groups, int wide, hipStream_t st);
 long long adapter_backward_workspace(const AnerfAdapterIO& A);
 int launch_adapter_backward(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, void* ws, hipStream_t st);
 int launch_code_reduce(const float* du, int uw, const float* cam, int n, int S, int n_codes, float* rowsum, float* dcodes,
@@ -1339,12 +1341,30 @@ int64_t anerf_adapter_h_size(const AnerfAdapterIO* a) {
   return rc ? rc : adapter_h_bytes(*a);
 }
 
-int anerf_adapter_linear(const AnerfAdapterIO* a, void* stream) {
+int64_t anerf_adapter_workspace_size(const AnerfAdapterIO* a) {
+  const int rc = adapter_check(a);
+  return rc ? rc : adapter_workspace(*a);
+}
+
+int anerf_adapter_linear(const AnerfAdapterIO* a, void* workspace, int64_t ws_bytes, void* stream) {
   const int rc = adapter_check(a);
   if (rc || a->n_rows == 0) return rc;
   if (!a->x || !a->weight || !a->down || !a->up || !a->offsets || !a->y || !a->h) return set_error(ANERF_E_NULL, "adapter_linear: null pointer");
   if ((uintptr_t)a->h & 15) return set_error(ANERF_E_SHAPE, "adapter_linear: h must be 16-byte aligned");
-  return launch_adapter_linear(*a, static_cast<hipStream_t>(stream));
+  const int64_t need = adapter_workspace(*a);
+  if (ws_bytes < need || (need && !workspace)) return set_error(ANERF_E_WORKSPACE, "adapter_linear: workspace too small");
+  if ((uintptr_t)workspace & 15) return set_error(ANERF_E_SHAPE, "adapter_linear: workspace must be 16-byte aligned");
+  return launch_adapter_linear(*a, workspace, static_cast<hipStream_t>(stream));
+}
+
+int anerf_adapter_linear_few(const AnerfAdapterIO* a, const void* groups, int32_t wide, void* stream) {
+  const int rc = adapter_check(a);
+  if (rc) return rc;
+  if (a->n_rows > ANERF_FEW_ROWS) return set_error(ANERF_E_SHAPE, "adapter_linear_few: at most 64 rows");
+  if (a->n_rows == 0) return ANERF_OK;
+  if (!a->x || !a->weight || !a->down || !a->up || !a->y || !a->h || !groups) return set_error(ANERF_E_NULL, "adapter_linear_few: null pointer");
+  if ((uintptr_t)a->h & 15) return set_error(ANERF_E_SHAPE, "adapter_linear_few: h must be 16-byte aligned");
+  return launch_adapter_few(*a, groups, wide, static_cast<hipStream_t>(stream));
 }
 
 int64_t anerf_adapter_backward_workspace_size(const AnerfAdapterIO* a) {

@@ -1061,7 +1061,7 @@ def _adapter_io(x, weight, down, up, rows, bias, scale, scale_of):
     io.dtype, io.n_adapters, io.rank, io.scale = ROW_DTYPES[x.dtype], down.shape[0], down.shape[1], float(scale)
     io.n_rows, io.n_in, io.n_out, io.x_stride = x.shape[0], weight.shape[1], weight.shape[0], x.stride(0)
     order = rows.source if isinstance(rows, RowPlan) else None
-    keep = [x, weight, down, up, bias, scale_of, rows.offsets, order]
+    keep = [x, weight, down, up, bias, scale_of, None if rows is None else rows.offsets, order]
     for name, t in zip(("x", "weight", "down", "up", "bias", "scale_of", "offsets", "order"), keep):
         setattr(io, name, None if t is None else t.data_ptr())
     return io, keep
@@ -1076,8 +1076,22 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=Non
     h, _ = _workspace(lib.anerf_adapter_h_size, "anerf_adapter_h_size", x.device, C.byref(io))
     io.y, io.h = y.data_ptr(), h.data_ptr()
     with on_device(x.device):
-        _lib.check(lib.anerf_adapter_linear(C.byref(io), _stream()), "anerf_adapter_linear")
+        need = lib.anerf_adapter_workspace_size(C.byref(io))
+        ws = torch.empty(need // 4, dtype=torch.float32, device=x.device) if need > 0 else None
+        _lib.check(lib.anerf_adapter_linear(C.byref(io), _p(ws), need, _stream()), "anerf_adapter_linear")
     return y, h
+
+
+def adapter_linear_few(x, weight, down, up, groups, bias=None, scale=1.0, scale_of=None):
+    """adapter_linear of up to 64 rows with their adapter indices instead of a plan (anerf_adapter_linear_few) -> y [M, N]"""
+    io, keep = _adapter_io(x, weight, down, up, None, bias, scale, scale_of)
+    M, N, R = x.shape[0], weight.shape[0], down.shape[1]
+    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    h = torch.empty(M * R, dtype=torch.float32, device=x.device)
+    io.y, io.h = y.data_ptr(), h.data_ptr()
+    with on_device(x.device):
+        _lib.check(_lib.load().anerf_adapter_linear_few(C.byref(io), _p(groups), int(groups.dtype == torch.int64), _stream()), "anerf_adapter_linear_few")
+    return y
 
 
 def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, want_dx=True, want_ddown=True, want_dup=True):

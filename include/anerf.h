@@ -599,7 +599,13 @@ typedef struct AnerfAdapterIO {
   void* h;
 } AnerfAdapterIO;
 int64_t anerf_adapter_h_size(const AnerfAdapterIO* io);
-int anerf_adapter_linear(const AnerfAdapterIO* io, void* stream);
+/* workspace: anerf_adapter_workspace_size bytes (0 unless the rows are few), 16-byte aligned. */
+int64_t anerf_adapter_workspace_size(const AnerfAdapterIO* io);
+int anerf_adapter_linear(const AnerfAdapterIO* io, void* workspace, int64_t ws_bytes, void* stream);
+/* The same for up to 64 rows (a decoding step), without a plan: groups [n_rows] int64 (wide != 0) or int32 holds every row's adapter, a value
+ * outside 0 .. n_adapters-1 none.  offsets and order are not read; h: n_rows * rank floats of scratch, 16-byte aligned. */
+#define ANERF_FEW_ROWS 64
+int anerf_adapter_linear_few(const AnerfAdapterIO* io, const void* groups, int32_t wide, void* stream);
 /* Gradients with weight and bias frozen, from g = d loss / d y ([n_rows][n_out], rows g_stride apart) and the forward's io (its h as
  * the forward left it; y and bias are not read): dx [n_rows][n_in], ddown / dup shaped as down / up; each may be NULL.  Every element is
  * written (adapters without rows: zeros), every sum has one order.  workspace: anerf_adapter_backward_workspace_size bytes, 256-byte aligned. */

@@ -46,14 +46,29 @@ def _io(**kw):
 
 def test_adapter_linear_refuses():
     lib = _lib.load()
-    call = lambda **kw: lib.anerf_adapter_linear(ctypes.byref(_io(**kw)), None)
+    call = lambda ws=P(9), n=1 << 30, **kw: lib.anerf_adapter_linear(ctypes.byref(_io(**kw)), ws, n, None)
     for kw in (dict(n_adapters=0), dict(n_adapters=1025), dict(rank=0), dict(rank=1025), dict(n_rows=-1), dict(n_rows=2 ** 31), dict(n_in=0), dict(n_out=0),
                dict(n_in=2 ** 25), dict(n_rows=2 ** 31 - 1, n_out=2 ** 12), dict(h=P(7).value + 4)):
         assert call(**kw) == E_SHAPE, kw
-    assert call(dtype=7) == E_CONFIG and lib.anerf_adapter_linear(None, None) == E_NULL
+    assert call(dtype=7) == E_CONFIG and lib.anerf_adapter_linear(None, None, 0, None) == E_NULL
     for k in ("x", "weight", "down", "up", "offsets", "y", "h"):
         assert call(**{k: None}) == E_NULL, k
     assert call(n_rows=0) == 0
+    few = dict(n_rows=128, n_in=4096, n_out=4096)
+    need = lib.anerf_adapter_workspace_size(ctypes.byref(_io(**few)))
+    assert need > 0 and lib.anerf_adapter_workspace_size(ctypes.byref(_io(n_rows=100000, n_in=512, n_out=512))) == 0
+    assert call(n=need - 1, **few) == E_WORKSPACE and call(ws=None, n=need, **few) == E_WORKSPACE
+    assert call(ws=ctypes.c_void_p(P(9).value + 4), **few) == E_SHAPE
+    assert lib.anerf_adapter_h_size(ctypes.byref(_io())) >= 10 * 16 * 4 and lib.anerf_adapter_h_size(ctypes.byref(_io(rank=0))) == E_SHAPE
+
+
+def test_adapter_linear_few_refuses():
+    lib = _lib.load()
+    call = lambda g=P(8), **kw: lib.anerf_adapter_linear_few(ctypes.byref(_io(**{**dict(offsets=None), **kw})), g, 1, None)
+    assert call(n_rows=65) == E_SHAPE and call(rank=0) == E_SHAPE and call(dtype=5) == E_CONFIG and call(h=P(7).value + 4) == E_SHAPE
+    assert call(g=None) == E_NULL and call(n_rows=0) == 0 and lib.anerf_adapter_linear_few(None, P(8), 1, None) == E_NULL
+    for k in ("x", "weight", "down", "up", "y", "h"):
+        assert call(**{k: None}) == E_NULL, k
 
 
 def test_adapter_backward_refuses():
@@ -61,6 +76,7 @@ def test_adapter_backward_refuses():
     need = lib.anerf_adapter_backward_workspace_size(ctypes.byref(_io()))
     assert need > 0 and lib.anerf_adapter_backward_workspace_size(ctypes.byref(_io(rank=0))) == E_SHAPE
     g = _lib.AnerfAdapterGradIO(P(1).value, 32, P(2).value, P(3).value, P(4).value)
+    assert lib.anerf_adapter_backward_workspace_size(ctypes.byref(_io(n_rows=0))) > 0 and lib.anerf_adapter_workspace_size(ctypes.byref(_io(n_rows=0))) == 0
     call = lambda io, g=g, ws=P(16), n=need: lib.anerf_adapter_backward(ctypes.byref(io), None if g is None else ctypes.byref(g), ws, n, None)
     assert call(_io(), None) == E_NULL and call(_io(), n=need - 1) == E_WORKSPACE and call(_io(), ws=None) == E_WORKSPACE
     assert call(_io(), ws=ctypes.c_void_p(P(16).value + 16)) == E_SHAPE and call(_io(h=None)) == E_NULL and call(_io(x=None)) == E_NULL
