@@ -42,8 +42,6 @@ _graphs = WeakIdKeyDictionary()     # leaf -> its living graphs
 
 
 def _graph_of(*tensors):
-    if not torch.is_grad_enabled():
-        return None
     leaves = [t for t in tensors if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
     if not leaves:
         return None
@@ -100,6 +98,8 @@ class _CombineFn(torch.autograd.Function):
 def dispatch_rows(x, plan):
     """x [T, ...] -> [T * k, ...]: row t at the positions plan.slot[t] of its groups; the rows behind the kept ones are zero."""
     _check_plan(plan, "dispatch_rows")
+    if not _needs_grad(x):
+        return ops.dispatch_rows(x, plan)
     return _DispatchFn.apply(x, plan, _graph_of(x))
 
 
@@ -107,7 +107,13 @@ def combine_rows(z, plan, weights=None):
     """z [T * k, ...] in group order -> [T, ...]: y[t] = sum_j weights[t, j] * z[plan.slot[t, j]] over the kept pairs (weights None: 1).
     A row whose pairs are all dropped gets zeros; what z or weights hold for a dropped pair is not read."""
     _check_plan(plan, "combine_rows")
+    if not _needs_grad(z, weights):
+        return ops.combine_rows(z, plan, weights)
     return _CombineFn.apply(z, weights, plan, _graph_of(z, weights))
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in tensors)
 
 
 def _check_plan(plan, name):
@@ -175,23 +181,23 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
             raise ValueError(f"adapter_linear: indices on {rows.device}, rows on {dev}")
         if rows.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"adapter_linear: adapter indices must be int32 / int64, got {rows.dtype}")
-        grad = torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad)
-        if M <= ops._lib.FEW_ROWS and not grad:      # a decoding step: no plan, W streams through once
-            flat = flat if flat.stride(1) == 1 and flat.stride(0) >= K else flat.contiguous()
-            return ops.adapter_linear_few(flat, weight.contiguous(), down.contiguous(), up.contiguous(), rows.reshape(-1).contiguous(),
-                                          None if bias is None else bias.contiguous(), float(scale), scale_of).reshape(lead + (N,))
-        rows = route_rows(rows.reshape(-1), L)
+        few = M <= ops._lib.FEW_ROWS and not _needs_grad(x, down, up)      # a decoding step: no plan, W streams through once
+        rows = rows.reshape(-1).contiguous() if few else route_rows(rows.reshape(-1), L)
     elif not isinstance(rows, (RowPlan, SortedRows)):
         raise TypeError(f"adapter_linear: rows must be indices, a RowPlan or its sorted(), got {type(rows).__name__}")
-    if rows.n_rows != M or rows.device != dev or getattr(rows, "k", 1) != 1:
-        raise ValueError(f"adapter_linear: a plan of {rows.n_rows} rows with {getattr(rows, 'k', 1)} group(s) each on {rows.device} for {M} rows on {dev}")
-    if rows.n_groups < L:
-        raise ValueError(f"adapter_linear: a plan of {rows.n_groups} groups for {L} adapters")
     if flat.stride(1) != 1 or flat.stride(0) < K:
         flat = flat.contiguous()
-    y = _AdapterFn.apply(flat, down.contiguous(), up.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(), rows, float(scale),
-                         scale_of, _graph_of(x, down, up))
-    return y.reshape(lead + (N,))
+    weight, down_, up_, bias = weight.contiguous(), down.contiguous(), up.contiguous(), None if bias is None else bias.contiguous()
+    scale = float(scale)
+    if torch.is_tensor(rows):
+        return ops.adapter_linear_few(flat, weight, down_, up_, rows, bias, scale, scale_of).reshape(lead + (N,))
+    if rows.n_rows != M or rows.device != dev or rows.k != 1:
+        raise ValueError(f"adapter_linear: a plan of {rows.n_rows} rows with {rows.k} group(s) each on {rows.device} for {M} rows on {dev}")
+    if rows.n_groups < L:
+        raise ValueError(f"adapter_linear: a plan of {rows.n_groups} groups for {L} adapters")
+    if not _needs_grad(x, down, up):
+        return ops.adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of)[0].reshape(lead + (N,))
+    return _AdapterFn.apply(flat, down_, up_, weight, bias, rows, scale, scale_of, _graph_of(x, down, up)).reshape(lead + (N,))
 
 
 LAYERS = [f"pts_linears.{i}" for i in range(8)] + ["alpha_linear", "feature_linear", "views_linears.0", "rgb_linear"]

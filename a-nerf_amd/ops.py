@@ -3,6 +3,7 @@ memory and the stream; every op below enqueues hand-written HIP kernels from lib
 torch's current stream and returns torch tensors that alias the buffers the kernels wrote.
 """
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -913,19 +914,19 @@ def backward(state, g, packed_t_c, packed_t_f, perm, shapes_c, shapes_f, packed_
 ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-class on_device:
-    """make `dev` the current device for the launches inside (the library launches on the current device's current stream)"""
+def _launch(dev, fn, name, *args):
+    """fn(*args, stream) on `dev`, which need not be the current device (the library launches on the current device's current stream)"""
+    if dev.index == torch._C._cuda_getDevice() or dev.index is None:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, name)
 
-    def __init__(self, dev):
-        self.ctx = torch.cuda.device(dev) if dev.index is not None and dev.index != torch._C._cuda_getDevice() else None
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *a):
-        if self.ctx is not None:
-            self.ctx.__exit__(*a)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows_like(t, name, dev=None, dtype=None):
@@ -946,30 +947,49 @@ class RowPlan:
     dropped ones (group outside 0 .. n_groups-1) last:
       offsets [n_groups + 1] int32   first position of every group; the last entry counts the kept pairs
       source  [n_rows * k]   int32   position -> pair t * k + j
-      slot    [n_rows, k] or [n_rows] int32   pair -> position (shape of the groups it was made from)"""
+      slot    [n_rows, k] or [n_rows] int32   pair -> position (shape of the groups it was made from)
+    The three are views of one buffer (made when asked for: a call of the library takes addresses)."""
 
-    def __init__(self, offsets, source, slot, n_rows, k, n_groups):
-        self.offsets, self.source, self.slot = offsets, source, slot
-        self.n_rows, self.k, self.n_groups = n_rows, k, n_groups
+    def __init__(self, buf, n_rows, k, n_groups, shape):
+        self.buf, self.n_rows, self.k, self.n_groups, self.shape, self.device = buf, n_rows, k, n_groups, shape, buf.device
+        self.pairs = n_rows * k
+        base = buf.data_ptr()
+        self.offsets_ptr, self.kept_ptr = base, base + 4 * n_groups
+        self.source_ptr = base + 4 * ((n_groups + 4) // 4 * 4)
+        self.slot_ptr = self.source_ptr + 4 * ((self.pairs + 3) // 4 * 4)
+        self.order_ptr = self.source_ptr
+
+    def _view(self, ptr, n):
+        at = (ptr - self.buf.data_ptr()) // 4
+        return self.buf[at:at + n]
 
     @property
-    def device(self):
-        return self.offsets.device
+    def offsets(self):
+        return self._view(self.offsets_ptr, self.n_groups + 1)
+
+    @property
+    def source(self):
+        return self._view(self.source_ptr, self.pairs)
+
+    @property
+    def slot(self):
+        return self._view(self.slot_ptr, self.pairs).view(self.shape)
 
     def sorted(self):
         """the plan of the DISPATCHED rows: n_rows * k of them, lying in group order already"""
-        return SortedRows(self.offsets, self.n_rows * self.k, self.n_groups)
+        return SortedRows(self)
 
 
 class SortedRows:
     """rows that lie in group order: group g owns rows offsets[g] .. offsets[g+1]-1, the rows behind offsets[n_groups] have none"""
 
-    def __init__(self, offsets, n_rows, n_groups):
-        self.offsets, self.n_rows, self.n_groups = offsets, n_rows, n_groups
+    def __init__(self, plan):
+        self.plan, self.n_rows, self.k, self.n_groups, self.device = plan, plan.pairs, 1, plan.n_groups, plan.device
+        self.offsets_ptr, self.order_ptr = plan.offsets_ptr, None
 
     @property
-    def device(self):
-        return self.offsets.device
+    def offsets(self):
+        return self.plan.offsets
 
 
 def route_rows(groups, n_groups):
@@ -986,18 +1006,16 @@ def route_rows(groups, n_groups):
     if not 1 <= n_groups <= _lib.MAX_GROUPS:
         raise ValueError(f"route_rows: n_groups must be 1 .. {_lib.MAX_GROUPS}, got {n_groups}")
     groups = groups.contiguous()
-    n, dev, lib = T * k, groups.device, _lib.load()
+    n, lib = T * k, _lib.load()
     need = lib.anerf_route_rows_workspace_size(n, n_groups)
     if need < 0:
         _lib.check(int(need), "anerf_route_rows_workspace_size")
     # one allocation: offsets | source | slot | workspace (every part starts on 16 bytes)
     no, ns = (n_groups + 4) // 4 * 4, (n + 3) // 4 * 4
-    buf = torch.empty(no + 2 * ns + (need + 3) // 4, dtype=torch.int32, device=dev)
-    offsets, source, slot, ws = buf[:n_groups + 1], buf[no:no + n], buf[no + ns:no + ns + n], buf[no + 2 * ns:]
-    with on_device(dev):
-        _lib.check(lib.anerf_route_rows(_p(groups), int(groups.dtype == torch.int64), n, n_groups, _p(offsets), _p(source), _p(slot), _p(ws), need,
-                                        _stream()), "anerf_route_rows")
-    return RowPlan(offsets, source, slot.view(groups.shape), T, k, n_groups)
+    plan = RowPlan(torch.empty(no + 2 * ns + (need + 3) // 4, dtype=torch.int32, device=groups.device), T, k, n_groups, groups.shape)
+    _launch(plan.device, lib.anerf_route_rows, "anerf_route_rows", groups.data_ptr(), groups.dtype == torch.int64, n, n_groups, plan.offsets_ptr,
+            plan.source_ptr, plan.slot_ptr, plan.slot_ptr + 4 * ns, need)
+    return plan
 
 
 def _row_weights(weights, plan):
@@ -1014,31 +1032,26 @@ def _rows_2d(t, n, name, dev):
     t = _rows_like(t, name, dev)
     if t.dim() < 1 or t.shape[0] != n:
         raise ValueError(f"{name}: {tuple(t.shape)} for a plan of {n} rows")
-    width = 1
-    for d in t.shape[1:]:
-        width *= d
-    return t.contiguous(), width
+    return t.contiguous(), math.prod(t.shape[1:])
 
 
 def dispatch_rows(x, plan, weights=None):
     """x [T, ...] -> [T * k, ...] in group order (times weights [T, k] if given); zero rows behind the kept ones"""
     x, width = _rows_2d(x, plan.n_rows, "dispatch_rows", plan.device)
     weights = _row_weights(weights, plan)
-    out = torch.empty((plan.n_rows * plan.k,) + tuple(x.shape[1:]), dtype=x.dtype, device=x.device)
-    with on_device(x.device):
-        _lib.check(_lib.load().anerf_dispatch_rows(_p(x), ROW_DTYPES[x.dtype], _p(weights), _p(plan.slot), _p(plan.offsets[-1:]), plan.n_rows, plan.k,
-                                                   width, _p(out), _stream()), "anerf_dispatch_rows")
+    out = torch.empty((plan.pairs,) + x.shape[1:], dtype=x.dtype, device=x.device)
+    _launch(x.device, _lib.load().anerf_dispatch_rows, "anerf_dispatch_rows", x.data_ptr(), ROW_DTYPES[x.dtype], _ptr(weights), plan.slot_ptr, plan.kept_ptr,
+            plan.n_rows, plan.k, width, out.data_ptr())
     return out
 
 
 def combine_rows(z, plan, weights=None):
     """z [T * k, ...] in group order -> [T, ...]: the sum of every row's kept entries (times weights [T, k] if given)"""
-    z, width = _rows_2d(z, plan.n_rows * plan.k, "combine_rows", plan.device)
+    z, width = _rows_2d(z, plan.pairs, "combine_rows", plan.device)
     weights = _row_weights(weights, plan)
-    y = torch.empty((plan.n_rows,) + tuple(z.shape[1:]), dtype=z.dtype, device=z.device)
-    with on_device(z.device):
-        _lib.check(_lib.load().anerf_combine_rows(_p(z), ROW_DTYPES[z.dtype], _p(weights), _p(plan.slot), _p(plan.offsets[-1:]), plan.n_rows, plan.k,
-                                                  width, _p(y), _stream()), "anerf_combine_rows")
+    y = torch.empty((plan.n_rows,) + z.shape[1:], dtype=z.dtype, device=z.device)
+    _launch(z.device, _lib.load().anerf_combine_rows, "anerf_combine_rows", z.data_ptr(), ROW_DTYPES[z.dtype], _ptr(weights), plan.slot_ptr, plan.kept_ptr,
+            plan.n_rows, plan.k, width, y.data_ptr())
     return y
 
 
@@ -1047,64 +1060,52 @@ def combine_rows_backward(dy, z, plan, weights, want_dz=True, want_dw=True):
     dy, width = _rows_2d(dy, plan.n_rows, "combine_rows_backward", plan.device)
     z = z.contiguous() if want_dw else None
     w = _row_weights(weights, plan)
-    dz = torch.empty((plan.n_rows * plan.k,) + tuple(dy.shape[1:]), dtype=dy.dtype, device=dy.device) if want_dz else None
+    dz = torch.empty((plan.pairs,) + dy.shape[1:], dtype=dy.dtype, device=dy.device) if want_dz else None
     dw = torch.empty(weights.shape, dtype=torch.float32, device=dy.device) if want_dw else None
-    with on_device(dy.device):
-        _lib.check(_lib.load().anerf_combine_rows_backward(_p(dy), _p(z), ROW_DTYPES[dy.dtype], _p(w), _p(plan.slot), _p(plan.offsets[-1:]), plan.n_rows,
-                                                           plan.k, width, _p(dz), _p(dw), _stream()), "anerf_combine_rows_backward")
+    _launch(dy.device, _lib.load().anerf_combine_rows_backward, "anerf_combine_rows_backward", dy.data_ptr(), _ptr(z), ROW_DTYPES[dy.dtype], _ptr(w),
+            plan.slot_ptr, plan.kept_ptr, plan.n_rows, plan.k, width, _ptr(dz), _ptr(dw))
     return dz, dw
 
 
 def _adapter_io(x, weight, down, up, rows, bias, scale, scale_of):
-    """AnerfAdapterIO of 2-D rows x (any row stride) + the tensors whose pointers it holds"""
-    io = _lib.AnerfAdapterIO()
-    io.dtype, io.n_adapters, io.rank, io.scale = ROW_DTYPES[x.dtype], down.shape[0], down.shape[1], float(scale)
-    io.n_rows, io.n_in, io.n_out, io.x_stride = x.shape[0], weight.shape[1], weight.shape[0], x.stride(0)
-    order = rows.source if isinstance(rows, RowPlan) else None
-    keep = [x, weight, down, up, bias, scale_of, None if rows is None else rows.offsets, order]
-    for name, t in zip(("x", "weight", "down", "up", "bias", "scale_of", "offsets", "order"), keep):
-        setattr(io, name, None if t is None else t.data_ptr())
-    return io, keep
+    """AnerfAdapterIO of 2-D rows x (any row stride); rows None: no plan.  The caller holds the tensors."""
+    return _lib.AnerfAdapterIO(ROW_DTYPES[x.dtype], down.shape[0], down.shape[1], scale, x.shape[0], weight.shape[1], weight.shape[0], x.stride(0),
+                               x.data_ptr(), weight.data_ptr(), _ptr(bias), down.data_ptr(), up.data_ptr(), _ptr(scale_of),
+                               None if rows is None else rows.offsets_ptr, None if rows is None else rows.order_ptr, None, None)
 
 
 def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=None):
     """x [M, K] W^T + bias + s_i (x A_i^T) B_i^T (anerf_adapter_linear) -> (y [M, N], h): h is what the backward needs.  weight [N, K],
     down [L, R, K] (A), up [L, N, R] (B), rows: RowPlan (k = 1) or SortedRows of the M rows over the L adapters."""
-    io, keep = _adapter_io(x, weight, down, up, rows, bias, scale, scale_of)
-    y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=x.device)
-    lib = _lib.load()
-    h, _ = _workspace(lib.anerf_adapter_h_size, "anerf_adapter_h_size", x.device, C.byref(io))
+    io, lib, dev = _adapter_io(x, weight, down, up, rows, bias, scale, scale_of), _lib.load(), x.device
+    ref = C.byref(io)
+    y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
+    h, _ = _workspace(lib.anerf_adapter_h_size, "anerf_adapter_h_size", dev, ref)
     io.y, io.h = y.data_ptr(), h.data_ptr()
-    with on_device(x.device):
-        need = lib.anerf_adapter_workspace_size(C.byref(io))
-        ws = torch.empty(need // 4, dtype=torch.float32, device=x.device) if need > 0 else None
-        _lib.check(lib.anerf_adapter_linear(C.byref(io), _p(ws), need, _stream()), "anerf_adapter_linear")
+    need = lib.anerf_adapter_workspace_size(ref)
+    ws = torch.empty(need // 4, dtype=torch.float32, device=dev) if need > 0 else None
+    _launch(dev, lib.anerf_adapter_linear, "anerf_adapter_linear", ref, _ptr(ws), need)
     return y, h
 
 
 def adapter_linear_few(x, weight, down, up, groups, bias=None, scale=1.0, scale_of=None):
     """adapter_linear of up to 64 rows with their adapter indices instead of a plan (anerf_adapter_linear_few) -> y [M, N]"""
-    io, keep = _adapter_io(x, weight, down, up, None, bias, scale, scale_of)
-    M, N, R = x.shape[0], weight.shape[0], down.shape[1]
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    h = torch.empty(M * R, dtype=torch.float32, device=x.device)
+    io, dev = _adapter_io(x, weight, down, up, None, bias, scale, scale_of), x.device
+    y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
+    h = torch.empty(x.shape[0] * down.shape[1], dtype=torch.float32, device=dev)
     io.y, io.h = y.data_ptr(), h.data_ptr()
-    with on_device(x.device):
-        _lib.check(_lib.load().anerf_adapter_linear_few(C.byref(io), _p(groups), int(groups.dtype == torch.int64), _stream()), "anerf_adapter_linear_few")
+    _launch(dev, _lib.load().anerf_adapter_linear_few, "anerf_adapter_linear_few", C.byref(io), groups.data_ptr(), groups.dtype == torch.int64)
     return y
 
 
 def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, want_dx=True, want_ddown=True, want_dup=True):
     """gradients of adapter_linear with weight and bias frozen (anerf_adapter_backward) -> (dx, ddown, dup), None where not wanted"""
-    io, keep = _adapter_io(x, weight, down, up, rows, None, scale, scale_of)
+    io, lib, dev = _adapter_io(x, weight, down, up, rows, None, scale, scale_of), _lib.load(), x.device
     io.h = h.data_ptr()
-    dx = torch.empty(x.shape[0], weight.shape[1], dtype=x.dtype, device=x.device) if want_dx else None
+    dx = torch.empty(x.shape[0], weight.shape[1], dtype=x.dtype, device=dev) if want_dx else None
     ddown = torch.empty_like(down) if want_ddown else None
     dup = torch.empty_like(up) if want_dup else None
-    go = _lib.AnerfAdapterGradIO(g.data_ptr(), g.stride(0), None if dx is None else dx.data_ptr(), None if ddown is None else ddown.data_ptr(),
-                                 None if dup is None else dup.data_ptr())
-    lib = _lib.load()
-    with on_device(x.device):
-        ws, nbytes = _workspace(lib.anerf_adapter_backward_workspace_size, "anerf_adapter_backward_workspace_size", x.device, C.byref(io))
-        _lib.check(lib.anerf_adapter_backward(C.byref(io), C.byref(go), _p(ws), nbytes, _stream()), "anerf_adapter_backward")
+    go = _lib.AnerfAdapterGradIO(g.data_ptr(), g.stride(0), _ptr(dx), _ptr(ddown), _ptr(dup))
+    ws, nbytes = _workspace(lib.anerf_adapter_backward_workspace_size, "anerf_adapter_backward_workspace_size", dev, C.byref(io))
+    _launch(dev, lib.anerf_adapter_backward, "anerf_adapter_backward", C.byref(io), C.byref(go), ws.data_ptr(), nbytes)
     return dx, ddown, dup
