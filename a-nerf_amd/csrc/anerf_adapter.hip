@@ -671,17 +671,34 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
 // BY_RANK: part [piece][Rp][C] (operand order Z, V), else [piece][C][Rp] (V, Z): a lane ends with four values that lie together.
 constexpr int TG_WAVES = 4, TG_COLS = 64, TG_DEPTH = 4;
 
+struct GradJob {
+  const void* Z;
+  const float* V;
+  float* part;
+  void* out;
+  long long ldz, C;
+  int rows, blocks, by_rank;          // rows of a piece; workgroups along the columns (the sum's: outputs / 64)
+};
+struct GradJobs {
+  GradJob j[2];
+  const int32_t *offsets, *order;
+  int L, R, Rp, ways;
+};
+
 template <int DT, int NJ, bool BY_RANK>
-__global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(const typename Elem<DT>::T* __restrict__ Z, long long ldz, const int32_t* __restrict__ order,
-                                                             const float* __restrict__ V, const int32_t* __restrict__ offsets, int L, long long C,
-                                                             int Rp, int rows, float* __restrict__ part) {
+__device__ __forceinline__ void thin_grad(const GradJobs& G, const GradJob& J, int bx, f32x4 (*red)[4 * NJ][64]) {
   typedef typename Elem<DT>::T E;
   typedef E vec __attribute__((ext_vector_type(4)));
-  __shared__ f32x4 red[TG_WAVES - 1][4 * NJ][64];
+  const E* Z = static_cast<const E*>(J.Z);
+  const float* V = J.V;
+  const int32_t* order = G.order;
+  float* part = J.part;
+  const long long ldz = J.ldz, C = J.C;
+  const int Rp = G.Rp;
   int a, p0, p1;
-  if (!find_piece(offsets, L, rows, blockIdx.y, a, p0, p1)) return;
+  if (!find_piece(G.offsets, G.L, J.rows, blockIdx.y, a, p0, p1)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-  const long long c = (long long)blockIdx.x * TG_COLS + 4 * i;
+  const long long c = (long long)bx * TG_COLS + 4 * i;
   const int j0 = blockIdx.z * 16 * NJ;
   const bool whole = c + 4 <= C;
   f32x4 acc[4][NJ];
@@ -736,7 +753,7 @@ __global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(const typename Elem
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int n = 0; n < NJ; ++n) acc[e][n] += red[w][e * NJ + n][lane];
-  const long long base = (long long)blockIdx.y * Rp * C, c0 = (long long)blockIdx.x * TG_COLS;
+  const long long base = (long long)blockIdx.y * Rp * C, c0 = (long long)bx * TG_COLS;
 #pragma unroll
   for (int n = 0; n < NJ; ++n) {
     if (j0 + 16 * n >= Rp) break;
@@ -755,32 +772,49 @@ __global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(const typename Elem
   }
 }
 
-// adds an adapter's pieces, wave w those of q = w mod 4 in order, then the four sums.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
-template <int DT, bool BY_RANK>
-__global__ void __launch_bounds__(256) k_thin_grad_sum(const float* __restrict__ part, const int32_t* __restrict__ offsets, int L, long long C, int R,
-                                                       int Rp, int rows, typename Elem<DT>::T* __restrict__ out) {
+template <int DT, int NJ>
+__global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(GradJobs G) {
+  __shared__ f32x4 red[TG_WAVES - 1][4 * NJ][64];
+  const int second = (int)blockIdx.x >= G.j[0].blocks;
+  const GradJob& J = G.j[second];
+  const int bx = (int)blockIdx.x - (second ? G.j[0].blocks : 0);
+  if (J.by_rank) thin_grad<DT, NJ, true>(G, J, bx, red);
+  else thin_grad<DT, NJ, false>(G, J, bx, red);
+}
+
+// adds an adapter's pieces in their order; many pieces an adapter (ways = 4): wave w those of q = w mod 4, then the four sums.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
+template <int DT>
+__global__ void __launch_bounds__(256) k_thin_grad_sum(GradJobs G) {
   typedef typename Elem<DT>::T E;
+  __shared__ float red[4][64];
+  const int second = (int)blockIdx.x >= G.j[0].blocks;
+  const GradJob& J = G.j[second];
+  const int bx = (int)blockIdx.x - (second ? G.j[0].blocks : 0), rows = J.rows;
   const int a = blockIdx.y, lane = threadIdx.x & 63;
   int first = 0;
-  for (int b = lane; b < a; b += 64) first += (offsets[b + 1] - offsets[b] + rows - 1) / rows;
+  for (int b = lane; b < a; b += 64) first += (G.offsets[b + 1] - G.offsets[b] + rows - 1) / rows;
 #pragma unroll
   for (int d = 32; d; d >>= 1) first += __shfl_xor(first, d);
-  const int n = (offsets[a + 1] - offsets[a] + rows - 1) / rows;
-  const long long all = C * R, stride = C * Rp;
-  __shared__ float red[4][64];
-  const int w = threadIdx.x >> 6;
-  for (long long e0 = (long long)blockIdx.x * 64; e0 < all; e0 += (long long)gridDim.x * 64) {
-    const long long e = e0 + lane;
+  const int n = (G.offsets[a + 1] - G.offsets[a] + rows - 1) / rows;
+  const long long all = J.C * G.R, stride = J.C * G.Rp;
+  E* out = static_cast<E*>(J.out) + a * all;
+  const int ways = G.ways, outs = 256 / ways, w = ways == 1 ? 0 : threadIdx.x >> 6, mine = ways == 1 ? threadIdx.x : lane;
+  for (long long e0 = (long long)bx * outs; e0 < all; e0 += (long long)J.blocks * outs) {
+    const long long e = e0 + mine;
     float v = 0.f;
     if (e < all) {
-      const float* src = part + first * stride + (BY_RANK ? e : e / R * Rp + e % R);
+      const float* src = J.part + first * stride + (J.by_rank ? e : e / G.R * G.Rp + e % G.R);
 #pragma unroll 4
-      for (int q = w; q < n; q += 4) v += src[q * stride];
+      for (int q = w; q < n; q += ways) v += src[q * stride];
+    }
+    if (ways == 1) {
+      if (e < all) out[e] = (E)v;
+      continue;
     }
     __syncthreads();
     red[w][lane] = v;
     __syncthreads();
-    if (w == 0 && e < all) out[(long long)a * all + e] = (E)(red[0][lane] + red[1][lane] + (red[2][lane] + red[3][lane]));
+    if (w == 0 && e < all) out[e] = (E)(red[0][lane] + red[1][lane] + (red[2][lane] + red[3][lane]));
   }
 }
 
@@ -794,9 +828,12 @@ struct TransposeJobs {
   TransposeJob j[3];
 };
 
+// 64 x 64 values a workgroup through LDS, 16 bytes a lane on both sides where the rows allow it
 template <typename U>
 __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
-  __shared__ U t[64][65];
+  constexpr int V = 16 / sizeof(U);
+  typedef U vec __attribute__((ext_vector_type(V)));
+  __shared__ U t[64][64 + 2];
   long long b = blockIdx.x;
   int k = 0;
   while (k < 2 && b >= J.j[k].tiles * J.j[k].batch) b -= J.j[k].tiles * J.j[k].batch, ++k;
@@ -804,12 +841,35 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   const U* in = static_cast<const U*>(T.in) + b / T.tiles * T.rows * T.cols;
   U* out = static_cast<U*>(T.out) + b / T.tiles * T.rows * T.cols;
   const long long r0 = b % T.tiles / T.tiles_c * 64, c0 = b % T.tiles % T.tiles_c * 64;
-  const int cx = threadIdx.x & 63, ry = threadIdx.x >> 6;
-  for (int r = ry; r < 64; r += 4)
-    if (r0 + r < T.rows && c0 + cx < T.cols) t[r][cx] = in[(r0 + r) * T.cols + c0 + cx];
+  constexpr int LANES = 64 / V;      // lanes of a row
+  const int x = threadIdx.x % LANES * V;
+  for (int r = threadIdx.x / LANES; r < 64; r += 256 / LANES) {
+    if (r0 + r >= T.rows) break;
+    const U* src = in + (r0 + r) * T.cols + c0 + x;
+    if (c0 + x + V <= T.cols) {
+      vec v;
+      __builtin_memcpy(&v, src, 16);
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[r][x + e] = v[e];
+    } else {
+      for (int e = 0; e < V; ++e)
+        if (c0 + x + e < T.cols) t[r][x + e] = src[e];
+    }
+  }
   __syncthreads();
-  for (int c = ry; c < 64; c += 4)
-    if (c0 + c < T.cols && r0 + cx < T.rows) out[(c0 + c) * T.rows + r0 + cx] = t[cx][c];
+  for (int c = threadIdx.x / LANES; c < 64; c += 256 / LANES) {
+    if (c0 + c >= T.cols) break;
+    U* dst = out + (c0 + c) * T.rows + r0 + x;
+    if (r0 + x + V <= T.rows) {
+      vec v;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = t[x + e][c];
+      __builtin_memcpy(dst, &v, 16);
+    } else {
+      for (int e = 0; e < V; ++e)
+        if (r0 + x + e < T.rows) dst[e] = t[x + e][c];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- launchers
@@ -989,31 +1049,42 @@ static BackwardPlan backward_plan(const AnerfAdapterIO& A) {
   B.u = at, at += up16(h_layout(A).bytes);
   const long long pa = part_floats(A.n_rows, A.n_adapters, A.n_in, Rp), pb = part_floats(A.n_rows, A.n_adapters, A.n_out, Rp);
   const long long pd = adapter_workspace(swapped(A));
-  B.part = at, at += up16(std::max(std::max(pa, pb) * 4, pd));
+  B.part = at, at += up16(std::max((pa + pb) * 4 + 512, pd));
   B.bytes = at;
   return B;
 }
 long long adapter_backward_workspace(const AnerfAdapterIO& A) { return backward_plan(A).bytes; }
 
-template <int DT, bool BY_RANK>
-static int thin_grad_t(const void* Z, long long ldz, const int32_t* order, const float* V, const AnerfAdapterIO& A, long long C, float* part, void* out,
-                       hipStream_t st) {
-  typedef typename Elem<DT>::T E;
-  const int Rp = (A.rank + 15) / 16 * 16, rows = grad_rows(A.n_rows, C, Rp);
-  const long long pieces = pieces_bound(A.n_rows, A.n_adapters, rows);
+// both sums of an adapter's gradient in one launch each (job 0: dA from (x, u), job 1: dB from (g, h); one of them may be off)
+template <int DT>
+static int thin_grads(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, const float* u, float* part, hipStream_t st) {
+  const int Rp = (A.rank + 15) / 16 * 16, nj = grad_ranks(Rp);
+  GradJobs J = {};
+  J.offsets = A.offsets, J.order = A.order, J.L = A.n_adapters, J.R = A.rank, J.Rp = Rp;
+  int n = 0;
+  long long pieces = 0;
+  auto add = [&](const void* Z, long long ldz, const float* V, long long C, void* out, int by_rank) {
+    const int rows = grad_rows(A.n_rows, C, Rp);
+    const long long mine = pieces_bound(A.n_rows, A.n_adapters, rows);
+    J.j[n++] = {Z, V, part, out, ldz, C, rows, (int)((C + TG_COLS - 1) / TG_COLS), by_rank};
+    part += (mine * Rp * C + 63) / 64 * 64;
+    pieces = std::max(pieces, mine);
+  };
+  if (G.ddown) add(A.x, A.x_stride, u, A.n_in, G.ddown, 1);
+  if (G.dup) add(G.g, G.g_stride, static_cast<const float*>(A.h), A.n_out, G.dup, 0);
+  if (n == 0) return ANERF_OK;
   if (pieces > 0) {
-    const int nj = grad_ranks(Rp);
-    const dim3 grid((unsigned)((C + TG_COLS - 1) / TG_COLS), (unsigned)pieces, (Rp + 16 * nj - 1) / (16 * nj));
-    auto run = [&](auto kernel) { kernel<<<grid, TG_WAVES * 64, 0, st>>>(static_cast<const E*>(Z), ldz, order, V, A.offsets, A.n_adapters, C, Rp, rows, part); };
-    if (nj == 1) run(k_thin_grad<DT, 1, BY_RANK>);
-    else if (nj == 2) run(k_thin_grad<DT, 2, BY_RANK>);
-    else run(k_thin_grad<DT, 4, BY_RANK>);
+    const dim3 grid((unsigned)(J.j[0].blocks + J.j[1].blocks), (unsigned)pieces, (Rp + 16 * nj - 1) / (16 * nj));
+    if (nj == 1) k_thin_grad<DT, 1><<<grid, TG_WAVES * 64, 0, st>>>(J);
+    else if (nj == 2) k_thin_grad<DT, 2><<<grid, TG_WAVES * 64, 0, st>>>(J);
+    else k_thin_grad<DT, 4><<<grid, TG_WAVES * 64, 0, st>>>(J);
     const int rc = check_launch("k_thin_grad");
     if (rc) return rc;
   }
-  const long long all = C * A.rank, bx = (all + 63) / 64;
-  k_thin_grad_sum<DT, BY_RANK><<<dim3((unsigned)(bx < 4096 ? bx : 4096), A.n_adapters), 256, 0, st>>>(part, A.offsets, A.n_adapters, C, A.rank, Rp, rows,
-                                                                                                   static_cast<E*>(out));
+  J.ways = pieces > 8ll * A.n_adapters ? 4 : 1;
+  const long long most = std::max(1, 4096 / A.n_adapters), outs = 256 / J.ways;
+  for (int k = 0; k < n; ++k) J.j[k].blocks = (int)std::min((J.j[k].C * A.rank + outs - 1) / outs, most);
+  k_thin_grad_sum<DT><<<dim3((unsigned)(J.j[0].blocks + J.j[1].blocks), A.n_adapters), 256, 0, st>>>(J);
   return check_launch("k_thin_grad_sum");
 }
 
@@ -1045,15 +1116,7 @@ static int backward_t(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, char
     rc = linear_t<DT>(T, ws + B.part, st);
     if (rc) return rc;
   }
-  if (G.ddown) {
-    const int rc = thin_grad_t<DT, true>(A.x, A.x_stride, A.order, u, A, A.n_in, part, G.ddown, st);
-    if (rc) return rc;
-  }
-  if (G.dup) {
-    const int rc = thin_grad_t<DT, false>(G.g, G.g_stride, A.order, static_cast<const float*>(A.h), A, A.n_out, part, G.dup, st);
-    if (rc) return rc;
-  }
-  return ANERF_OK;
+  return thin_grads<DT>(A, G, u, part, st);
 }
 
 int launch_adapter_backward(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, void* ws, hipStream_t st) {

@@ -12,7 +12,7 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int ROWS_MAX_GROUPS = 1024;   // a wave's group counters live in LDS: 8 waves x 1025 x 4 bytes
+constexpr int ROWS_MAX_GROUPS = 1024;   // every wave's group counters live in LDS: 18 x 1025 x 4 bytes
 constexpr int ANERF_MAX_RANK = 1024;
 constexpr int ROWS_MAX_CHOICES = 64;    // a token's slots sit in the lanes of one wave
 

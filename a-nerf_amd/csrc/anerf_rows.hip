@@ -10,8 +10,8 @@
 
 namespace anerf {
 
-constexpr int RT_WAVES = 8, RT_THREADS = RT_WAVES * 64;
-constexpr int RT_SINGLE = 4096;     // pairs that one workgroup sorts in one launch: 8 steps of 64 pairs a wave
+constexpr int RT_WAVES = 16, RT_THREADS = RT_WAVES * 64;
+constexpr int RT_SINGLE = 4096;     // pairs that one workgroup sorts in one launch: 4 steps of 64 pairs a wave
 constexpr int RT_MAX_BLOCKS = 256;
 
 template <typename I>
@@ -156,6 +156,8 @@ static int launch_route_t(const I* idx, long long n, int G, int32_t* offsets, in
   while ((1 << bits) <= G) ++bits;
   const int chunk = n ? route_chunk(n) : RT_THREADS;
   const unsigned lds = (RT_WAVES + 2) * (G + 1) * 4;
+  static unsigned long long done = 0;
+  ensure_dynamic_lds(reinterpret_cast<const void*>(k_route_place<I>), (RT_WAVES + 2) * (ROWS_MAX_GROUPS + 1) * 4, &done);
   if (n <= RT_SINGLE) {
     k_route_place<I><<<1, RT_THREADS, lds, st>>>(idx, n, G, chunk, bits, nullptr, offsets, source, slot);
   } else {
