@@ -347,9 +347,9 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   }
 
   // ---- x W^T
-  constexpr bool TWO = DT == ANERF_F32;
-  Acc sum[TWO ? MI : 1][TWO ? NI : 1];
-  if constexpr (TWO) {
+  constexpr bool F32 = DT == ANERF_F32;
+  Acc sum[F32 ? MI : 1][F32 ? NI : 1];
+  if constexpr (F32) {
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   for (int s = first; s < whole; s += 2) {
     stage(s, 0, Const<0>());
     if (s + 1 < whole) stage(s + 1, 1, Const<0>());
-    if constexpr (TWO) {
+    if constexpr (F32) {
       if ((s - first) % FOLD == FOLD - 2) {
 #pragma unroll
         for (int m = 0; m < MI; ++m)
@@ -436,47 +436,106 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   }
   if (DIRECT && full < stages) stage(full, (full - first) & 1, Const<1>());
 
-  // ---- bias, rounding, store: lane (i, q) holds outputs 8g + 4q .. +3 of its row, a group g of four registers of every block
-  const E* bias = static_cast<const E*>(P.bias);
+  // ---- bias, rounding, store.  A lane holds groups of four outputs of its row.  fp32: 16 bytes each, stored as they are
+  if constexpr (F32) {
+    const float* bias = static_cast<const float*>(P.bias);
 #pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    const long long p = m0 + wm * TM + BS * m + i;
-    if (p >= P.M) continue;
-    const long long row = P.order ? (long long)P.order[p] : p;
-    E* yr = static_cast<E*>(P.y) + row * P.N;
-    float* pr = P.part + (part * P.M + row) * P.N;
+    for (int m = 0; m < MI; ++m) {
+      const long long p = m0 + wm * TM + BS * m + i;
+      if (p >= P.M) continue;
+      const long long row = P.order ? (long long)P.order[p] : p;
+      float* yr = P.splits > 1 ? P.part + (part * P.M + row) * P.N : static_cast<float*>(P.y) + row * P.N;
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int g = 0; g < NV / 4; ++g) {
+          const long long col = n0 + wn * TN + BS * n + 8 * g + 4 * q;
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = acc[m][n][4 * g + e] + sum[m][n][4 * g + e];
+            if (bias && P.splits == 1 && col + e < P.N) v[e] += bias[col + e];
+          }
+          if (col + 4 <= P.N) {
+            store16(yr + col, __builtin_bit_cast(u32x4, v));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < P.N) yr[col + e] = v[e];
+          }
+        }
+    }
+    return;
+  }
+  // 16-bit types: through LDS, a wave's half of its rows at a time, to leave 16 bytes a lane along the rows (8 bytes a lane in 32-byte
+  // pieces straight from the registers: 8192 x 4096 outputs 6 us more)
+  auto emit = [&](auto one, auto* to, const E* bias) {
+    typedef decltype(one) S;
+    typedef S four __attribute__((ext_vector_type(4)));
+    constexpr int LINE = TN * (int)sizeof(S) + 16, ROWS = MG * BS, PER = 16 / (int)sizeof(S), LPR = TN / PER, RPI = 64 / LPR;
+    static_assert(NW * ROWS * LINE <= 2 * STAGE * 16 && ROWS % RPI == 0, "the staged rows fit where the stages were");
+    char* mine = reinterpret_cast<char*>(lds) + wave * (ROWS * LINE);
+    const long long cw = n0 + wn * TN;
+    const int r0 = lane / LPR, c = lane % LPR * PER;
+    float add[NI][NV];
 #pragma unroll
     for (int n = 0; n < NI; ++n)
 #pragma unroll
-      for (int g = 0; g < NV / 4; ++g) {
-        const long long col = n0 + wn * TN + BS * n + 8 * g + 4 * q;
-        float v[4];
+      for (int e = 0; e < NV; ++e) {
+        const long long col = cw + BS * n + 8 * (e / 4) + 4 * q + e % 4;
+        add[n][e] = bias && col < P.N ? (float)bias[col] : 0.f;
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = acc[m][n][4 * g + e];
-          if constexpr (TWO) v[e] += sum[m][n][4 * g + e];
-        }
-        typedef E out4 __attribute__((ext_vector_type(4)));
-        if (P.splits > 1) {
+    for (int g = 0; g < 2; ++g) {
+      const long long pw = m0 + wm * TM + g * ROWS;
+      long long row[ROWS / RPI];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col + e < P.N) pr[col + e] = v[e];
-        } else if (col + 4 <= P.N) {
-          if (bias) {
+      for (int t = 0; t < ROWS / RPI; ++t) {
+        const long long p = pw + t * RPI + r0;
+        row[t] = p < P.M ? (P.order ? (long long)P.order[p] : p) : -1;
+      }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += (float)bias[col + e];
+      for (int m = 0; m < MG; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+          for (int k = 0; k < NV / 4; ++k) {
+            four o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float v = acc[g * MG + m][n][4 * k + e];
+              o[e] = (S)(bias ? v + add[n][4 * k + e] : v);
+            }
+            *reinterpret_cast<four*>(mine + (BS * m + i) * LINE + (BS * n + 8 * k + 4 * q) * (int)sizeof(S)) = o;
           }
-          out4 o;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the wave's own lines: no barrier
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = (E)v[e];
-          __builtin_memcpy(yr + col, &o, sizeof(o));
-        } else {
+      for (int t = 0; t < ROWS / RPI; ++t) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + (t * RPI + r0) * LINE + c * (int)sizeof(S));
+        S* o = to + row[t] * P.N + cw + c;
+        if (row[t] >= 0) {
+          if (cw + c + PER <= P.N) {
+            store16(o, v);
+          } else {
+            typedef S vec __attribute__((ext_vector_type(PER)));
+            const vec w = __builtin_bit_cast(vec, v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col + e < P.N) yr[col + e] = (E)(bias ? v[e] + (float)bias[col + e] : v[e]);
+            for (int e = 0; e < PER; ++e)
+              if (cw + c + e < P.N) o[e] = w[e];
+          }
         }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  };
+  __syncthreads();                           // every wave is done with the stages
+  if constexpr (!F32 && BM == 64 && BN == 64) {
+    if (P.splits > 1) {
+      emit(0.f, P.part + part * P.M * P.N, static_cast<const E*>(nullptr));
+      return;
+    }
   }
+  if constexpr (!F32) emit(E(), static_cast<E*>(P.y), static_cast<const E*>(P.bias));
 }
 
 // y = the parts' sum in order + bias; [M][N] as one row of values
@@ -899,8 +958,9 @@ static int split_of(int dtype, long long M, long long K, long long N) {
 
 // Tile: the larger, the fewer LDS reads a product (a 256 x 256 tile's waves read 3/8 of what a 64 x 64 tile's do), but the tiles of one CU
 // run one after the other, and what the last round leaves idle grows.  Cost: tiles of the busiest CU x size / rate; the rates are
-// what the tiles reach where there are many of them, relative to 256 x 256 (bf16, 8192 x 4096 x 4096: 256 x 256 274 us, 128 x 128 318, 128 x 64
-// 368, 64 x 64 446).  fp32 is bound by its products, and one size is as fast as the other (1941 .. 2009 us).
+// what the tiles reach where there are many of them, relative to 256 x 128 (bf16, 8192 x 4096 x 4096, rank 8: 256 x 256 271 us, 256 x 128 307,
+// 128 x 128 310, 128 x 64 360, 64 x 64 432; 1000 x 1000 x 1000: 45, 29, 25, 19, 16).  fp32 is bound by its products, and one size is as fast
+// as the other (1941 .. 2009 us).
 template <int DT>
 static int launch_main(const MainArgs& P, hipStream_t st) {
   constexpr long long es = sizeof(typename Elem<DT>::T), span = 1ll << 32;      // DIRECT's offsets have 32 bits
@@ -908,7 +968,7 @@ static int launch_main(const MainArgs& P, hipStream_t st) {
                       P.M * P.ldx * es < span && P.N * P.K * es < span;
   auto cost = [&](int bm, int bn, double rate, bool few_waves) {
     const long long tiles = (P.M + bm - 1) / bm * ((P.N + bn - 1) / bn), mine = (tiles + 255) / 256;
-    return (double)mine * bm * bn / (few_waves && mine == 1 ? 0.85 * rate : rate);      // (one wave a SIMD does not hide its own waits)
+    return (double)mine * bm * bn / (few_waves && mine == 1 ? 0.7 * rate : rate);      // (one wave a SIMD does not hide its own waits)
   };
   constexpr bool F32 = DT == ANERF_F32;
   const double c64 = cost(64, 64, F32 ? 0.97 : 0.6, true), c128 = cost(128, 128, F32 ? 1.0 : 0.87, true);
