@@ -20,17 +20,26 @@ namespace anerf {
 // piece in MFMA accumulators, fed straight from memory: a row of A serves 32 rows of x, and nothing is read twice from HBM.
 // Kept as [position][Rp] fp32 (Rp = rank rounded up to 16, zeros behind the rank) for the gradient of B, and, for the 16-bit types, as what
 // k_main multiplies with: the nearest value hi and the rest lo, [hi of 16 ranks | lo of the same 16] per 16 ranks, which meet [B | B]
-// there -- h keeps 16 (bf16) or 21 (fp16) of its bits.  fp16's range does not hold every h: k_split_rows scales its rows first.
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-template <typename E, typename V4>
-__device__ __forceinline__ void split4(f32x4 v, V4& hi, V4& lo) {
+// there -- h keeps 16 (bf16) or 21 (fp16) of its bits.  fp16's range does not hold every h: its rows are scaled first.
+// ranks j .. j+3 of a row
+template <typename E>
+__device__ __forceinline__ void store_split(f32x4 v, E* row, int j) {
+  typedef E four __attribute__((ext_vector_type(4)));
+  four hi, lo;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     hi[e] = (E)v[e];
     const float rest = v[e] - (float)hi[e];
     lo[e] = __builtin_isfinite((float)hi[e]) ? (E)rest : (E)0.f;       // (infinity and NaN are carried by hi alone)
   }
+  E* o = row + 2 * (j & ~15) + (j & 15);
+  *reinterpret_cast<four*>(o) = hi;
+  *reinterpret_cast<four*>(o + 16) = lo;
+}
+
+// a row of h is divided by the power of two that brings its largest value into [1, 2); rows of zeros, infinities and NaN stay
+__device__ __forceinline__ int row_exponent(float big) {
+  return big > 0.f && __builtin_isfinite(big) ? min(max(ilogbf(big), -100), 100) : 0;
 }
 
 constexpr int TH_ROWS = 32, TH_WAVES = 4, TH_DEPTH = 4;
@@ -42,7 +51,7 @@ template <int DT, int NJ>
 __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const int32_t* __restrict__ order,
                                                         const typename Elem<DT>::T* __restrict__ down, const int32_t* __restrict__ offsets,
                                                         int L, long long K, int R, int Rp, const float* __restrict__ scale_of, float scale,
-                                                        float* __restrict__ h, typename Elem<DT>::T* __restrict__ split) {
+                                                        float* __restrict__ h, typename Elem<DT>::T* __restrict__ split, float* __restrict__ factor) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
   __shared__ f32x4 red[TH_WAVES][2 * NJ][64];
@@ -109,27 +118,50 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
 #pragma unroll
     for (int n = 0; n < NJ; ++n) red[wave][m * NJ + n][lane] = acc[m][n];
   __syncthreads();
+  constexpr int LINE = 16 * NJ + 4;
+  __shared__ float tile[TH_ROWS * LINE];            // the piece's h, row by row
   for (int f = wave; f < 2 * NJ; f += TH_WAVES) {
     f32x4 v = red[0][f][lane];
 #pragma unroll
     for (int w = 1; w < TH_WAVES; ++w) v += red[w][f][lane];
-    const int p = p0 + 16 * (f / NJ) + i, j = j0 + 16 * (f % NJ) + 4 * q;
-    if (p < p1 && j < Rp) {
+    *reinterpret_cast<f32x4*>(tile + (16 * (f / NJ) + i) * LINE + 16 * (f % NJ) + 4 * q) = v;
+  }
+  __syncthreads();
+  // eight lanes a row, four ranks each and turn
+  const int r = threadIdx.x >> 3, part = threadIdx.x & 7, p = p0 + r;
+  if (p >= p1) return;
+  f32x4 v[(4 * NJ + 7) / 8];
+  float big = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = j + e < R ? v[e] * s_a : 0.f;      // ranks of the padding: zero
-      *reinterpret_cast<f32x4*>(h + (long long)p * Rp + j) = v;
-      if constexpr (DT == ANERF_BF16) {
-        bf16x4 hi, lo;
-        split4<E, bf16x4>(v, hi, lo);
-        E* o = split + (long long)p * 2 * Rp + 2 * (j & ~15) + (j & 15);
-        *reinterpret_cast<bf16x4*>(o) = hi;
-        *reinterpret_cast<bf16x4*>(o + 16) = lo;
-      }
+  for (int t = 0; t < (4 * NJ + 7) / 8; ++t) {
+    const int j = 4 * (part + 8 * t);
+    if (j >= 16 * NJ || j0 + j >= Rp) continue;
+    v[t] = *reinterpret_cast<const f32x4*>(tile + r * LINE + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[t][e] = j0 + j + e < R ? v[t][e] * s_a : 0.f;          // ranks of the padding: zero
+      big = fmaxf(big, fabsf(v[t][e]));
     }
+    *reinterpret_cast<f32x4*>(h + (long long)p * Rp + j0 + j) = v[t];
+  }
+  if constexpr (DT == ANERF_F32) return;
+  if (DT == ANERF_F16 && gridDim.y > 1) return;                // (k_split_rows needs the whole row)
+  float shrink = 1.f;
+  if constexpr (DT == ANERF_F16) {
+#pragma unroll
+    for (int d = 4; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d));
+    const int e = row_exponent(big);
+    shrink = ldexpf(1.f, -e);
+    if (part == 0) factor[p] = ldexpf(1.f, e);
+  }
+#pragma unroll
+  for (int t = 0; t < (4 * NJ + 7) / 8; ++t) {
+    const int j = 4 * (part + 8 * t);
+    if (j < 16 * NJ && j0 + j < Rp) store_split<E>(v[t] * shrink, split + (long long)p * 2 * Rp, j0 + j);
   }
 }
 
-// fp16: a row of h is divided by the power of two that brings its largest value into [1, 2) before it is split
+// fp16 with more ranks than a workgroup of k_thin holds: the rows' scaling and splitting
 __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h, const int32_t* __restrict__ kept, int Rp, _Float16* __restrict__ split,
                                                     float* __restrict__ factor) {
   const int p = blockIdx.x * 16 + (threadIdx.x >> 4), i = threadIdx.x & 15;
@@ -139,18 +171,10 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
   for (int j = i; j < Rp; j += 16) big = fmaxf(big, fabsf(r[j]));
 #pragma unroll
   for (int d = 8; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d));
-  int e = 0;
-  if (big > 0.f && __builtin_isfinite(big)) e = min(max(ilogbf(big), -100), 100);
+  const int e = row_exponent(big);
   if (i == 0) factor[p] = ldexpf(1.f, e);
   const float down = ldexpf(1.f, -e);
-  for (int j = 4 * i; j < Rp; j += 64) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(r + j) * down;
-    f16x4 hi, lo;
-    split4<_Float16, f16x4>(v, hi, lo);
-    _Float16* o = split + (long long)p * 2 * Rp + 2 * (j & ~15) + (j & 15);
-    *reinterpret_cast<f16x4*>(o) = hi;
-    *reinterpret_cast<f16x4*>(o + 16) = lo;
-  }
+  for (int j = 4 * i; j < Rp; j += 64) store_split<_Float16>(*reinterpret_cast<const f32x4*>(r + j) * down, split + (long long)p * 2 * Rp, j);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ y = x W^T ...
@@ -574,6 +598,12 @@ __global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ par
 //               operands (W is read once, no LDS on its way), x comes from L2, and the waves' sums are added through LDS.  The low-rank term of
 //               an output is a dot of `rank` values in fp32, read in front of the loop, so that B's latency hides behind W's.
 constexpr int FEW_WAVES = 8;
+#ifndef FEW_DEPTH
+#define FEW_DEPTH (MT * NT >= 4 ? 2 : 4)
+#endif
+#ifndef FEW_WIDE
+#define FEW_WIDE 8192
+#endif
 static_assert(ANERF_FEW_ROWS == 64, "four blocks of 16 rows");
 
 template <typename I>
@@ -617,7 +647,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
                                                         const void* __restrict__ groups, int wide, int L, int M, long long K, long long N, int R,
                                                         const float* __restrict__ h, typename Elem<DT>::T* __restrict__ y) {
   typedef typename Elem<DT>::T E;
-  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, DEPTH = MT * NT >= 4 ? 2 : 4;
+  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, DEPTH = FEW_DEPTH;
   typedef E vec __attribute__((ext_vector_type(EPC)));
   constexpr int OUT = 16 * NT, VALUES = OUT * 16 * MT, MINE = (VALUES + FEW_WAVES * 64 - 1) / (FEW_WAVES * 64);
   __shared__ f32x4 red[FEW_WAVES / 2][MT * NT][64];
@@ -639,7 +669,11 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
     for (; j + EPC <= R; j += EPC) {
       const vec b = __builtin_bit_cast(vec, load16(br + j));
 #pragma unroll
-      for (int e = 0; e < EPC; ++e) thin[t] = fmaf(hr[j + e], (float)b[e], thin[t]);
+      for (int e = 0; e < EPC; e += 4) {
+        const f32x4 hv = __builtin_bit_cast(f32x4, load16(hr + j + e));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) thin[t] = fmaf(hv[k], (float)b[e + k], thin[t]);
+      }
     }
     for (; j < R; ++j) thin[t] = fmaf(hr[j], (float)br[j], thin[t]);
   }
@@ -1019,13 +1053,13 @@ static int linear_t(const AnerfAdapterIO& A, void* ws, hipStream_t st) {
   float* factor = reinterpret_cast<float*>(static_cast<char*>(A.h) + H.factor);
   auto thin = [&](auto kernel, int parts) {
     kernel<<<dim3((unsigned)pieces, parts), TH_WAVES * 64, 0, st>>>(static_cast<const E*>(A.x), A.x_stride, A.order, static_cast<const E*>(A.down), A.offsets,
-                                                                  A.n_adapters, A.n_in, A.rank, Rp, A.scale_of, A.scale, h, split);
+                                                                  A.n_adapters, A.n_in, A.rank, Rp, A.scale_of, A.scale, h, split, factor);
   };
   if (Rp <= 16) thin(k_thin<DT, 1>, 1);
   else if (Rp <= 32) thin(k_thin<DT, 2>, 1);
   else thin(k_thin<DT, 4>, (Rp + 63) / 64);
   if constexpr (DT == ANERF_F16) {
-    if (A.y) k_split_rows<<<(unsigned)((A.n_rows + 15) / 16), 256, 0, st>>>(h, A.offsets + A.n_adapters, Rp, split, factor);
+    if (A.y && Rp > 64) k_split_rows<<<(unsigned)((A.n_rows + 15) / 16), 256, 0, st>>>(h, A.offsets + A.n_adapters, Rp, split, factor);
   }
   const int rc = check_launch("k_thin");
   if (rc || !A.y) return rc;       // (the gradient of A alone needs h only)
@@ -1060,7 +1094,7 @@ static int few_t(const AnerfAdapterIO& A, const void* groups, int wide, hipStrea
                                                                           A.rank, h, static_cast<E*>(A.y));
   };
   // 32 outputs a workgroup halve what x costs in L2 traffic, where they still fill the chip
-  const bool wide_out = A.n_out >= 8192;
+  const bool wide_out = A.n_out >= FEW_WIDE;
   if (M <= 16) wide_out ? run(k_few<DT, 1, 2>, 32) : run(k_few<DT, 1, 1>, 16);
   else if (M <= 32) wide_out ? run(k_few<DT, 2, 2>, 32) : run(k_few<DT, 2, 1>, 16);
   else wide_out ? run(k_few<DT, 4, 2>, 32) : run(k_few<DT, 4, 1>, 16);
