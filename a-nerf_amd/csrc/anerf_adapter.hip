@@ -594,16 +594,10 @@ __global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ par
 // -------------------------------------------------------------------------------------------------------- few rows (a decoding step)
 // Up to 64 rows, each with an adapter index of its own, no plan: the time is what the shared weight takes to arrive.
 //   k_few_thin  h[r][j] = s_i <x[r], A_i[j]>: one wave a value
-//   k_few       a workgroup owns 16*NT outputs of all rows; its eight waves take every eighth 64-byte step of W's rows straight into MFMA
-//               operands (W is read once, no LDS on its way), x comes from L2, and the waves' sums are added through LDS.  The low-rank term of
+//   k_few       a workgroup owns 16*NT outputs of all rows; its eight waves take every eighth 128 bytes of W's rows straight into MFMA operands
+//               (W is read once, no LDS on its way), x comes from L2, and the waves' sums are added through LDS.  The low-rank term of
 //               an output is a dot of `rank` values in fp32, read in front of the loop, so that B's latency hides behind W's.
 constexpr int FEW_WAVES = 8;
-#ifndef FEW_DEPTH
-#define FEW_DEPTH (MT * NT >= 4 ? 2 : 4)
-#endif
-#ifndef FEW_WIDE
-#define FEW_WIDE 8192
-#endif
 static_assert(ANERF_FEW_ROWS == 64, "four blocks of 16 rows");
 
 template <typename I>
@@ -647,7 +641,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
                                                         const void* __restrict__ groups, int wide, int L, int M, long long K, long long N, int R,
                                                         const float* __restrict__ h, typename Elem<DT>::T* __restrict__ y) {
   typedef typename Elem<DT>::T E;
-  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, DEPTH = FEW_DEPTH;
+  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, DEPTH = MT * NT >= 4 ? 2 : 4;
   typedef E vec __attribute__((ext_vector_type(EPC)));
   constexpr int OUT = 16 * NT, VALUES = OUT * 16 * MT, MINE = (VALUES + FEW_WAVES * 64 - 1) / (FEW_WAVES * 64);
   __shared__ f32x4 red[FEW_WAVES / 2][MT * NT][64];
@@ -696,7 +690,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
     u32x4 wv[D][NT], xv[D][MT];
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      const long long k = (s0 + d * FEW_WAVES) * STEP + q * EPC;
+      const long long k = (s0 + (d >> 1) * 2 * FEW_WAVES + (d & 1)) * STEP + q * EPC;
 #pragma unroll
       for (int n = 0; n < NT; ++n) wv[d][n] = decltype(tail)::value ? load_tail<DT>(wr[n], k, K) : load16(wr[n] + k);
 #pragma unroll
@@ -712,10 +706,13 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
           for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(wv[d][n], xv[d][m], acc[m][n], e);
   };
   const long long steps = K / STEP;
-  long long s = wave;
-  for (; s + (DEPTH - 1) * FEW_WAVES < steps; s += DEPTH * FEW_WAVES) walk(s, Const<DEPTH>(), Const<0>());
-  for (; s < steps; s += FEW_WAVES) walk(s, Const<1>(), Const<0>());
-  if (steps * STEP < K && wave == (int)(steps % FEW_WAVES)) walk(steps, Const<1>(), Const<1>());
+  long long s = 2 * wave;
+  for (; s + (DEPTH - 2) * FEW_WAVES + 1 < steps; s += DEPTH * FEW_WAVES) walk(s, Const<DEPTH>(), Const<0>());
+  for (; s < steps; s += 2 * FEW_WAVES) {
+    walk(s, Const<1>(), Const<0>());
+    if (s + 1 < steps) walk(s + 1, Const<1>(), Const<0>());
+  }
+  if (steps * STEP < K && wave == (int)(steps % (2 * FEW_WAVES)) / 2) walk(steps, Const<1>(), Const<1>());
   // 8 -> 4 -> 2 -> 1 waves
 #pragma unroll
   for (int half = FEW_WAVES / 2; half; half >>= 1) {
@@ -1094,9 +1091,10 @@ static int few_t(const AnerfAdapterIO& A, const void* groups, int wide, hipStrea
                                                                           A.rank, h, static_cast<E*>(A.y));
   };
   // 32 outputs a workgroup halve what x costs in L2 traffic, where they still fill the chip
-  const bool wide_out = A.n_out >= FEW_WIDE;
+  const bool wide_out = A.n_out >= 8192;
   if (M <= 16) wide_out ? run(k_few<DT, 1, 2>, 32) : run(k_few<DT, 1, 1>, 16);
   else if (M <= 32) wide_out ? run(k_few<DT, 2, 2>, 32) : run(k_few<DT, 2, 1>, 16);
+  else if (M <= 48) wide_out ? run(k_few<DT, 3, 2>, 32) : run(k_few<DT, 3, 1>, 16);
   else wide_out ? run(k_few<DT, 4, 2>, 32) : run(k_few<DT, 4, 1>, 16);
   return check_launch("k_few");
 }
