@@ -294,6 +294,72 @@ def _net_params(net):
     return out
 
 
+ENCODE_POINTS = 1 << 18      # sample points of one pass of encode_rows (its saved planes take 14 KB a point)
+
+
+@torch.no_grad()
+def encode_rows(net, kw, z):
+    """The encoded network input of the sample points (rays, z [N,S]) as rows [N*S, input width] in the reference's column order
+    (encode_inputs, raycasters.py:476-577): what the training forward saves for its backward, columns put back, --freq_schedule factors
+    and the frame-code column applied.  No gradient to the poses."""
+    cfg, rays, dev = kw["cfg"], kw["ray_batch"], kw["ray_batch"].device
+    skts = ops._f32c(ops.first_row(kw["skts"]), "skts")
+    n, s = z.shape
+    codes = None if not net.use_framecode else net.framecodes.codes.weight.detach()
+    cam = None if codes is None else kw["cam_idx"].reshape(-1).expand(n).contiguous()
+    out = torch.empty(n * s, cfg.x_width, dtype=torch.float32, device=dev)
+    packed, aux = net.packed(0)
+    px, pu = (t.long() for t in perm_tables(cfg, dev))
+    cc = cfg.c()
+    step = max(1, ENCODE_POINTS // s)
+    for a in range(0, n, step):
+        b = min(n, a + step)
+        P = (b - a) * s
+        T = train_layout(cfg, P)
+        # (rows behind the samples are not read here, so nothing is zeroed)
+        h, f, g, x, u = (torch.empty(T.p_pad * w, dtype=torch.float32, device=dev) for w in (8 * 256, 256, 128, T.x_width, T.u_width))
+        st = _lib.AnerfSaved(_p(h), _p(f), _p(g), _p(x), _p(u), T.p_pad)
+        raw = torch.empty(P, 4, dtype=torch.float32, device=dev)
+        rb, zz = rays[a:b], z[a:b].contiguous()
+        sk = skts if skts.shape[0] == 1 else skts[a:b]
+        # (the fused network's own output is not used: any code row will do for it, eval mode's extra mean-code row is not in this table)
+        cm = None if cam is None else cam[a:b].clamp(0, codes.shape[0] - 1)
+        _lib.check(_lib.load().anerf_mlp_raw_train(
+            C.byref(cc), _p(packed), _p(aux), _p(rb), rays.shape[1], _p(zz), _p(sk), 0 if sk.shape[0] == 1 else 16 * cfg.n_joints, _p(cm), _p(codes),
+            0 if codes is None else codes.shape[0], float(kw["tau_v"]), float(kw["tau_d"]), _p(kw["cut_v"]), _p(kw["cut_d"]), b - a, s, _p(raw),
+            C.byref(st), _stream()), "anerf_mlp_raw_train")
+        o = out[a * s:b * s]
+        o[:, px] = x.view(T.p_pad, -1)[:P]
+        o[:, cfg.dim_x + pu[:cfg.dim_d]] = u.view(T.p_pad, -1)[:P, :cfg.dim_d]
+        if cm is not None:
+            o[:, -1] = cam[a:b, None].expand(b - a, s).reshape(-1)
+    sched = net.input_schedule()
+    if sched is not None:
+        out[:, :cfg.dim_x] *= sched.sx
+        out[:, cfg.dim_x:cfg.dim_x + cfg.dim_d] *= sched.su[:cfg.dim_d]
+    return out
+
+
+def render_rays_adapted(caster, kw, subject_idxs):
+    """RayCaster.render_rays with a subject per ray (subject_idxs [N] or [1]) and adapters on both networks: the staged passes with the
+    adapted network (adapters.NetAdapters) in the place of the fused one.  Gradients reach the adapters (and the frame codes); the shared
+    weights are frozen and the poses are constants."""
+    n = kw["ray_batch"].shape[0]
+    if torch.is_grad_enabled() and kw["skts"].requires_grad:
+        raise NotImplementedError("subject_idxs: the adapted network gives the poses no gradient (detach skts)")
+    if kw.get("pts_noise") is not None:
+        raise NotImplementedError("subject_idxs with sample-point offsets (ray_noise_std > 0)")
+    if not torch.is_tensor(subject_idxs) or subject_idxs.dtype not in (torch.int32, torch.int64) or subject_idxs.numel() not in (1, n):
+        raise ValueError(f"subject_idxs: one int32 / int64 subject per ray, got {getattr(subject_idxs, 'shape', type(subject_idxs))} for {n} rays")
+    subject = subject_idxs.reshape(-1).to(kw["ray_batch"].device)
+    kw = dict(kw, cyls=kw["cyls"].expand(n, 5))
+
+    def mlp(net, zz):
+        idx = subject.reshape(-1, 1).expand(n, zz.shape[1]).reshape(-1)
+        return net(encode_rows(net, kw, zz), subject_idxs=idx).view(n, zz.shape[1], 4)
+    return _staged(caster, kw, mlp)
+
+
 def render_rays_train(caster, kw):
     """Differentiable RayCaster.render_rays (raycasters.py:361-474); kw as assembled by RayCaster.render_rays."""
     cfg, rays, skts, cyls = kw["cfg"], kw["ray_batch"], kw["skts"], kw["cyls"]
@@ -307,9 +373,6 @@ def render_rays_train(caster, kw):
     if kw.get("pts_noise") is not None:
         raise NotImplementedError("ray_noise_std > 0 trains through the one-call route (two-network configurations)")
     skts_c = skts.contiguous()
-    with torch.no_grad():
-        nf_raw, stats = ops.ray_bounds(rays, cyls)
-        z, _ = ops.coarse_z(nf_raw, stats, rays, S, kw["t_rand"], kw["lindisp"])
 
     def mlp(net, zz):
         codes = _codes_with_grad(net)
@@ -319,6 +382,18 @@ def render_rays_train(caster, kw):
                     packed=net.packed(0) if prec == "fp32" else None, packed_t=net.packed(4 if prec == "bf16x3" else 1), packed_i=lambda: net.packed(5 if prec == "bf16x3" else 2),
                     precision=prec, packed_b3=net.packed(3) if prec == "bf16x3" else None, sched=net.input_schedule())
         return _MlpRawFn.apply(meta, skts_c, codes, *_net_params(net))
+
+    return _staged(caster, kw, mlp)
+
+
+def _staged(caster, kw, mlp):
+    """render_rays pass by pass: mlp(net, depths [N,S]) -> raw [N,S,4]"""
+    cfg, rays, cyls = kw["cfg"], kw["ray_batch"], kw["cyls"]
+    S, Ni = kw["n_samples"], kw["n_importance"]
+    net_c, net_f = caster.network, caster.network_fine
+    with torch.no_grad():
+        nf_raw, stats = ops.ray_bounds(rays, cyls)
+        z, _ = ops.coarse_z(nf_raw, stats, rays, S, kw["t_rand"], kw["lindisp"])
 
     def comp(raw, zz, noise):
         return _CompositeFn.apply(dict(cfg=cfg, rays=rays, z=zz, noise=noise), raw)

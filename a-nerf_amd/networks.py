@@ -198,13 +198,16 @@ class NeRF(nn.Module):
         self.__dict__["_adapters"] = adapters
         return self
 
+    def adapters(self):
+        return self.__dict__.get("_adapters")
+
     def forward(self, x, subject_idxs=None, subject_weights=None):
         """x [..., input_ch+input_ch_bones+input_ch_views(+1)] -> [..., 4]   (nerf.py:133-148).
         subject_idxs [...] or [..., k]: the subject(s) of every row, with attached adapters (set_adapters)."""
         if subject_idxs is not None:
-            if self.__dict__.get("_adapters") is None:
+            if self.adapters() is None:
                 raise ValueError("NeRF.forward: subject_idxs without adapters (NeRF.set_adapters)")
-            return self._adapters(self, x, subject_idxs, subject_weights)
+            return self.adapters()(self, x, subject_idxs, subject_weights)
         stream, aux = self.packed(fold=False)
         codes = self.framecodes.codes.weight if self.use_framecode else None
         if self.use_framecode and not self.training:

@@ -60,6 +60,16 @@ class RayCaster(nn.Module):
         self.train_precision = "fp32"
         self.train_route = "one_call"          # "staged": compose the per-stage autograd nodes instead (same kernels; tests)
 
+    def set_adapters(self, adapters, adapters_fine=None):
+        """adapters.NetAdapters of the coarse and of the fine network (None: detach both): render_rays(subject_idxs=...) then gives every ray
+        its subject's adapter.  They are not part of this module's parameters or checkpoint: save and step them by themselves."""
+        if adapters is not None and self.network_fine is not None and self.network_fine is not self.network and adapters_fine is None:
+            raise ValueError("set_adapters: this caster has a fine network, which needs adapters of its own")
+        self.network.set_adapters(adapters)
+        if self.network_fine is not None and self.network_fine is not self.network:
+            self.network_fine.set_adapters(adapters_fine if adapters is not None else None)
+        return self
+
     @torch.no_grad()
     def forward_eval(self, *args, **kwargs):
         return self.render_rays(*args, **kwargs)
@@ -159,7 +169,8 @@ class RayCaster(nn.Module):
         """Same arguments and returned dict as core/raycasters.py:361-474."""
         if skts is None or cyls is None:
             raise ValueError("skts and cyls are required (world->bone transforms and bounding cylinders)")
-        if subject_idxs is not None:
+        adapted = subject_idxs is not None and self.network.adapters() is not None
+        if subject_idxs is not None and not adapted:
             # the reference's own NeRF.forward rejects the extra input column encode_inputs appends for it
             # (torch.split sizes, nerf.py:135-137 vs raycasters.py:545-548): no network in the repository consumes it
             raise NotImplementedError("subject_idxs: no network of the reference consumes the subject column")
@@ -209,6 +220,9 @@ class RayCaster(nn.Module):
                   n_importance=N_importance, tau_v=tau_v, tau_d=tau_d, cut_v=cut_v, cut_d=cut_d,
                   cam_idx=cam_c if cam_c is not None else cam_idx, t_rand=t_rand, u_imp=u_imp, noise=noise,
                   noise_fine=noise_f, lindisp=lindisp, single_net=self.single_net, pts_noise=pts_noise, pts_noise_is=pts_noise_is)
+        if adapted:
+            from . import autograd_path
+            return autograd_path.render_rays_adapted(self, kw, subject_idxs)
         needs_grad = torch.is_grad_enabled() and (any(p.requires_grad for p in self._all_params()) or skts.requires_grad)
         if needs_grad:
             from . import autograd_path

@@ -486,3 +486,101 @@ def test_refusals():
     for kw in (dict(n_subjects=0), dict(n_subjects=1024), dict(n_subjects=2, rank=0)):
         with pytest.raises(ValueError):
             ad.NetAdapters(net, **kw)
+
+
+@pytest.mark.parametrize("case", ["eval_hier", "train_pytest", "mixamo_train"])
+def test_rays_of_many_subjects_through_the_caster(oracle, case):
+    """RayCaster.render_rays(subject_idxs=...) with adapters on both networks against the oracle's render of every subject with the merged
+    weights W + scale B A, outputs and the adapters' gradients"""
+    from cases import build
+    raycaster = importlib.import_module("a-nerf_amd.raycaster")
+    pipeline = importlib.import_module("a-nerf_amd.pipeline")
+    c = build(case)
+    fc = c["cfg"].get("framecode_ch", 0)
+    t = lambda v: torch.tensor(np.asarray(v), dtype=torch.float32)
+    kw = dict(use_framecode=True, framecode_ch=16, n_framecodes=8) if fc else {}
+    mk = lambda: networks.NeRF(D=8, W=256, input_ch=360, input_ch_bones=72, input_ch_views=648, use_viewdirs=True, **kw)
+    nets = []
+    for P in (c["Pc"], c["Pf"]):
+        n = mk()
+        n.load_state_dict({k: t(v) for k, v in P.items()})
+        nets.append(n)
+    ck = dict(cutoff=True, cutoff_dist=0.5, cutoff_inputs=True, cutoff_dim=24)
+    ev, eb, ed = (networks.get_embedder(7, 0, 24, cutoff_kwargs=dict(ck))[0], networks.get_embedder(0, 0, 72)[0],
+                  networks.get_embedder(4, 0, 72, cutoff_kwargs=dict(ck, dist_inputs=True))[0])
+    caster = raycaster.RayCaster(nets[0], ev, eb, ed, network_fine=nets[1]).cuda().requires_grad_(False)
+    caster.train(bool(c.get("train")))
+    S_, n, S, Ni = 3, c["n"], c["S"], c["Ni"]
+    torch.manual_seed(4)
+    ads = [ad.NetAdapters(net, S_, rank=4, scale=0.5).cuda() for net in nets]
+    with torch.no_grad():
+        for a in ads:
+            for name in ad.LAYERS:
+                a.up(name).normal_(0, 0.05)
+    caster.set_adapters(*ads)
+    subj = torch.arange(n) % 4 - (torch.arange(n) % 4 == 3).long() * 4            # 0, 1, 2 and -1
+    rb = pipeline.make_ray_batch(t(c["rays_o"]).cuda(), t(c["rays_d"]).cuda())
+    cams = t(c["cams"]) if fc else None
+    out = caster(rb, N_samples=S, kp_batch=t(c["kp"]).cuda(), skts=t(c["skts"]).cuda(), cyls=t(c["cyls"]).cuda(), cams=None if cams is None else cams.cuda(),
+                 subject_idxs=subj.cuda(), N_importance=Ni, preproc_kwargs={"density_scale": 1.0})
+    ocfg = oracle.OracleConfig(**c["cfg"])
+    thin = [{k: [a.down(k).detach().cpu().requires_grad_(), a.up(k).detach().cpu().requires_grad_()] for k in ad.LAYERS} for a in ads]
+    want = {k: torch.zeros(out[k].shape) for k in ("rgb_map", "acc_map", "rgb0")}
+    skts = t(c["skts"])
+    for s in (0, 1, 2, -1):
+        r = (subj == s).nonzero()[:, 0]
+        P = []
+        for base, th, a in zip((c["Pc"], c["Pf"]), thin, ads):
+            p = {k: t(v) for k, v in base.items()}
+            if s >= 0:
+                for k in ad.LAYERS:
+                    p[k + ".weight"] = p[k + ".weight"] + a.scale * th[k][1][s] @ th[k][0][s]
+            P.append(p)
+        # the nan-mean of missed rays is a statistic of the call: rays of a subject alone would see another one, so the whole batch is rendered
+        ref = oracle.render_rays(ocfg, P[0], P[1], oracle.make_ray_batch(t(c["rays_o"]), t(c["rays_d"])), skts, t(c["cyls"]), S, Ni,
+                                 **({"cam_idx": cams} if fc else {}))
+        for k in want:
+            want[k] = want[k].index_copy(0, r, ref[k][r])
+    for k in want:
+        np.testing.assert_allclose(out[k].detach().cpu().numpy(), want[k].detach().numpy(), atol=1e-4, err_msg=k)
+    gen = torch.Generator().manual_seed(1)
+    g = torch.randn(n, 3, generator=gen)
+    ((out["rgb_map"] + out["rgb0"]) * g.cuda()).sum().backward() if out["rgb_map"].requires_grad else None
+    if not out["rgb_map"].requires_grad:
+        assert case == "eval_hier"                                                  # eval mode renders without gradients
+        return
+    ((want["rgb_map"] + want["rgb0"]) * g).sum().backward()
+    for a, th in zip(ads, thin):
+        for k in ad.LAYERS:
+            for got, ref in zip((a.down(k).grad, a.up(k).grad), th[k]):
+                # (units within rounding of their ReLU's edge, and samples that importance places elsewhere by a rounding: as in the other gradient tests)
+                assert float((got.cpu() - ref.grad).norm()) < 2e-2 * float(ref.grad.norm()) + 1e-6, k
+
+
+def test_the_caster_refuses_subjects_it_cannot_serve():
+    raycaster = importlib.import_module("a-nerf_amd.raycaster")
+    mk = lambda: networks.NeRF(D=8, W=256, input_ch=360, input_ch_bones=72, input_ch_views=648, use_viewdirs=True)
+    ck = dict(cutoff=True, cutoff_dist=0.5, cutoff_inputs=True, cutoff_dim=24)
+    ev, eb, ed = (networks.get_embedder(7, 0, 24, cutoff_kwargs=dict(ck))[0], networks.get_embedder(0, 0, 72)[0],
+                  networks.get_embedder(4, 0, 72, cutoff_kwargs=dict(ck, dist_inputs=True))[0])
+    caster = raycaster.RayCaster(mk(), ev, eb, ed, network_fine=mk()).cuda()
+    rb = torch.rand(4, 11, device="cuda")
+    args = dict(N_samples=8, kp_batch=torch.zeros(1, 24, 3, device="cuda"), skts=torch.eye(4, device="cuda").expand(1, 24, 4, 4), cyls=torch.ones(4, 5, device="cuda"),
+                N_importance=8)
+    with pytest.raises(NotImplementedError):
+        caster(rb, subject_idxs=torch.zeros(4, dtype=torch.long, device="cuda"), **args)
+    a = ad.NetAdapters(caster.network, 2)
+    with pytest.raises(ValueError):
+        caster.set_adapters(a)
+    caster.set_adapters(a, ad.NetAdapters(caster.network_fine, 2))
+    with pytest.raises(ValueError):
+        caster(rb, subject_idxs=torch.zeros(3, dtype=torch.long, device="cuda"), **args)
+    with pytest.raises(ValueError):
+        caster(rb, subject_idxs=torch.zeros(4, device="cuda"), **args)
+    with pytest.raises(ValueError):                                                  # shared weights that ask for gradients
+        caster.train()(rb, subject_idxs=torch.zeros(4, dtype=torch.long, device="cuda"), **args)
+    with pytest.raises(NotImplementedError):
+        sk = torch.eye(4, device="cuda").repeat(4, 24, 1, 1).requires_grad_()
+        caster.requires_grad_(False)(rb, subject_idxs=torch.zeros(4, dtype=torch.long, device="cuda"), **dict(args, skts=sk))
+    caster.set_adapters(None)
+    assert caster.network.adapters() is None and caster.network_fine.adapters() is None
