@@ -4,6 +4,7 @@ Tolerances are counted, not fitted.  A sum of n products held in fp32 is off by 
 magnitudes (2^-23 a step: half a step would do for additions rounded to nearest, the matrix units are not bound to that), and rounding to
 the rows' type adds half a step of the result, eps / 2.  Where a sum's terms are themselves rounded sums (h = x A^T, u = g B) their own
 bound times the factor's magnitude is added; h enters the 16-bit products as two values and loses 2^-16 of itself there."""
+import gc
 import importlib
 import math
 
@@ -19,6 +20,14 @@ networks = importlib.import_module("a-nerf_amd.networks")
 
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 STEP = 2.0 ** -23
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_back_what_the_allocator_cached():
+    """other tests account for single allocations: blocks of this module's odd sizes would serve them instead of fresh ones"""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 def half(dt):
