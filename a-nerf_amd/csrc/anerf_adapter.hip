@@ -195,7 +195,7 @@ struct MainArgs {
   const float* factor;         // fp16: power of two of every row of h
   void* y;
   float* part;                 // splits > 1: fp32 [splits][M][N]
-  long long ldx, K, N;
+  long long ldx, ldw, K, N;
   long long M;
   int L, R, Rp, splits;
 };
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   for (int l = 0; l < WL; ++l) {
     long long n = n0 + 8 * (wave + NW * l) + sub;
     if (n >= P.N) n = P.N - 1;
-    wo[l] = (Off)((n * P.K + ch * EPC) * (long long)sizeof(E));
+    wo[l] = (Off)((n * P.ldw + ch * EPC) * (long long)sizeof(E));
   }
   u32x4 rx[XL], rw[WL];
   auto at = [&](int buf, int row8) { return buf * STAGE + row8 * 64; };      // eight rows of 128 bytes
@@ -912,7 +912,8 @@ __global__ void __launch_bounds__(256) k_thin_grad_sum(GradJobs G) {
 struct TransposeJob {
   const void* in;
   void* out;
-  long long rows, cols, batch, tiles, tiles_c;   // in [batch][rows][cols] -> out [batch][cols][rows]
+  long long rows, cols, batch, tiles, tiles_c;   // in [batch][rows][cols] -> out [batch][cols][ldo], zeros behind the rows
+  long long ldo;
 };
 struct TransposeJobs {
   TransposeJob j[3];
@@ -929,7 +930,7 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   while (k < 2 && b >= J.j[k].tiles * J.j[k].batch) b -= J.j[k].tiles * J.j[k].batch, ++k;
   const TransposeJob& T = J.j[k];
   const U* in = static_cast<const U*>(T.in) + b / T.tiles * T.rows * T.cols;
-  U* out = static_cast<U*>(T.out) + b / T.tiles * T.rows * T.cols;
+  U* out = static_cast<U*>(T.out) + b / T.tiles * T.ldo * T.cols;
   const long long r0 = b % T.tiles / T.tiles_c * 64, c0 = b % T.tiles % T.tiles_c * 64;
   constexpr int LANES = 64 / V;      // lanes of a row
   const int x = threadIdx.x % LANES * V;
@@ -949,7 +950,7 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   __syncthreads();
   for (int c = threadIdx.x / LANES; c < 64; c += 256 / LANES) {
     if (c0 + c >= T.cols) break;
-    U* dst = out + (c0 + c) * T.rows + r0 + x;
+    U* dst = out + (c0 + c) * T.ldo + r0 + x;
     if (r0 + x + V <= T.rows) {
       vec v;
 #pragma unroll
@@ -957,8 +958,29 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
       __builtin_memcpy(dst, &v, 16);
     } else {
       for (int e = 0; e < V; ++e)
-        if (r0 + x + e < T.rows) dst[e] = t[x + e][c];
+        if (r0 + x + e < T.ldo) dst[e] = r0 + x + e < T.rows ? t[x + e][c] : (U)0;
     }
+  }
+}
+
+// rows with zeros behind them up to a multiple of 128 bytes, 16-byte aligned: what k_main's direct loads want
+struct PadJob {
+  const void* in;
+  void* out;
+  long long rows, ld;
+};
+template <int DT>
+__global__ void __launch_bounds__(256) k_pad(PadJob a, PadJob b, long long K, long long Kp) {
+  typedef typename Elem<DT>::T E;
+  constexpr int EPC = Elem<DT>::EPC;
+  const unsigned line = (unsigned)(Kp / EPC);
+  const long long first = a.rows * line, all = first + b.rows * line;
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < all; t += (long long)gridDim.x * 256) {
+    const bool two = t >= first;
+    const long long u = two ? t - first : t;
+    const long long r = u / line, k = (u - r * line) * EPC;
+    const E* src = static_cast<const E*>(two ? b.in : a.in) + r * (two ? b.ld : a.ld);
+    *reinterpret_cast<u32x4*>(static_cast<E*>(two ? b.out : a.out) + r * Kp + k) = load_tail<DT>(src, k, K);
   }
 }
 
@@ -996,7 +1018,7 @@ template <int DT>
 static int launch_main(const MainArgs& P, hipStream_t st) {
   constexpr long long es = sizeof(typename Elem<DT>::T), span = 1ll << 32;      // DIRECT's offsets have 32 bits
   const bool direct = (((uintptr_t)P.x | (uintptr_t)P.w) & 15) == 0 && P.K % Elem<DT>::EPC == 0 && P.ldx % Elem<DT>::EPC == 0 &&
-                      P.M * P.ldx * es < span && P.N * P.K * es < span;
+                      P.ldw % Elem<DT>::EPC == 0 && P.M * P.ldx * es < span && P.N * P.ldw * es < span;
   auto cost = [&](int bm, int bn, double rate, bool few_waves) {
     const long long tiles = (P.M + bm - 1) / bm * ((P.N + bn - 1) / bn), mine = (tiles + 255) / 256;
     return (double)mine * bm * bn / (few_waves && mine == 1 ? 0.7 * rate : rate);      // (one wave a SIMD does not hide its own waits)
@@ -1034,13 +1056,25 @@ static HLayout h_layout(const AnerfAdapterIO& A) {
   return H;
 }
 long long adapter_h_bytes(const AnerfAdapterIO& A) { return h_layout(A).bytes; }
+// Rows that cannot be loaded 16 bytes aligned go through registers and smaller tiles (8192 x 4097 x 4096 bf16: 473 us, 4096: 302).  With
+// enough outputs a row and rows an output a copy with padded rows costs less (one pass over x and W; from about 1200 of each).
+// The width of the copies, 0: none.  ldw > n_in: W's rows lie padded already.
+static long long padded_width(const AnerfAdapterIO& A, long long ldw) {
+  const long long es = A.dtype == ANERF_F32 ? 4 : 2, epc = 16 / es, Kp = (A.n_in + 8 * epc - 1) / (8 * epc) * (8 * epc);
+  const bool odd = A.n_in % epc || A.x_stride % epc || (((uintptr_t)A.x | (uintptr_t)A.weight) & 15);
+  if (!odd || A.n_rows < 1280 || A.n_out < 1280 || A.n_in < 256) return 0;
+  if (A.n_rows * Kp * es >= (1ll << 32) || A.n_out * Kp * es >= (1ll << 32)) return 0;
+  return ldw > A.n_in && ldw != Kp ? 0 : Kp;
+}
+
 long long adapter_workspace(const AnerfAdapterIO& A) {
   const int splits = split_of(A.dtype, A.n_rows, A.n_in, A.n_out);
-  return splits > 1 ? splits * A.n_rows * A.n_out * 4 : 0;
+  if (splits > 1) return splits * A.n_rows * A.n_out * 4;
+  return padded_width(A, A.n_in) * (A.n_rows + A.n_out) * (A.dtype == ANERF_F32 ? 4 : 2);
 }
 
 template <int DT>
-static int linear_t(const AnerfAdapterIO& A, void* ws, hipStream_t st) {
+static int linear_t(const AnerfAdapterIO& A, long long ldw, void* ws, hipStream_t st) {
   typedef typename Elem<DT>::T E;
   const HLayout H = h_layout(A);
   const long long pieces = pieces_bound(A.n_rows, A.n_adapters, TH_ROWS);
@@ -1062,16 +1096,27 @@ static int linear_t(const AnerfAdapterIO& A, void* ws, hipStream_t st) {
   if (rc || !A.y) return rc;       // (the gradient of A alone needs h only)
   const void* operand = split;
   if constexpr (DT == ANERF_F32) operand = h;
-  const MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, A.y, static_cast<float*>(ws),
-                      A.x_stride, A.n_in, A.n_out, A.n_rows, A.n_adapters, A.rank, Rp, split_of(DT, A.n_rows, A.n_in, A.n_out)};
+  MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, A.y, static_cast<float*>(ws), A.x_stride, ldw, A.n_in, A.n_out,
+                A.n_rows, A.n_adapters, A.rank, Rp, split_of(DT, A.n_rows, A.n_in, A.n_out)};
+  if (const long long Kp = padded_width(A, ldw)) {
+    char* w = static_cast<char*>(ws);
+    const bool w_lies = ldw == Kp && ((uintptr_t)A.weight & 15) == 0;
+    PadJob jx = {A.x, w, A.n_rows, A.x_stride}, jw = {A.weight, w + A.n_rows * Kp * (long long)sizeof(E), w_lies ? 0 : A.n_out, ldw};
+    k_pad<DT><<<2048, 256, 0, st>>>(jx, jw, A.n_in, Kp);
+    const int rc = check_launch("k_pad");
+    if (rc) return rc;
+    P.x = jx.out, P.ldx = Kp;
+    if (!w_lies) P.w = jw.out;
+    P.ldw = P.K = Kp;
+  }
   return launch_main<DT>(P, st);
 }
 
 int launch_adapter_linear(const AnerfAdapterIO& A, void* ws, hipStream_t st) {
   switch (A.dtype) {
-    case ANERF_F32: return linear_t<ANERF_F32>(A, ws, st);
-    case ANERF_BF16: return linear_t<ANERF_BF16>(A, ws, st);
-    default: return linear_t<ANERF_F16>(A, ws, st);
+    case ANERF_F32: return linear_t<ANERF_F32>(A, A.n_in, ws, st);
+    case ANERF_BF16: return linear_t<ANERF_BF16>(A, A.n_in, ws, st);
+    default: return linear_t<ANERF_F16>(A, A.n_in, ws, st);
   }
 }
 
@@ -1124,10 +1169,11 @@ static long long part_floats(long long M, int L, long long C, int Rp) {
 static AnerfAdapterIO swapped(const AnerfAdapterIO& A) {      // sizes of the product that dx is
   AnerfAdapterIO T = A;
   T.n_in = A.n_out, T.n_out = A.n_in;
+  T.x = nullptr, T.weight = nullptr, T.x_stride = 1;      // (not known yet: the worst case where sizes are asked for)
   return T;
 }
 struct BackwardPlan {
-  long long wt, dt, ut, u, part, bytes;     // byte offsets in the workspace; the parts of dx's product and those of dA, dB share `part`
+  long long wt_ld, wt, dt, ut, u, part, bytes;     // row length of W^T; byte offsets in the workspace; the parts of dx's product and those of dA, dB share `part`
 };
 static BackwardPlan backward_plan(const AnerfAdapterIO& A) {
   const long long es = A.dtype == ANERF_F32 ? 4 : 2;
@@ -1135,7 +1181,9 @@ static BackwardPlan backward_plan(const AnerfAdapterIO& A) {
   auto up16 = [](long long b) { return (b + 255) / 256 * 256; };
   BackwardPlan B;
   long long at = 0;
-  B.wt = at, at += up16(A.n_in * A.n_out * es);
+  B.wt_ld = padded_width(swapped(A), A.n_out);
+  if (!B.wt_ld) B.wt_ld = A.n_out;
+  B.wt = at, at += up16(A.n_in * B.wt_ld * es);
   B.dt = at, at += up16((long long)A.n_adapters * A.rank * A.n_in * es);
   B.ut = at, at += up16((long long)A.n_adapters * A.rank * A.n_out * es);
   B.u = at, at += up16(h_layout(A).bytes);
@@ -1188,24 +1236,24 @@ static int backward_t(const AnerfAdapterIO& A, const AnerfAdapterGradIO& G, char
   float* part = reinterpret_cast<float*>(ws + B.part);
   if (A.n_rows > 0 && (G.dx || G.ddown)) {
     // dx = the forward product of (g, W^T, B^T, A^T); its low-rank middle u is what dA needs
-    auto job = [](const void* in, void* out, long long rows, long long cols, long long batch) {
-      TransposeJob t = {in, out, rows, cols, batch, (rows + 63) / 64 * ((cols + 63) / 64), (cols + 63) / 64};
+    auto job = [](const void* in, void* out, long long rows, long long cols, long long batch, long long ldo) {
+      TransposeJob t = {in, out, rows, cols, batch, (rows + 63) / 64 * ((cols + 63) / 64), (cols + 63) / 64, ldo};
       return t;
     };
+    AnerfAdapterIO T = swapped(A);
+    T.x = G.g, T.x_stride = G.g_stride, T.weight = ws + B.wt, T.bias = nullptr, T.down = ws + B.ut, T.up = ws + B.dt, T.y = G.dx, T.h = ws + B.u;
+    const long long Kp = padded_width(T, A.n_out), ldw = Kp ? Kp : A.n_out;
     TransposeJobs J;
-    J.j[0] = job(A.weight, ws + B.wt, A.n_out, A.n_in, 1);
-    J.j[1] = job(A.down, ws + B.dt, A.rank, A.n_in, A.n_adapters);
-    J.j[2] = job(A.up, ws + B.ut, A.n_out, A.rank, A.n_adapters);
+    J.j[0] = job(A.weight, ws + B.wt, A.n_out, A.n_in, G.dx ? 1 : 0, ldw);
+    J.j[1] = job(A.down, ws + B.dt, A.rank, A.n_in, G.dx ? A.n_adapters : 0, A.rank);
+    J.j[2] = job(A.up, ws + B.ut, A.n_out, A.rank, A.n_adapters, A.n_out);
     long long blocks = 0;
     for (int k = 0; k < 3; ++k) blocks += J.j[k].tiles * J.j[k].batch;
     if constexpr (DT == ANERF_F32) k_transpose<uint32_t><<<(unsigned)blocks, 256, 0, st>>>(J);
     else k_transpose<uint16_t><<<(unsigned)blocks, 256, 0, st>>>(J);
     int rc = check_launch("k_transpose");
     if (rc) return rc;
-    AnerfAdapterIO T = swapped(A);
-    T.x = G.g, T.x_stride = G.g_stride, T.weight = ws + B.wt, T.bias = nullptr, T.down = ws + B.ut, T.up = ws + B.dt;
-    T.y = G.dx, T.h = ws + B.u;
-    rc = linear_t<DT>(T, ws + B.part, st);
+    rc = linear_t<DT>(T, ldw, ws + B.part, st);
     if (rc) return rc;
   }
   return thin_grads<DT>(A, G, u, part, st);

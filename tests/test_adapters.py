@@ -198,7 +198,7 @@ def oracle_linear(d, scale, dtype):
 
 SHAPES = [(1, 1, 1, 1, 1), (1, 4096, 512, 4, 16), (3, 7, 5, 2, 3), (17, 64, 33, 17, 8), (48, 512, 640, 64, 16), (64, 100, 64, 3, 1), (65, 131, 66, 5, 12),
           (130, 256, 130, 2, 33), (257, 688, 256, 16, 8), (300, 432, 256, 300, 4), (1000, 129, 1, 7, 5), (515, 40, 3, 2, 64), (90, 904, 128, 4, 130),
-          (2051, 96, 257, 24, 24)]
+          (2051, 96, 257, 24, 24), (1300, 261, 1290, 3, 7), (1281, 1290, 1300, 2, 20)]
 
 
 @pytest.mark.parametrize("M,K,N,L,R", SHAPES)
