@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
 #pragma unroll
         for (int n = 0; n < NJ; ++n)
 #pragma unroll
-          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(av[d][n], xv[d][m], acc[m][n], e);
+          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(av[d][n], xv[d][m], acc[m][n], e);
   };
   long long s = wave;
   for (; s + (TH_DEPTH - 1) * TH_WAVES < steps; s += TH_DEPTH * TH_WAVES) walk(s, Const<TH_DEPTH>());
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
 #pragma unroll
       for (int n = 0; n < NJ; ++n)
 #pragma unroll
-        for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(av[n], xv[m], acc[m][n], e);
+        for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(av[n], xv[m], acc[m][n], e);
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 }
 
 // ------------------------------------------------------------------------------------------------------------------ y = x W^T ...
-// BM positions x BN outputs a workgroup of WM x WN waves, BS x BS MFMA blocks with W's rows as the first operand, so that a lane ends
-// with groups of four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, double-buffered; 16-byte
+// BM positions x BN outputs a workgroup of WM x WN waves, 16 x 16 MFMA blocks with W's rows as the first operand, so that a lane ends
+// with four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, double-buffered; 16-byte
 // chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.  DIRECT: global_load_lds_dwordx4, eight rows
 // an instruction, the lanes fetching the chunks in the order they have to lie in LDS (16-byte aligned rows); otherwise through registers,
 // at any alignment.
@@ -202,14 +202,12 @@ struct MainArgs {
 
 constexpr int FOLD = 16;
 
-template <int DT, int BS, int BM, int BN, int WM, int WN, bool DIRECT>
+template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
 __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) k_main(MainArgs P) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, KB = 8 * EPC;        // elements of a 128-byte row piece
   constexpr int NW = WM * WN;
-  constexpr int TM = BM / WM, TN = BN / WN, MI = TM / BS, NI = TN / BS;
-  constexpr int NV = BS * BS / 64, QB = 64 / BS;          // accumulators of a lane and block, lane groups of a step
-  typedef typename Block<BS>::Acc Acc;
+  constexpr int BS = 16, TM = BM / WM, TN = BN / WN, MI = TM / BS, NI = TN / BS;
   constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;       // 16-byte loads of a lane and stage
   constexpr int STAGE = (BM + BN) * 8;                    // 16-byte units
   extern __shared__ u32x4 lds[];                          // [2][STAGE]
@@ -299,11 +297,11 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     }
   };
   start(first, 0);
-  Acc acc[MI][NI];
+  f32x4 acc[MI][NI];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
 #pragma unroll
-    for (int n = 0; n < NI; ++n) acc[m][n] = Acc{};
+    for (int n = 0; n < NI; ++n) acc[m][n] = f32x4{};
 
   // ---- low-rank term
   const int kept = P.offsets[P.L];
@@ -342,16 +340,16 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
               for (int n = 0; n < NI; ++n)
 #pragma unroll
-                for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<BS>(bf[n], hf[m], acc[m][n], e);
+                for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(bf[n], hf[m], acc[m][n], e);
             } else {
               const bool mine = BS * m + i >= r0 && BS * m + i < r1;
 #pragma unroll
               for (int n = 0; n < NI; ++n) {
-                Acc t = Acc{};
+                f32x4 t = f32x4{};
 #pragma unroll
-                for (int e = 0; e < Elem<DT>::INSTR; ++e) t = Elem<DT>::template mma<BS>(bf[n], hf[m], t, e);
+                for (int e = 0; e < Elem<DT>::INSTR; ++e) t = Elem<DT>::mma(bf[n], hf[m], t, e);
 #pragma unroll
-                for (int e = 0; e < NV; ++e) acc[m][n][e] = mine ? acc[m][n][e] + t[e] : acc[m][n][e];
+                for (int e = 0; e < 4; ++e) acc[m][n][e] = mine ? acc[m][n][e] + t[e] : acc[m][n][e];
               }
             }
           }
@@ -372,19 +370,19 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 
   // ---- x W^T
   constexpr bool F32 = DT == ANERF_F32;
-  Acc sum[F32 ? MI : 1][F32 ? NI : 1];
+  f32x4 sum[F32 ? MI : 1][F32 ? NI : 1];
   if constexpr (F32) {
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
-      for (int n = 0; n < NI; ++n) sum[m][n] = Acc{};
+      for (int n = 0; n < NI; ++n) sum[m][n] = f32x4{};
   }
   // A half stage's rows of x are taken in two groups, and every group's fragments are read from LDS while the products of the group
   // before it run (two sets of W's fragments, one of each group of x's), so that the matrix units need not wait for LDS.  The one barrier
   // of a stage lies before its last group's products: there every wave has read the last of stage s, whose buffer stage s + 2 may then
   // overwrite, and every wave's loads of stage s + 1 have arrived.
   constexpr int MG = MI / 2;
-  static_assert(8 / QB == 2 && MI % 2 == 0, "two halves a stage, two groups a half");
+  static_assert(MI % 2 == 0, "two groups of row blocks a half stage");
   u32x4 wf[2][NI], xf[2][MG];
   // fragment addresses: row i of a block has r & 7 = i & 7, the halves' chunks differ in bit 2
   const int px = (wm * TM + i) * 8, pw = (BM + wn * TN + i) * 8, ch0 = q ^ (i & 7);
@@ -404,7 +402,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
       for (int n = 0; n < NI; ++n)
 #pragma unroll
-        for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[g * MG + m][n] = Elem<DT>::template mma<BS>(wf[h][n], xf[g][m], acc[g * MG + m][n], e);
+        for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[g * MG + m][n] = Elem<DT>::mma(wf[h][n], xf[g][m], acc[g * MG + m][n], e);
   };
   auto arrive = [&]() {
     if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -416,7 +414,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   read_w(0, 0);
   read_x(0, 0, 0);
   auto zero_behind = [&](u32x4* f, int n, int h) {      // fragments of the partial stage: chunks behind the row
-    const bool there = full * KB + (QB * h + q) * EPC < K;
+    const bool there = full * KB + (4 * h + q) * EPC < K;
 #pragma unroll
     for (int e = 0; e < n; ++e) f[e] = there ? f[e] : u32x4{0, 0, 0, 0};
   };
@@ -453,14 +451,14 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
           for (int n = 0; n < NI; ++n) {
             sum[m][n] += acc[m][n];
-            acc[m][n] = Acc{};
+            acc[m][n] = f32x4{};
           }
       }
     }
   }
   if (DIRECT && full < stages) stage(full, (full - first) & 1, Const<1>());
 
-  // ---- bias, rounding, store.  A lane holds groups of four outputs of its row.  fp32: 16 bytes each, stored as they are
+  // ---- bias, rounding, store.  A lane holds four outputs of its row in each block.  fp32: 16 bytes, stored as they are
   if constexpr (F32) {
     const float* bias = static_cast<const float*>(P.bias);
 #pragma unroll
@@ -470,24 +468,20 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       const long long row = P.order ? (long long)P.order[p] : p;
       float* yr = P.splits > 1 ? P.part + (part * P.M + row) * P.N : static_cast<float*>(P.y) + row * P.N;
 #pragma unroll
-      for (int n = 0; n < NI; ++n)
+      for (int n = 0; n < NI; ++n) {
+        const long long col = n0 + wn * TN + BS * n + 4 * q;
+        f32x4 v = acc[m][n] + sum[m][n];
 #pragma unroll
-        for (int g = 0; g < NV / 4; ++g) {
-          const long long col = n0 + wn * TN + BS * n + 8 * g + 4 * q;
-          f32x4 v;
+        for (int e = 0; e < 4; ++e)
+          if (bias && P.splits == 1 && col + e < P.N) v[e] += bias[col + e];
+        if (col + 4 <= P.N) {
+          store16(yr + col, __builtin_bit_cast(u32x4, v));
+        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = acc[m][n][4 * g + e] + sum[m][n][4 * g + e];
-            if (bias && P.splits == 1 && col + e < P.N) v[e] += bias[col + e];
-          }
-          if (col + 4 <= P.N) {
-            store16(yr + col, __builtin_bit_cast(u32x4, v));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + e < P.N) yr[col + e] = v[e];
-          }
+          for (int e = 0; e < 4; ++e)
+            if (col + e < P.N) yr[col + e] = v[e];
         }
+      }
     }
     return;
   }
@@ -501,12 +495,12 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     char* mine = reinterpret_cast<char*>(lds) + wave * (ROWS * LINE);
     const long long cw = n0 + wn * TN;
     const int r0 = lane / LPR, c = lane % LPR * PER;
-    float add[NI][NV];
+    float add[NI][4];
 #pragma unroll
     for (int n = 0; n < NI; ++n)
 #pragma unroll
-      for (int e = 0; e < NV; ++e) {
-        const long long col = cw + BS * n + 8 * (e / 4) + 4 * q + e % 4;
+      for (int e = 0; e < 4; ++e) {
+        const long long col = cw + BS * n + 4 * q + e;
         add[n][e] = bias && col < P.N ? (float)bias[col] : 0.f;
       }
 #pragma unroll
@@ -521,17 +515,15 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
       for (int m = 0; m < MG; ++m)
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
+        for (int n = 0; n < NI; ++n) {
+          four o;
 #pragma unroll
-          for (int k = 0; k < NV / 4; ++k) {
-            four o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = acc[g * MG + m][n][4 * k + e];
-              o[e] = (S)(bias ? v + add[n][4 * k + e] : v);
-            }
-            *reinterpret_cast<four*>(mine + (BS * m + i) * LINE + (BS * n + 8 * k + 4 * q) * (int)sizeof(S)) = o;
+          for (int e = 0; e < 4; ++e) {
+            const float v = acc[g * MG + m][n][e];
+            o[e] = (S)(bias ? v + add[n][e] : v);
           }
+          *reinterpret_cast<four*>(mine + (BS * m + i) * LINE + (BS * n + 4 * q) * (int)sizeof(S)) = o;
+        }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the wave's own lines: no barrier
 #pragma unroll
       for (int t = 0; t < ROWS / RPI; ++t) {
@@ -703,7 +695,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::template mma<16>(wv[d][n], xv[d][m], acc[m][n], e);
+          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(wv[d][n], xv[d][m], acc[m][n], e);
   };
   const long long steps = K / STEP;
   long long s = 2 * wave;
@@ -989,7 +981,7 @@ template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
 static int run_main(const MainArgs& P, hipStream_t st) {
   static unsigned long long done = 0;
   constexpr int bytes = 2 * (BM + BN) * 128;
-  const auto kernel = k_main<DT, 16, BM, BN, WM, WN, DIRECT>;
+  const auto kernel = k_main<DT, BM, BN, WM, WN, DIRECT>;
   ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes, &done);
   kernel<<<(unsigned)((P.M + BM - 1) / BM * ((P.N + BN - 1) / BN) * P.splits), WM * WN * 64, bytes, st>>>(P);
   const int rc = check_launch("k_main");

@@ -1320,6 +1320,8 @@ int anerf_combine_rows_backward(const void* dy, const void* z, int32_t dtype, co
   if (rc || n_rows == 0) return rc;
   if (!dz && !dweights) return ANERF_OK;
   if (!slot || !kept || !weights || (width && (!dy || (dweights && !z)))) return set_error(ANERF_E_NULL, "combine_rows_backward: null pointer");
+  // dz alone is the weighted way out, which reads dy's rows once
+  if (!dweights) return width ? launch_rows(0, dtype, dy, nullptr, weights, slot, kept, n_rows, k, width, dz, nullptr, static_cast<hipStream_t>(stream)) : ANERF_OK;
   return launch_rows(2, dtype, dy, z, weights, slot, kept, n_rows, k, width, dz, dweights, static_cast<hipStream_t>(stream));
 }
 
@@ -1331,6 +1333,7 @@ static int adapter_check(const AnerfAdapterIO* a) {
   const int64_t lim = INT64_C(1) << 31, side = INT64_C(1) << 24;      // (tiles, pieces and byte offsets stay inside their integers)
   if (a->n_in < 1 || a->n_out < 1 || a->n_in > side || a->n_out > side) return set_error(ANERF_E_SHAPE, "adapter: n_in / n_out must be 1 .. 2^24");
   if (a->n_rows < 0 || a->n_rows >= lim) return set_error(ANERF_E_SHAPE, "adapter: the number of rows must be 0 .. 2^31 - 1");
+  if (a->x_stride < 0) return set_error(ANERF_E_SHAPE, "adapter: x_stride must not be negative");
   if (((a->n_rows + 63) / 64) * ((a->n_out + 63) / 64) >= lim || ((a->n_rows + 63) / 64) * ((a->n_in + 63) / 64) >= lim)
     return set_error(ANERF_E_SHAPE, "adapter: too many output tiles for one launch");
   return ANERF_OK;
@@ -1376,6 +1379,7 @@ int anerf_adapter_backward(const AnerfAdapterIO* a, const AnerfAdapterGradIO* g,
   const int rc = adapter_check(a);
   if (rc) return rc;
   if (!g) return set_error(ANERF_E_NULL, "adapter_backward: null gradients");
+  if (g->g_stride < 0) return set_error(ANERF_E_SHAPE, "adapter_backward: g_stride must not be negative");
   if (!g->dx && !g->ddown && !g->dup) return ANERF_OK;
   if (a->n_rows == 0 && !g->ddown && !g->dup) return ANERF_OK;
   if (!a->weight || !a->down || !a->up || !a->offsets || (a->n_rows && (!g->g || !a->h || (g->ddown && !a->x))))

@@ -16,43 +16,30 @@ constexpr int ROWS_MAX_GROUPS = 1024;   // every wave's group counters live in L
 constexpr int ANERF_MAX_RANK = 1024;
 constexpr int ROWS_MAX_CHOICES = 64;    // a token's slots sit in the lanes of one wave
 
-// element types of the C ABI: storage type, elements in 16 bytes, and the MFMA products of 16-byte operands.  In a BS x BS block
-// (BS = 16 or 32) lane (i = lane % BS, q = lane / BS) holds 16 bytes of row i of each operand, so that a step contracts 64 / BS x 16 bytes of
-// a row.  fp32: INSTR = 4 instructions a step, instruction e contracting element e of the lane groups -- the indices are contracted
-// in another order than memory's, the same one for both operands.  The result: lane (i, q) holds column i, rows
-// BS == 16 ? 4q + r : 8 * (r / 4) + 4q + r % 4 in register r.
-template <int BS> struct Block {
-  typedef float Acc __attribute__((ext_vector_type(BS * BS / 64)));
-};
+// element types of the C ABI: storage type, elements in 16 bytes, and the MFMA products of 16-byte operands.  In a 16 x 16 block lane
+// (i = lane % 16, q = lane / 16) holds 16 bytes of row i of each operand, so that a step contracts 64 bytes of a row.  fp32: INSTR = 4
+// instructions a step, instruction e contracting element e of the lane groups -- the indices are contracted in another order than
+// memory's, the same one for both operands.  The result: lane (i, q) holds column i, rows 4q .. 4q+3.
 template <int DT> struct Elem;
 template <> struct Elem<ANERF_F32> {
   typedef float T;
   static constexpr int EPC = 4, INSTR = 4;
-  template <int BS>
-  static __device__ __forceinline__ typename Block<BS>::Acc mma(u32x4 a, u32x4 b, typename Block<BS>::Acc c, int e) {
-    const float fa = __builtin_bit_cast(f32x4, a)[e], fb = __builtin_bit_cast(f32x4, b)[e];
-    if constexpr (BS == 16) return __builtin_amdgcn_mfma_f32_16x16x4f32(fa, fb, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x2f32(fa, fb, c, 0, 0, 0);
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, int e) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a)[e], __builtin_bit_cast(f32x4, b)[e], c, 0, 0, 0);
   }
 };
 template <> struct Elem<ANERF_BF16> {
   typedef __bf16 T;
   static constexpr int EPC = 8, INSTR = 1;
-  template <int BS>
-  static __device__ __forceinline__ typename Block<BS>::Acc mma(u32x4 a, u32x4 b, typename Block<BS>::Acc c, int) {
-    const bf16x8 va = __builtin_bit_cast(bf16x8, a), vb = __builtin_bit_cast(bf16x8, b);
-    if constexpr (BS == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, vb, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, vb, c, 0, 0, 0);
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, int) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 template <> struct Elem<ANERF_F16> {
   typedef _Float16 T;
   static constexpr int EPC = 8, INSTR = 1;
-  template <int BS>
-  static __device__ __forceinline__ typename Block<BS>::Acc mma(u32x4 a, u32x4 b, typename Block<BS>::Acc c, int) {
-    const f16x8 va = __builtin_bit_cast(f16x8, a), vb = __builtin_bit_cast(f16x8, b);
-    if constexpr (BS == 16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(va, vb, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(va, vb, c, 0, 0, 0);
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, int) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 
