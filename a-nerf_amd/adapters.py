@@ -42,12 +42,15 @@ _graphs = WeakIdKeyDictionary()     # leaf -> its living graphs
 
 
 def _graph_of(*tensors):
-    leaves = [t for t in tensors if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     if not leaves:
         return None
     graph = _Graph(leaves)
     for t in leaves:
-        _graphs.setdefault(t, weakref.WeakSet()).add(graph)
+        alive = _graphs.get(t)
+        if alive is None:
+            alive = _graphs[t] = weakref.WeakSet()
+        alive.add(graph)
     return graph
 
 
@@ -64,6 +67,15 @@ def _check_capture(graph):
                                "is still referenced): drop it before the capture")
 
 
+def _once(backward):
+    """once_differentiable, at its price (10 us of a small step) only where a graph of the backward is asked for"""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class _DispatchFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan, graph):
@@ -71,7 +83,7 @@ class _DispatchFn(torch.autograd.Function):
         return ops.dispatch_rows(x, plan)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         _check_capture(ctx.graph)
         return ops.combine_rows(g, ctx.plan), None, None
@@ -85,7 +97,7 @@ class _CombineFn(torch.autograd.Function):
         return ops.combine_rows(z, plan, weights)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         _check_capture(ctx.graph)
         z, weights = ctx.saved_tensors
@@ -112,8 +124,8 @@ def combine_rows(z, plan, weights=None):
     return _CombineFn.apply(z, weights, plan, _graph_of(z, weights))
 
 
-def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in tensors)
+def _needs_grad(t, w=None):
+    return torch.is_grad_enabled() and (torch.is_tensor(t) and t.requires_grad or torch.is_tensor(w) and w.requires_grad)
 
 
 def _check_plan(plan, name):
@@ -124,21 +136,26 @@ def _check_plan(plan, name):
 class _AdapterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, down, up, weight, bias, rows, scale, scale_of, graph):
-        y, h = ops.adapter_linear(x, weight, down, up, rows, bias, scale, scale_of)
+        y, h = ops._adapter_linear(x, weight, down, up, rows, bias, scale, scale_of)
         ctx.save_for_backward(x, down, up, weight, scale_of, h)
         ctx.rows, ctx.scale, ctx.graph = rows, scale, graph
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         _check_capture(ctx.graph)
         x, down, up, weight, scale_of, h = ctx.saved_tensors
         if g.stride(-1) != 1 or g.stride(0) < g.shape[1]:
             g = g.contiguous()
         want = ctx.needs_input_grad
-        dx, ddown, dup = ops.adapter_backward(g, x, weight, down, up, ctx.rows, h, ctx.scale, scale_of, want[0], want[1], want[2])
+        dx, ddown, dup = ops._adapter_backward(g, x, weight, down, up, ctx.rows, h, ctx.scale, scale_of, want[0], want[1], want[2])
         return dx, ddown, dup, None, None, None, None, None, None
+
+
+def _refuse(t, name, dim, x):
+    ops._rows_like(t, f"adapter_linear: {name}", None if t is x else x.device, None if t is x else x.dtype)
+    raise ValueError(f"adapter_linear: {name} must have {dim} dimensions, got {tuple(t.shape)}")
 
 
 def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
@@ -149,21 +166,20 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
     projection alone), the RowPlan of such indices (k = 1; worth keeping where several layers see the same rows), or plan.sorted()
     for dispatched rows.  scale: a number, or a float32 tensor [L].
     Gradients: x, A and B; weight and bias are frozen."""
-    x = ops._rows_like(x, "adapter_linear: x")
-    dev, dt = x.device, x.dtype
-    for t, name, dim in ((weight, "weight", 2), (down, "down", 3), (up, "up", 3)) + (() if bias is None else ((bias, "bias", 1),)):
-        ops._rows_like(t, f"adapter_linear: {name}", dev, dt)
-        if t.dim() != dim:
-            raise ValueError(f"adapter_linear: {name} must have {dim} dimensions, got {tuple(t.shape)}")
-    N, K = weight.shape
-    L, R = down.shape[:2]
-    if x.dim() < 1 or x.shape[-1] != K or down.shape[2] != K or tuple(up.shape) != (L, N, R) or (bias is not None and bias.shape[0] != N):
+    for t, name, dim in ((x, "x", None), (weight, "weight", 2), (down, "down", 3), (up, "up", 3), (bias, "bias", 1)):
+        if t is None and name == "bias":
+            continue
+        if not (torch.is_tensor(t) and t.is_cuda and t.dtype in ops.ROW_DTYPES and t.dtype is x.dtype and t.device == x.device and (dim is None or t.dim() == dim)):
+            _refuse(t, name, dim, x)
+    dev, (N, K), (L, R, down_in), grads = x.device, weight.shape, down.shape, torch.is_grad_enabled()
+    if x.dim() < 1 or x.shape[-1] != K or down_in != K or up.shape != (L, N, R) or (bias is not None and bias.shape[0] != N):
         raise ValueError(f"adapter_linear: x {tuple(x.shape)}, weight {tuple(weight.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)}" +
                          ("" if bias is None else f", bias {tuple(bias.shape)}") + " do not fit together")
     if N < 1 or K < 1 or L < 1 or R < 1 or L > ops._lib.MAX_GROUPS or R > ops._lib.MAX_RANK:
         raise ValueError(f"adapter_linear: 1 .. {ops._lib.MAX_GROUPS} adapters of rank 1 .. {ops._lib.MAX_RANK} and no empty side, got {tuple(down.shape)}")
-    if torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if grads and (weight.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("adapter_linear: weight and bias are frozen beside adapters (requires_grad_(False) them, or detach)")
+    grads = grads and (x.requires_grad or down.requires_grad or up.requires_grad)
     scale_of = None
     if torch.is_tensor(scale):
         if scale.dtype != torch.float32 or scale.device != dev or tuple(scale.shape) != (L,):
@@ -181,7 +197,7 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
             raise ValueError(f"adapter_linear: indices on {rows.device}, rows on {dev}")
         if rows.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"adapter_linear: adapter indices must be int32 / int64, got {rows.dtype}")
-        few = M <= ops._lib.FEW_ROWS and not _needs_grad(x, down, up)      # a decoding step: no plan, W streams through once
+        few = M <= ops._lib.FEW_ROWS and not grads      # a decoding step: no plan, W streams through once
         rows = rows.reshape(-1).contiguous() if few else route_rows(rows.reshape(-1), L)
     elif not isinstance(rows, (RowPlan, SortedRows)):
         raise TypeError(f"adapter_linear: rows must be indices, a RowPlan or its sorted(), got {type(rows).__name__}")
@@ -190,13 +206,13 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
     weight, down_, up_, bias = weight.contiguous(), down.contiguous(), up.contiguous(), None if bias is None else bias.contiguous()
     scale = float(scale)
     if torch.is_tensor(rows):
-        return ops.adapter_linear_few(flat, weight, down_, up_, rows, bias, scale, scale_of).reshape(lead + (N,))
+        return ops._adapter_linear_few(flat, weight, down_, up_, rows, bias, scale, scale_of).reshape(lead + (N,))
     if rows.n_rows != M or rows.device != dev or rows.k != 1:
         raise ValueError(f"adapter_linear: a plan of {rows.n_rows} rows with {rows.k} group(s) each on {rows.device} for {M} rows on {dev}")
     if rows.n_groups < L:
         raise ValueError(f"adapter_linear: a plan of {rows.n_groups} groups for {L} adapters")
-    if not _needs_grad(x, down, up):
-        return ops.adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of)[0].reshape(lead + (N,))
+    if not grads:
+        return ops._adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of)[0].reshape(lead + (N,))
     return _AdapterFn.apply(flat, down_, up_, weight, bias, rows, scale, scale_of, _graph_of(x, down, up)).reshape(lead + (N,))
 
 
@@ -257,7 +273,7 @@ class NetAdapters(nn.Module):
         pos, u = xs[:, :dnet], [xs[:, dnet:dnet + view]]
         if net.use_framecode:
             table, cam = net.framecodes.table_for(xs[:, -1], net.training)
-            u.append(table[cam.long()])
+            u.append(table[cam.long().clamp(0, table.shape[0] - 1)])      # (as the fused kernels take indices)
         h = pos
         for i in range(net.D):
             h = torch.relu(lin(f"pts_linears.{i}", h))

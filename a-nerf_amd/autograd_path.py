@@ -305,6 +305,8 @@ def encode_rows(net, kw, z):
     cfg, rays, dev = kw["cfg"], kw["ray_batch"], kw["ray_batch"].device
     skts = ops._f32c(ops.first_row(kw["skts"]), "skts")
     n, s = z.shape
+    if skts.shape[0] not in (1, n) or tuple(skts.shape[1:]) != (cfg.n_joints, 4, 4):
+        raise ValueError(f"skts {tuple(skts.shape)} for {n} rays: expected [1 or {n}, {cfg.n_joints}, 4, 4]")
     codes = None if not net.use_framecode else net.framecodes.codes.weight.detach()
     cam = None if codes is None else kw["cam_idx"].reshape(-1).expand(n).contiguous()
     out = torch.empty(n * s, cfg.x_width, dtype=torch.float32, device=dev)

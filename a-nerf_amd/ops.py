@@ -979,6 +979,9 @@ class RowPlan:
         """the plan of the DISPATCHED rows: n_rows * k of them, lying in group order already"""
         return SortedRows(self)
 
+    def __reduce__(self):      # a copy has addresses of its own buffer
+        return RowPlan, (self.buf, self.n_rows, self.k, self.n_groups, self.shape)
+
 
 class SortedRows:
     """rows that lie in group order: group g owns rows offsets[g] .. offsets[g+1]-1, the rows behind offsets[n_groups] have none"""
@@ -986,6 +989,9 @@ class SortedRows:
     def __init__(self, plan):
         self.plan, self.n_rows, self.k, self.n_groups, self.device = plan, plan.pairs, 1, plan.n_groups, plan.device
         self.offsets_ptr, self.order_ptr = plan.offsets_ptr, None
+
+    def __reduce__(self):
+        return SortedRows, (self.plan,)
 
     @property
     def offsets(self):
@@ -1058,8 +1064,13 @@ def combine_rows(z, plan, weights=None):
 def combine_rows_backward(dy, z, plan, weights, want_dz=True, want_dw=True):
     """gradients of combine_rows with weights -> (dz [T * k, ...] or None, dweights like weights or None)"""
     dy, width = _rows_2d(dy, plan.n_rows, "combine_rows_backward", plan.device)
-    z = z.contiguous() if want_dw else None
     w = _row_weights(weights, plan)
+    if want_dw:
+        z, zw = _rows_2d(z, plan.pairs, "combine_rows_backward", plan.device)
+        if zw != width or z.dtype != dy.dtype:
+            raise ValueError(f"combine_rows_backward: z {tuple(z.shape)} {z.dtype} for dy {tuple(dy.shape)} {dy.dtype}")
+    else:
+        z = None
     dz = torch.empty((plan.pairs,) + dy.shape[1:], dtype=dy.dtype, device=dy.device) if want_dz else None
     dw = torch.empty(weights.shape, dtype=torch.float32, device=dy.device) if want_dw else None
     _launch(dy.device, _lib.load().anerf_combine_rows_backward, "anerf_combine_rows_backward", dy.data_ptr(), _ptr(z), ROW_DTYPES[dy.dtype], _ptr(w),
@@ -1073,10 +1084,61 @@ def _adapter_io(x, weight, down, up, rows, bias, scale, scale_of):
                                x.data_ptr(), weight.data_ptr(), _ptr(bias), down.data_ptr(), up.data_ptr(), _ptr(scale_of),
                                None if rows is None else rows.offsets_ptr, None if rows is None else rows.order_ptr, None, None)
 
+def _adapter_args(name, x, weight, down, up, bias, scale_of):
+    """2-D rows (any row stride), everything else contiguous and of the rows' type"""
+    _rows_like(x, f"{name}: x")
+    for t, what, dim in ((x, "x", 2), (weight, "weight", 2), (down, "down", 3), (up, "up", 3), (bias, "bias", 1)):
+        if t is None and what == "bias":
+            continue
+        _rows_like(t, f"{name}: {what}", x.device, x.dtype)
+        if t.dim() != dim or not (t.is_contiguous() if t is not x else t.stride(1) == 1 or t.shape[1] == 1):
+            raise ValueError(f"{name}: {what} must be {dim}-dimensional and contiguous{' along its rows' if t is x else ''}, got {tuple(t.shape)} {t.stride()}")
+    (N, K), (L, R, _) = weight.shape, down.shape
+    if x.shape[1] != K or down.shape[2] != K or up.shape != (L, N, R) or (bias is not None and bias.shape[0] != N):
+        raise ValueError(f"{name}: x {tuple(x.shape)}, weight {tuple(weight.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)}" +
+                         ("" if bias is None else f", bias {tuple(bias.shape)}") + " do not fit together")
+    if scale_of is not None and (scale_of.dtype != torch.float32 or scale_of.device != x.device or scale_of.shape != (L,) or not scale_of.is_contiguous()):
+        raise ValueError(f"{name}: scale_of must be a contiguous float32 tensor [{L}] on {x.device}")
+
+
+def _adapter_plan(name, x, rows, L):
+    if not isinstance(rows, (RowPlan, SortedRows)):
+        raise TypeError(f"{name}: rows must be a RowPlan or its sorted(), got {type(rows).__name__}")
+    if rows.n_rows != x.shape[0] or rows.k != 1 or rows.device != x.device or rows.n_groups < L:
+        raise ValueError(f"{name}: a plan of {rows.n_rows} rows, {rows.k} group(s) each of {rows.n_groups}, on {rows.device} for {x.shape[0]} rows and {L} adapters "
+                         f"on {x.device}")
+
 
 def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=None):
     """x [M, K] W^T + bias + s_i (x A_i^T) B_i^T (anerf_adapter_linear) -> (y [M, N], h): h is what the backward needs.  weight [N, K],
     down [L, R, K] (A), up [L, N, R] (B), rows: RowPlan (k = 1) or SortedRows of the M rows over the L adapters."""
+    _adapter_args("adapter_linear", x, weight, down, up, bias, scale_of)
+    _adapter_plan("adapter_linear", x, rows, down.shape[0])
+    return _adapter_linear(x, weight, down, up, rows, bias, scale, scale_of)
+
+
+def adapter_linear_few(x, weight, down, up, groups, bias=None, scale=1.0, scale_of=None):
+    """adapter_linear of up to 64 rows with their adapter indices instead of a plan (anerf_adapter_linear_few) -> y [M, N]"""
+    _adapter_args("adapter_linear_few", x, weight, down, up, bias, scale_of)
+    if not torch.is_tensor(groups) or groups.dtype not in (torch.int32, torch.int64) or groups.device != x.device or groups.shape != x.shape[:1]:
+        raise ValueError(f"adapter_linear_few: groups must be an int32 / int64 tensor [{x.shape[0]}] on {x.device}")
+    return _adapter_linear_few(x, weight, down, up, groups.contiguous(), bias, scale, scale_of)
+
+
+def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, want_dx=True, want_ddown=True, want_dup=True):
+    """gradients of adapter_linear with weight and bias frozen (anerf_adapter_backward) -> (dx, ddown, dup), None where not wanted"""
+    _adapter_args("adapter_backward", x, weight, down, up, None, scale_of)
+    _adapter_plan("adapter_backward", x, rows, down.shape[0])
+    _rows_like(g, "adapter_backward: g", x.device, x.dtype)
+    if g.shape != (x.shape[0], weight.shape[0]) or not (g.stride(1) == 1 or g.shape[1] == 1):
+        raise ValueError(f"adapter_backward: g {tuple(g.shape)} with strides {g.stride()} for y {(x.shape[0], weight.shape[0])}")
+    need = _lib.load().anerf_adapter_h_size(C.byref(_adapter_io(x, weight, down, up, rows, None, scale, scale_of)))
+    if h.device != x.device or not h.is_contiguous() or h.numel() * h.element_size() < need:
+        raise ValueError("adapter_backward: h must be what adapter_linear returned for these rows")
+    return _adapter_backward(g, x, weight, down, up, rows, h, scale, scale_of, want_dx, want_ddown, want_dup)
+
+
+def _adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=None):
     io, lib, dev = _adapter_io(x, weight, down, up, rows, bias, scale, scale_of), _lib.load(), x.device
     ref = C.byref(io)
     y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
@@ -1088,8 +1150,7 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=Non
     return y, h
 
 
-def adapter_linear_few(x, weight, down, up, groups, bias=None, scale=1.0, scale_of=None):
-    """adapter_linear of up to 64 rows with their adapter indices instead of a plan (anerf_adapter_linear_few) -> y [M, N]"""
+def _adapter_linear_few(x, weight, down, up, groups, bias=None, scale=1.0, scale_of=None):
     io, dev = _adapter_io(x, weight, down, up, None, bias, scale, scale_of), x.device
     y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
     h = torch.empty(x.shape[0] * down.shape[1], dtype=torch.float32, device=dev)
@@ -1098,8 +1159,7 @@ def adapter_linear_few(x, weight, down, up, groups, bias=None, scale=1.0, scale_
     return y
 
 
-def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, want_dx=True, want_ddown=True, want_dup=True):
-    """gradients of adapter_linear with weight and bias frozen (anerf_adapter_backward) -> (dx, ddown, dup), None where not wanted"""
+def _adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, want_dx=True, want_ddown=True, want_dup=True):
     io, lib, dev = _adapter_io(x, weight, down, up, rows, None, scale, scale_of), _lib.load(), x.device
     io.h = h.data_ptr()
     dx = torch.empty(x.shape[0], weight.shape[1], dtype=x.dtype, device=dev) if want_dx else None

@@ -593,3 +593,185 @@ def test_the_caster_refuses_subjects_it_cannot_serve():
         caster.requires_grad_(False)(rb, subject_idxs=torch.zeros(4, dtype=torch.long, device="cuda"), **dict(args, skts=sk))
     caster.set_adapters(None)
     assert caster.network.adapters() is None and caster.network_fine.adapters() is None
+
+
+# ------------------------------------------------------------------------------------------- large products, few rows, long offsets
+def on_the_device(M, K, N, L, R, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    mk = lambda *s, f=1.0: (torch.randn(*s, generator=gen, device="cuda") * f).to(dtype)
+    d = dict(x=mk(M, K), weight=mk(N, K, f=K ** -0.5), bias=mk(N), down=mk(L, R, K, f=K ** -0.5), up=mk(L, N, R, f=R ** -0.5), g=mk(M, N))
+    d["idx"] = torch.randint(-1, L, (M,), generator=gen, device="cuda")
+    return d
+
+
+def oracle_rows(d, scale, dtype, rows):
+    """(y, bound) of some rows of a large product, 64 bits on the device"""
+    x, W, A, B, b, i = d["x"][rows].double(), d["weight"].double(), d["down"].double(), d["up"].double(), d["bias"].double(), d["idx"][rows]
+    K, R = x.shape[1], A.shape[1]
+    split = 2.0 ** -16 if dtype != torch.float32 else 0.0
+    y, yb = x @ W.t(), (K + R + 4) * STEP * (x.abs() @ W.abs().t())
+    for a in i.unique().tolist():
+        if a < 0:
+            continue
+        r = (i == a).nonzero()[:, 0]
+        h, hb = x[r] @ A[a].t(), (K + 2) * STEP * (x[r].abs() @ A[a].abs().t())
+        y[r] += scale * h @ B[a].t()
+        yb[r] += abs(scale) * (hb + ((K + R + 4) * STEP + split) * h.abs()) @ B[a].abs().t()
+    return y + b, yb + STEP * (b.abs() + y.abs())
+
+
+# M x N that the tile rule gives 64 x 64, 128 x 64, 128 x 128, 256 x 128 and 256 x 256 outputs a workgroup, with rows and outputs that end
+# inside a tile; K that ends inside a stage, few adapters (blocks inside one) and many (blocks that several share)
+LARGE = [(2051, 1030, 200, 3, 8), (2999, 1502, 136, 200, 16), (4001, 4098, 328, 5, 40), (4095, 4090, 72, 2, 8), (6001, 4098, 200, 300, 4), (8001, 4098, 136, 7, 20),
+         (8191, 8190, 264, 64, 16), (3501, 2042, 136, 30, 8), (2999, 4098, 200, 2, 16)]
+
+
+@pytest.mark.parametrize("M,N,K,L,R", LARGE)
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_large_products(M, N, K, L, R, dt):
+    d = on_the_device(M, K, N, L, R, DT[dt], M + N)
+    rows = torch.cat([torch.arange(0, M, 37), torch.arange(M - 130, M)]).cuda()
+    y, yb = oracle_rows(d, 0.75, DT[dt], rows)
+    args = (d["weight"], d["down"], d["up"])
+    got = ad.adapter_linear(d["x"], *args, d["idx"], bias=d["bias"], scale=0.75)
+    within(got[rows], y, yb, DT[dt])
+    # W is contracted over its rows in the gradient of x: the same tiles the other way round
+    plan = ad.route_rows(d["idx"], L)
+    ys = ad.adapter_linear(d["x"][plan.source.long()], *args, plan.sorted(), bias=d["bias"], scale=0.75)
+    within(ys[plan.slot.long()[rows]], y, yb, DT[dt])
+
+
+@pytest.mark.parametrize("M", [1, 15, 16, 17, 32, 33, 48, 49, 64])
+@pytest.mark.parametrize("N,K,R", [(8195, 520, 12), (300, 1029, 5), (4096, 4096, 16)])
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_few_rows(M, N, K, R, dt):
+    d = on_the_device(M, K, N, 9, R, DT[dt], M + N)
+    y, yb = oracle_rows(d, 0.5, DT[dt], torch.arange(M, device="cuda"))
+    within(ad.adapter_linear(d["x"], d["weight"], d["down"], d["up"], d["idx"], bias=d["bias"], scale=0.5), y, yb, DT[dt])
+    wide = torch.full((M, K + 9), float("nan"), device="cuda", dtype=DT[dt])
+    wide[:, 1:K + 1] = d["x"]
+    within(ad.adapter_linear(wide[:, 1:K + 1], d["weight"], d["down"], d["up"], d["idx"].int(), bias=d["bias"], scale=0.5), y, yb, DT[dt])
+
+
+def test_rows_behind_four_gigabytes():
+    """offsets past 32 bits on both sides: 70 000 rows of 36 000 halves (5 GB) out, back and through a product"""
+    T, D, G = 70000, 36000, 3
+    x = torch.empty(T, D, device="cuda", dtype=torch.float16)
+    for a in range(0, T, 10000):
+        x[a:a + 10000] = (torch.arange(a, a + 10000, device="cuda")[:, None] % 1000 + torch.arange(D, device="cuda") % 7).half()
+    idx = torch.arange(T, device="cuda") * 7919 % (G + 1)                 # a quarter has no group
+    plan = ad.route_rows(idx, G)
+    xs = ad.dispatch_rows(x, plan)
+    rows = torch.cat([torch.arange(0, T, 997), torch.arange(T - 50, T)]).cuda()
+    kept = idx[rows] < G
+    assert torch.equal(xs[plan.slot.long()[rows]], x[rows] * kept[:, None])
+    back = ad.combine_rows(xs, plan)
+    assert torch.equal(back[rows], x[rows] * kept[:, None])
+    del xs, back
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    mk = lambda *s: torch.randn(*s, generator=gen, device="cuda").half() * 0.01
+    d = dict(x=x, weight=mk(24, D), bias=mk(24), down=mk(G, 4, D), up=mk(G, 24, 4), idx=torch.where(idx < G, idx, -1))
+    y, yb = oracle_rows(d, 1.0, torch.float16, rows)
+    got = ad.adapter_linear(x, d["weight"], d["down"], d["up"], d["idx"], bias=d["bias"])
+    fits = (y.abs() < 6e4).all(1)
+    assert int(fits.sum()) > 50
+    within(got[rows][fits], y[fits], yb[fits], torch.float16)
+
+
+def test_few_rows_captured_beside_another_graph():
+    """a decoding step (indices, no plan) and a larger one, each in a graph of its own, replayed on two streams at once"""
+    K, N, L, R = 512, 384, 5, 8
+    small, big = on_the_device(7, K, N, L, R, torch.bfloat16, 1), on_the_device(100, K, N, L, R, torch.bfloat16, 2)
+    run = lambda d: ad.adapter_linear(d["x"], d["weight"], d["down"], d["up"], d["idx"], bias=d["bias"])
+    graphs = []
+    for d in (small, big):
+        run(d)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run(d)
+        graphs.append((d, g, out, torch.cuda.Stream()))
+    for r in range(4):
+        for d, *_ in graphs:
+            d["x"].copy_(torch.randn(d["x"].shape, device="cuda"))
+            d["idx"].random_(-1, L + 1)
+        want = [run(d) for d, *_ in graphs]
+        torch.cuda.synchronize()
+        for _, g, _, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, w) for (_, _, out, _), w in zip(graphs, want)), r
+
+
+def test_a_copied_plan_has_its_own_buffer():
+    import copy
+    import pickle
+    idx = groups(500, 2, 6, 4).cuda()
+    plan = ad.route_rows(idx, 6)
+    x = torch.randn(500, 12, device="cuda")
+    want = ad.dispatch_rows(x, plan)
+    other, rows = copy.deepcopy(plan), pickle.loads(pickle.dumps(plan.sorted()))
+    plan.buf.fill_(0)
+    assert other.buf.data_ptr() != plan.buf.data_ptr() and torch.equal(ad.dispatch_rows(x, other), want)
+    assert torch.equal(rows.offsets, other.offsets) and torch.equal(rows.plan.slot, other.slot)
+
+
+def test_tensor_level_calls_check_their_arguments():
+    d = on_the_device(80, 32, 24, 3, 4, torch.float32, 3)
+    plan = ad.route_rows(d["idx"], 3)
+    base = dict(x=d["x"], weight=d["weight"], down=d["down"], up=d["up"], rows=plan, bias=d["bias"])
+    y, h = ops.adapter_linear(**base)
+    assert torch.equal(y, ad.adapter_linear(d["x"], d["weight"], d["down"], d["up"], plan, bias=d["bias"]))
+    for kw, err in [(dict(x=d["x"][:79]), ValueError), (dict(x=d["x"].t()), ValueError), (dict(x=d["x"].half()), TypeError), (dict(weight=d["weight"][:, :31]), ValueError),
+                    (dict(weight=d["weight"].t().contiguous().t()), ValueError), (dict(down=d["down"][:, :3]), ValueError), (dict(up=d["up"][:2]), ValueError),
+                    (dict(bias=d["bias"][:3]), ValueError), (dict(rows=d["idx"]), TypeError), (dict(rows=ad.route_rows(d["idx"], 2)), ValueError),
+                    (dict(scale_of=torch.ones(2, device="cuda")), ValueError)]:
+        with pytest.raises(err):
+            ops.adapter_linear(**{**base, **kw})
+    few = {k: v for k, v in base.items() if k != "rows"}
+    few["x"] = d["x"][:9]
+    for g, err in [(d["idx"], ValueError), (d["idx"][:9].float(), ValueError), (d["idx"][:9].cpu(), ValueError)]:
+        with pytest.raises(err):
+            ops.adapter_linear_few(groups=g, **few)
+    with pytest.raises(Exception, match="64 rows"):
+        ops.adapter_linear_few(groups=d["idx"], **{**few, "x": d["x"]})
+    back = dict(g=d["g"], x=d["x"], weight=d["weight"], down=d["down"], up=d["up"], rows=plan, h=h)
+    assert ops.adapter_backward(**back)[0].shape == d["x"].shape
+    for kw, err in [(dict(g=d["g"][:, :5]), ValueError), (dict(h=h[:8]), ValueError), (dict(g=d["g"].half()), TypeError)]:
+        with pytest.raises(err):
+            ops.adapter_backward(**{**back, **kw})
+    z = ops.dispatch_rows(d["x"], plan)
+    for zz, err in [(z[:70], ValueError), (z[:, :5], ValueError), (z.half(), ValueError)]:
+        with pytest.raises(err):
+            ops.combine_rows_backward(d["x"], zz, plan, torch.ones(80, device="cuda"))
+
+
+def test_a_subject_for_all_rays_in_chunks():
+    """one subject handed over once, or per ray, whole or in chunks: the same picture"""
+    from cases import build
+    raycaster = importlib.import_module("a-nerf_amd.raycaster")
+    render = importlib.import_module("a-nerf_amd.render")
+    pipeline = importlib.import_module("a-nerf_amd.pipeline")
+    c = build("eval_hier")
+    t = lambda v: torch.tensor(np.asarray(v), dtype=torch.float32).cuda()
+    ck = dict(cutoff=True, cutoff_dist=0.5, cutoff_inputs=True, cutoff_dim=24)
+    ev, eb, ed = (networks.get_embedder(7, 0, 24, cutoff_kwargs=dict(ck))[0], networks.get_embedder(0, 0, 72)[0],
+                  networks.get_embedder(4, 0, 72, cutoff_kwargs=dict(ck, dist_inputs=True))[0])
+    nets = [networks.NeRF(D=8, W=256, input_ch=360, input_ch_bones=72, input_ch_views=648, use_viewdirs=True) for _ in range(2)]
+    caster = raycaster.RayCaster(nets[0], ev, eb, ed, network_fine=nets[1]).cuda().requires_grad_(False).eval()
+    ads = [ad.NetAdapters(n, 3, rank=4) for n in nets]
+    with torch.no_grad():
+        for a in ads:
+            for name in ad.LAYERS:
+                a.up(name).normal_(0, 0.05)
+    caster.set_adapters(*ads)
+    rb, n = pipeline.make_ray_batch(t(c["rays_o"]), t(c["rays_d"])), c["n"]
+    one = lambda v: t(v)[:1]
+    call = lambda subject, chunk: render.batchify_rays(rb, chunk, caster, N_samples=c["S"], kp_batch=one(c["kp"]), skts=one(c["skts"]), cyls=one(c["cyls"]),
+                                                       subject_idxs=subject, N_importance=c["Ni"], preproc_kwargs={"density_scale": 1.0})["rgb_map"]
+    per_ray = torch.full((n,), 2, device="cuda")
+    want = call(per_ray, n)
+    assert torch.equal(call(per_ray[:1], n), want)
+    chunk = n // 2 + 1
+    assert torch.equal(call(per_ray[:1], chunk), call(per_ray, chunk))
+    assert not torch.equal(call(torch.zeros_like(per_ray), n), want)
