@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 
 // ------------------------------------------------------------------------------------------------------------------ y = x W^T ...
 // BM positions x BN outputs a workgroup of WM x WN waves, 16 x 16 MFMA blocks with W's rows as the first operand, so that a lane ends
-// with four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, double-buffered; 16-byte
+// with four consecutive outputs of one row.  The contraction goes through LDS 128 bytes of every row at a time, NS stages deep; 16-byte
 // chunk c of row r lies at chunk c ^ (r & 7), which spreads a fragment read over the banks.  DIRECT: global_load_lds_dwordx4, eight rows
 // an instruction, the lanes fetching the chunks in the order they have to lie in LDS (16-byte aligned rows); otherwise through registers,
 // at any alignment.
@@ -202,7 +202,7 @@ struct MainArgs {
 
 constexpr int FOLD = 16;
 
-template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
+template <int DT, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
 __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) k_main(MainArgs P) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, KB = 8 * EPC;        // elements of a 128-byte row piece
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   constexpr int BS = 16, TM = BM / WM, TN = BN / WN, MI = TM / BS, NI = TN / BS;
   constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW;       // 16-byte loads of a lane and stage
   constexpr int STAGE = (BM + BN) * 8;                    // 16-byte units
-  extern __shared__ u32x4 lds[];                          // [2][STAGE]
+  extern __shared__ u32x4 lds[];                          // [NS][STAGE]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane % BS, q = lane / BS;
   const int wm = wave % WM, wn = wave / WM;
   // workgroups go round-robin to the 8 XCDs: each XCD gets a contiguous range of the tile order, in which 4 row tiles share a column of W
@@ -296,7 +296,9 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       fetch_regs(s);
     }
   };
-  start(first, 0);
+#pragma unroll
+  for (int s = 0; s < (DIRECT ? NS - 1 : 1); ++s)
+    if (first + s < stages) start(first + s, s);
   f32x4 acc[MI][NI];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   }
   // A half stage's rows of x are taken in two groups, and every group's fragments are read from LDS while the products of the group
   // before it run (two sets of W's fragments, one of each group of x's), so that the matrix units need not wait for LDS.  The one barrier
-  // of a stage lies before its last group's products: there every wave has read the last of stage s, whose buffer stage s + 2 may then
+  // of a stage lies before its last group's products: there every wave has read the last of stage s, whose buffer stage s + NS may then
   // overwrite, and every wave's loads of stage s + 1 have arrived.
   constexpr int MG = MI / 2;
   static_assert(MI % 2 == 0, "two groups of row blocks a half stage");
@@ -404,13 +406,21 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
         for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[g * MG + m][n] = Elem<DT>::mma(wf[h][n], xf[g][m], acc[g * MG + m][n], e);
   };
-  auto arrive = [&]() {
-    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // waits for the oldest stage in flight; `all`: of NS - 1
+  auto arrive = [&](bool all) {
+    if (DIRECT) {
+      if (NS > 2 && all) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * (XL + WL)) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
     __syncthreads();
   };
   if (!DIRECT) put(0);
-  arrive();
-  if (first + 1 < stages) start(first + 1, 1);
+  arrive(first + NS - 1 <= stages);
+  if (DIRECT) {
+    if (first + NS - 1 < stages) start(first + NS - 1, NS - 1);
+  } else if (first + 1 < stages) {
+    start(first + 1, 1);
+  }
   read_w(0, 0);
   read_x(0, 0, 0);
   auto zero_behind = [&](u32x4* f, int n, int h) {      // fragments of the partial stage: chunks behind the row
@@ -431,21 +441,28 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     if (PART) zero_behind(xf[1], MG, 1);
     products(1, 0);
     if (s + 1 < stages) {
-      if (!DIRECT) put(buf ^ 1);
-      arrive();
-      if (s + 2 < stages) start(s + 2, buf);
-      read_w(buf ^ 1, 0);
-      read_x(buf ^ 1, 0, 0);
+      const int next = buf + 1 == NS ? 0 : buf + 1;
+      if (!DIRECT) put(next);
+      arrive(s + NS <= stages);
+      if (s + NS < stages) start(s + NS, buf);
+      read_w(next, 0);
+      read_x(next, 0, 0);
     }
     products(1, 1);
   };
-  // the buffer is a constant of the loop's code: two stages a turn
+  // the buffer is a constant of the loop's code: NS stages a turn
   const int whole = DIRECT && full < stages ? full : stages;
-  for (int s = first; s < whole; s += 2) {
+  for (int s = first; s < whole; s += NS) {
     stage(s, 0, Const<0>());
     if (s + 1 < whole) stage(s + 1, 1, Const<0>());
+    if constexpr (NS > 2) {
+      if (s + 2 < whole) stage(s + 2, 2, Const<0>());
+    }
+    if constexpr (NS > 3) {
+      if (s + 3 < whole) stage(s + 3, 3, Const<0>());
+    }
     if constexpr (F32) {
-      if ((s - first) % FOLD == FOLD - 2) {
+      if ((s - first) % FOLD == FOLD - NS) {
 #pragma unroll
         for (int m = 0; m < MI; ++m)
 #pragma unroll
@@ -456,7 +473,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       }
     }
   }
-  if (DIRECT && full < stages) stage(full, (full - first) & 1, Const<1>());
+  if (DIRECT && full < stages) stage(full, (full - first) % NS, Const<1>());
 
   // ---- bias, rounding, store.  A lane holds four outputs of its row in each block.  fp32: 16 bytes, stored as they are
   if constexpr (F32) {
@@ -491,7 +508,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     typedef decltype(one) S;
     typedef S four __attribute__((ext_vector_type(4)));
     constexpr int LINE = TN * (int)sizeof(S) + 16, ROWS = MG * BS, PER = 16 / (int)sizeof(S), LPR = TN / PER, RPI = 64 / LPR;
-    static_assert(NW * ROWS * LINE <= 2 * STAGE * 16 && ROWS % RPI == 0, "the staged rows fit where the stages were");
+    static_assert(NW * ROWS * LINE <= NS * STAGE * 16 && ROWS % RPI == 0, "the staged rows fit where the stages were");
     char* mine = reinterpret_cast<char*>(lds) + wave * (ROWS * LINE);
     const long long cw = n0 + wn * TN;
     const int r0 = lane / LPR, c = lane % LPR * PER;
@@ -677,34 +694,57 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto walk = [&](long long s0, auto depth, auto tail) {
-    constexpr int D = decltype(depth)::value;
-    u32x4 wv[D][NT], xv[D][MT];
+  // two sets of operands: the next turn's loads are in flight while a turn's products run (48 x 4096 -> 8192 bf16: 28.0 -> 24.7 us)
+  struct Step {
+    u32x4 w[DEPTH][NT], x[DEPTH][MT];
+  };
+  auto fetch = [&](Step& S, long long s0, auto depth, auto tail) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
+    for (int d = 0; d < decltype(depth)::value; ++d) {
       const long long k = (s0 + (d >> 1) * 2 * FEW_WAVES + (d & 1)) * STEP + q * EPC;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) wv[d][n] = decltype(tail)::value ? load_tail<DT>(wr[n], k, K) : load16(wr[n] + k);
+      for (int n = 0; n < NT; ++n) S.w[d][n] = decltype(tail)::value ? load_tail<DT>(wr[n], k, K) : load16(wr[n] + k);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) xv[d][m] = decltype(tail)::value ? load_tail<DT>(xr[m], k, K) : load16(xr[m] + k);
+      for (int m = 0; m < MT; ++m) S.x[d][m] = decltype(tail)::value ? load_tail<DT>(xr[m], k, K) : load16(xr[m] + k);
     }
+  };
+  auto products = [&](const Step& S, auto depth) {
 #pragma unroll
-    for (int d = 0; d < D; ++d)
+    for (int d = 0; d < decltype(depth)::value; ++d)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(wv[d][n], xv[d][m], acc[m][n], e);
+          for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(S.w[d][n], S.x[d][m], acc[m][n], e);
+  };
+  auto walk = [&](long long s0, auto tail) {
+    Step S;
+    fetch(S, s0, Const<1>(), tail);
+    products(S, Const<1>());
   };
   const long long steps = K / STEP;
   long long s = 2 * wave;
-  for (; s + (DEPTH - 2) * FEW_WAVES + 1 < steps; s += DEPTH * FEW_WAVES) walk(s, Const<DEPTH>(), Const<0>());
-  for (; s < steps; s += 2 * FEW_WAVES) {
-    walk(s, Const<1>(), Const<0>());
-    if (s + 1 < steps) walk(s + 1, Const<1>(), Const<0>());
+  const long long turn = DEPTH * FEW_WAVES, reach = (DEPTH - 2) * FEW_WAVES + 1;
+  if (s + reach < steps) {
+    Step S[2];
+    fetch(S[0], s, Const<DEPTH>(), Const<0>());
+    for (;;) {
+      if (s + turn + reach >= steps) { products(S[0], Const<DEPTH>()); s += turn; break; }
+      fetch(S[1], s + turn, Const<DEPTH>(), Const<0>());
+      products(S[0], Const<DEPTH>());
+      s += turn;
+      if (s + turn + reach >= steps) { products(S[1], Const<DEPTH>()); s += turn; break; }
+      fetch(S[0], s + turn, Const<DEPTH>(), Const<0>());
+      products(S[1], Const<DEPTH>());
+      s += turn;
+    }
   }
-  if (steps * STEP < K && wave == (int)(steps % (2 * FEW_WAVES)) / 2) walk(steps, Const<1>(), Const<1>());
+  for (; s < steps; s += 2 * FEW_WAVES) {
+    walk(s, Const<0>());
+    if (s + 1 < steps) walk(s + 1, Const<0>());
+  }
+  if (steps * STEP < K && wave == (int)(steps % (2 * FEW_WAVES)) / 2) walk(steps, Const<1>());
   // 8 -> 4 -> 2 -> 1 waves
 #pragma unroll
   for (int half = FEW_WAVES / 2; half; half >>= 1) {
@@ -977,11 +1017,11 @@ __global__ void __launch_bounds__(256) k_pad(PadJob a, PadJob b, long long K, lo
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- launchers
-template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
+template <int DT, int BM, int BN, int WM, int WN, bool DIRECT, int NS = 2>
 static int run_main(const MainArgs& P, hipStream_t st) {
   static unsigned long long done = 0;
-  constexpr int bytes = 2 * (BM + BN) * 128;
-  const auto kernel = k_main<DT, BM, BN, WM, WN, DIRECT>;
+  constexpr int bytes = NS * (BM + BN) * 128;
+  const auto kernel = k_main<DT, BM, BN, WM, WN, NS, DIRECT>;
   ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes, &done);
   kernel<<<(unsigned)((P.M + BM - 1) / BM * ((P.N + BN - 1) / BN) * P.splits), WM * WN * 64, bytes, st>>>(P);
   const int rc = check_launch("k_main");
@@ -1004,33 +1044,40 @@ static int split_of(int dtype, long long M, long long K, long long N) {
 // Tile: the larger, the fewer LDS reads a product (a 256 x 256 tile's waves read 3/8 of what a 64 x 64 tile's do), but the tiles of one CU
 // run one after the other, and what the last round leaves idle grows.  Cost: tiles of the busiest CU x size / rate; the rates are
 // what the tiles reach where there are many of them, relative to 256 x 128 (bf16, 8192 x 4096 x 4096, rank 8: 256 x 256 271 us, 256 x 128 307,
-// 128 x 128 310, 128 x 64 360, 64 x 64 432; 1000 x 1000 x 1000: 45, 29, 25, 19, 16).  fp32 is bound by its products, and one size is as fast
-// as the other (1941 .. 2009 us).
+// 128 x 128 310, 128 x 64 360, 64 x 64 432; 1000 x 1000 x 1000: 45, 29, 25, 19, 16), times what they reach with one or two tiles a CU, whose
+// few waves do not hide their waits.  There the contraction is four stages deep in LDS, three of them in flight (bf16, 4096 inputs, 8192
+// outputs, two deep -> four deep: 128 rows on 64 x 64 52 -> 28 us, 256 rows 53 -> 41, 512 rows on 128 x 128 63 -> 50); with more tiles a CU two
+// stages leave room for more workgroups, and the larger tiles gain nothing from a third.  fp32 is bound by its products: one size is as
+// fast as the other (1941 .. 2009 us), and four stages help one tile a CU only (128 x 4096 -> 8192: 99 -> 83 us, 1024 x 2048 -> 2048: 69 -> 71).
 template <int DT>
 static int launch_main(const MainArgs& P, hipStream_t st) {
   constexpr long long es = sizeof(typename Elem<DT>::T), span = 1ll << 32;      // DIRECT's offsets have 32 bits
   const bool direct = (((uintptr_t)P.x | (uintptr_t)P.w) & 15) == 0 && P.K % Elem<DT>::EPC == 0 && P.ldx % Elem<DT>::EPC == 0 &&
                       P.ldw % Elem<DT>::EPC == 0 && P.M * P.ldx * es < span && P.N * P.ldw * es < span;
-  auto cost = [&](int bm, int bn, double rate, bool few_waves) {
-    const long long tiles = (P.M + bm - 1) / bm * ((P.N + bn - 1) / bn), mine = (tiles + 255) / 256;
-    return (double)mine * bm * bn / (few_waves && mine == 1 ? 0.7 * rate : rate);      // (one wave a SIMD does not hide its own waits)
-  };
   constexpr bool F32 = DT == ANERF_F32;
-  const double c64 = cost(64, 64, F32 ? 0.97 : 0.6, true), c128 = cost(128, 128, F32 ? 1.0 : 0.87, true);
+  auto a_cu = [&](int bm, int bn) { return ((P.M + bm - 1) / bm * ((P.N + bn - 1) / bn) * P.splits + 255) / 256; };      // tiles of the busiest CU
+  auto cost = [&](int bm, int bn, double rate, double one, double two) {
+    const long long mine = a_cu(bm, bn);
+    return (double)mine * bm * bn / (rate * (mine == 1 ? one : mine == 2 ? two : 1.0));
+  };
+  const double c64 = F32 ? cost(64, 64, 0.97, 0.7, 1.0) : cost(64, 64, 0.6, 0.55, 0.8);
+  const double c128 = F32 ? cost(128, 128, 1.0, 0.7, 1.0) : cost(128, 128, 0.87, 0.85, 1.0);
+  const bool deep = a_cu(64, 64) <= (F32 ? 1 : 2);
+  auto run64 = [&]() { return deep ? run_main<DT, 64, 64, 2, 2, true, 4>(P, st) : run_main<DT, 64, 64, 2, 2, true>(P, st); };
   if (P.splits > 1 || !direct || F32) {
     const bool small = P.splits > 1 || c64 <= c128;
-    if (direct) return small ? run_main<DT, 64, 64, 2, 2, true>(P, st) : run_main<DT, 128, 128, 2, 2, true>(P, st);
+    if (direct) return small ? run64() : run_main<DT, 128, 128, 2, 2, true>(P, st);
     return small ? run_main<DT, 64, 64, 2, 2, false>(P, st) : run_main<DT, 128, 128, 2, 2, false>(P, st);
   }
   if constexpr (!F32) {
-    const double c96 = cost(128, 64, 0.75, true), c192 = cost(256, 128, 0.97, false), c256 = cost(256, 256, 1.05, false);
+    const double c96 = cost(128, 64, 0.75, 0.6, 0.8), c192 = cost(256, 128, 0.97, 1.0, 1.0), c256 = cost(256, 256, 1.05, 1.0, 1.0);
     const double least = fmin(fmin(fmin(c64, c128), c96), fmin(c192, c256));
     if (c256 == least) return run_main<DT, 256, 256, 2, 4, true>(P, st);
     if (c192 == least) return run_main<DT, 256, 128, 4, 2, true>(P, st);
-    if (c128 == least) return run_main<DT, 128, 128, 2, 2, true>(P, st);
-    if (c96 == least) return run_main<DT, 128, 64, 2, 2, true>(P, st);
+    if (c128 == least) return a_cu(128, 128) == 1 ? run_main<DT, 128, 128, 2, 2, true, 4>(P, st) : run_main<DT, 128, 128, 2, 2, true>(P, st);
+    if (c96 < c64) return run_main<DT, 128, 64, 2, 2, true>(P, st);
   }
-  return run_main<DT, 64, 64, 2, 2, true>(P, st);
+  return run64();
 }
 
 // what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][2 Rp] (16-bit types) | factor [n_rows] (fp16); byte offsets

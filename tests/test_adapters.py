@@ -775,3 +775,13 @@ def test_a_subject_for_all_rays_in_chunks():
     chunk = n // 2 + 1
     assert torch.equal(call(per_ray[:1], chunk), call(per_ray, chunk))
     assert not torch.equal(call(torch.zeros_like(per_ray), n), want)
+
+
+@pytest.mark.parametrize("K", [8, 64, 72, 128, 192, 200, 256, 264, 320, 456, 1000, 4104])
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_every_number_of_stages(K, dt):
+    """contractions of fewer stages than are in flight, as many, and more, whole and ending inside one; split where they are long"""
+    for M, N in ((150, 136), (70, 2050)):
+        d = on_the_device(M, K, N, 6, 8, DT[dt], K)
+        y, yb = oracle_rows(d, 0.5, DT[dt], torch.arange(M, device="cuda"))
+        within(ad.adapter_linear(d["x"], d["weight"], d["down"], d["up"], ad.route_rows(d["idx"], 6), bias=d["bias"], scale=0.5), y, yb, DT[dt])
