@@ -788,10 +788,12 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
 // part[piece] = sum over the piece's positions p of Z[order[p]][c] * V[p][j]        (Z = x, V = u: dA;  Z = g, V = h: dB)
 // The contraction runs over rows, so that v_mfma_f32_16x16x4_f32 takes its operands as they lie in memory: lane (i, q) loads
 // columns 4i .. 4i+3 of row q of a group of four, element e being its operand for the block of columns 4i + e, and V[p][16n + i].
-// Values of 16-bit types become fp32 on the way (h and u stay whole): up to rank 32 the loads of Z are what bounds it, not the MFMAs.
-// A workgroup owns 64 columns x 16*NJ ranks of a piece; its four waves take every fourth group of rows and are added through LDS.
+// Values of 16-bit types become fp32 on the way (h and u stay whole).  A workgroup owns 64 columns x 16*NJ ranks of a piece; its four waves
+// take every fourth group of rows and are added through LDS, a quarter of the sums each.  What bounds it is the latency of Z's loads, so
+// the next turn's rows are on their way while a turn's products run, and two waves a SIMD are asked for (with one, whose registers then hold
+// more: rank 128, 8192 x (1024 + 1024) fp16, the whole backward 229 instead of 170 us).
 // BY_RANK: part [piece][Rp][C] (operand order Z, V), else [piece][C][Rp] (V, Z): a lane ends with four values that lie together.
-constexpr int TG_WAVES = 4, TG_COLS = 64, TG_DEPTH = 4;
+constexpr int TG_WAVES = 4, TG_COLS = 64, TG_DEPTH = 2;
 
 struct GradJob {
   const void* Z;
@@ -828,75 +830,91 @@ __device__ __forceinline__ void thin_grad(const GradJobs& G, const GradJob& J, i
   for (int e = 0; e < 4; ++e)
 #pragma unroll
     for (int n = 0; n < NJ; ++n) acc[e][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b = p0 + 4 * wave; b < p1; b += 4 * TG_WAVES * TG_DEPTH) {
-    f32x4 z[TG_DEPTH];
+  // two sets of operands: the next turn's rows are on their way while a turn's products run
+  struct Rows {
+    vec z[TG_DEPTH];
     float v[TG_DEPTH][NJ];
+  };
+  constexpr int TURN = 4 * TG_WAVES * TG_DEPTH;
+  auto fetch = [&](Rows& S, int b) {
 #pragma unroll
     for (int d = 0; d < TG_DEPTH; ++d) {
       const int p = b + 4 * TG_WAVES * d + q;
       const bool on = p < p1;
-      z[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) v[d][n] = on && j0 + 16 * n < Rp ? V[(long long)p * Rp + j0 + 16 * n + i] : 0.f;
+      for (int e = 0; e < 4; ++e) S.z[d][e] = (E)0.f;
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) S.v[d][n] = on && j0 + 16 * n < Rp ? V[(long long)p * Rp + j0 + 16 * n + i] : 0.f;
       if (on) {
         const E* zr = Z + (long long)(order ? order[p] : p) * ldz + c;
         if (whole) {
-          vec w;
-          __builtin_memcpy(&w, zr, sizeof(w));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) z[d][e] = (float)w[e];
+          __builtin_memcpy(&S.z[d], zr, sizeof(vec));
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c + e < C) z[d][e] = (float)zr[e];
+            if (c + e < C) S.z[d][e] = zr[e];
         }
       }
     }
+  };
+  auto products = [&](const Rows& S) {
 #pragma unroll
     for (int d = 0; d < TG_DEPTH; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int n = 0; n < NJ; ++n)
-          acc[e][n] = BY_RANK ? __builtin_amdgcn_mfma_f32_16x16x4f32(z[d][e], v[d][n], acc[e][n], 0, 0, 0)
-                              : __builtin_amdgcn_mfma_f32_16x16x4f32(v[d][n], z[d][e], acc[e][n], 0, 0, 0);
+          acc[e][n] = BY_RANK ? __builtin_amdgcn_mfma_f32_16x16x4f32((float)S.z[d][e], S.v[d][n], acc[e][n], 0, 0, 0)
+                              : __builtin_amdgcn_mfma_f32_16x16x4f32(S.v[d][n], (float)S.z[d][e], acc[e][n], 0, 0, 0);
+  };
+  {
+    Rows S[2];
+    int b = p0 + 4 * wave;
+    fetch(S[0], b);
+    for (; b < p1; b += 2 * TURN) {
+      fetch(S[1], b + TURN);
+      products(S[0]);
+      if (b + TURN >= p1) break;
+      fetch(S[0], b + 2 * TURN);
+      products(S[1]);
+    }
   }
-  if (wave) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+  for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) red[wave - 1][e * NJ + n][lane] = acc[e][n];
-  }
+    for (int n = 0; n < NJ; ++n) red[wave][e * NJ + n][lane] = acc[e][n];
   __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int w = 0; w < TG_WAVES - 1; ++w)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int n = 0; n < NJ; ++n) acc[e][n] += red[w][e * NJ + n][lane];
+  // every wave adds and stores a quarter
   const long long base = (long long)blockIdx.y * Rp * C, c0 = (long long)bx * TG_COLS;
 #pragma unroll
   for (int n = 0; n < NJ; ++n) {
     if (j0 + 16 * n >= Rp) break;
-    if (BY_RANK) {      // block e, register r: column 16q + 4r + e of rank 16n + i
-      float* o = part + base + (long long)(j0 + 16 * n + i) * C + c0 + 16 * q;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (BY_RANK) {      // register r of block e: column 16q + 4r + e of rank 16n + i; this wave's r is its number
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int w = 0; w < TG_WAVES; ++w)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += red[w][e * NJ + n][lane][wave];
+      const long long col = c0 + 16 * q + 4 * wave;
+      float* o = part + base + (long long)(j0 + 16 * n + i) * C + col;
+      if (col + 4 <= C) {
+        store16(o, __builtin_bit_cast(u32x4, v));
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (c0 + 16 * q + 4 * r + e < C) o[4 * r + e] = acc[e][n][r];
-    } else {            // block e, register r: rank 16n + 4q + r of column 4i + e
+          if (col + e < C) o[e] = v[e];
+      }
+    } else {            // register r of block e: rank 16n + 4q + r of column 4i + e; this wave's e is its number
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < C) *reinterpret_cast<f32x4*>(part + base + (c + e) * Rp + j0 + 16 * n + 4 * q) = acc[e][n];
+      for (int w = 0; w < TG_WAVES; ++w) v += red[w][wave * NJ + n][lane];
+      if (c + wave < C) *reinterpret_cast<f32x4*>(part + base + (c + wave) * Rp + j0 + 16 * n + 4 * q) = v;
     }
   }
 }
 
 template <int DT, int NJ>
-__global__ void __launch_bounds__(TG_WAVES * 64) k_thin_grad(GradJobs G) {
-  __shared__ f32x4 red[TG_WAVES - 1][4 * NJ][64];
+__global__ void __launch_bounds__(TG_WAVES * 64, 2) k_thin_grad(GradJobs G) {
+  __shared__ f32x4 red[TG_WAVES][4 * NJ][64];
   const int second = (int)blockIdx.x >= G.j[0].blocks;
   const GradJob& J = G.j[second];
   const int bx = (int)blockIdx.x - (second ? G.j[0].blocks : 0);
@@ -1191,11 +1209,12 @@ int launch_adapter_few(const AnerfAdapterIO& A, const void* groups, int wide, hi
   }
 }
 
-// rows of a piece of k_thin_grad: about 1024 workgroups (a chip full of them twice over), but 64 rows at least (a piece writes C x Rp floats)
+// rows of a piece of k_thin_grad: 64 at least, since a piece writes C x Rp floats, and so many that there are about 1024 workgroups -- 512 with
+// more than 32 ranks, whose sums weigh more (whole backward of 8192 x (2048 + 2048), rank 64: 225 -> 214 us; rank 16: 324 -> 333)
 static int grad_ranks(int Rp) { return Rp <= 16 ? 1 : Rp <= 32 ? 2 : 4; }
 static int grad_rows(long long M, long long C, int Rp) {
   const long long blocks = (C + TG_COLS - 1) / TG_COLS * ((Rp + 16 * grad_ranks(Rp) - 1) / (16 * grad_ranks(Rp)));
-  const long long pieces = (1024 + blocks - 1) / blocks;
+  const long long want = grad_ranks(Rp) == 4 ? 512 : 1024, pieces = (want + blocks - 1) / blocks;
   const long long rows = ((M + pieces - 1) / pieces + 63) / 64 * 64;
   return (int)(rows < 64 ? 64 : rows);
 }
