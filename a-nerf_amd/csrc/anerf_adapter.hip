@@ -18,9 +18,12 @@ namespace anerf {
 // ------------------------------------------------------------------------------------------------------------ h = s_i x A_i^T
 // HBM-bound on x.  The four waves split the contraction (every fourth 64-byte step), each holding all 32 rows x 16*NJ ranks of the
 // piece in MFMA accumulators, fed straight from memory: a row of A serves 32 rows of x, and nothing is read twice from HBM.
+// 65520 x 688 fp32, rank 8: 32 us, 5.6 TB/s; 8192 x 4096 bf16, 24 adapters of rank 32 (73 MB): 21 us.  Pieces of 16 rows read A twice as
+// often, 64 rows leave CUs idle at a few thousand rows.
 // Kept as [position][Rp] fp32 (Rp = rank rounded up to 16, zeros behind the rank) for the gradient of B, and, for the 16-bit types, as what
 // k_main multiplies with: the nearest value hi and the rest lo, [hi of 16 ranks | lo of the same 16] per 16 ranks, which meet [B | B]
 // there -- h keeps 16 (bf16) or 21 (fp16) of its bits.  fp16's range does not hold every h: its rows are scaled first.
+
 // ranks j .. j+3 of a row
 template <typename E>
 __device__ __forceinline__ void store_split(f32x4 v, E* row, int j) {
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   }
 }
 
-// fp16 with more ranks than a workgroup of k_thin holds: the rows' scaling and splitting
+// fp16 with more ranks than a workgroup of k_thin holds: the rows' scaling and splitting (8192 rows of rank 128: 5 us)
 __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h, const int32_t* __restrict__ kept, int Rp, _Float16* __restrict__ split,
                                                     float* __restrict__ factor) {
   const int p = blockIdx.x * 16 + (threadIdx.x >> 4), i = threadIdx.x & 15;
@@ -188,6 +191,9 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 // blocks of its rows; a block that two adapters share takes it by row (a NaN in one adapter stays with its rows).
 // fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set, so that no chain of
 // additions is longer than 8 * FOLD + K / (32 * FOLD).
+// Bound by the matrix units.  bf16, 8192 x 4096 -> 4096 with 24 adapters of rank 32: 245 us, 1140 TFLOP/s (without adapters, once the clocks
+// allow it, 1305; a plain product of that shape by the BLAS 1300 .. 1380); fp32, 65536 x 688 -> 256: 182 us, 127 TFLOP/s (the BLAS 135),
+// 8192 x 4096 -> 4096: 147 TFLOP/s of the 150 that it reaches.
 struct MainArgs {
   const void *x, *w, *bias, *up;
   const int32_t *offsets, *order;
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
   if constexpr (!F32) emit(E(), static_cast<E*>(P.y), static_cast<const E*>(P.bias));
 }
 
-// y = the parts' sum in order + bias; [M][N] as one row of values
+// y = the parts' sum in order + bias; [M][N] as one row of values (128 x 4096 outputs in 4 parts: 4 us)
 template <int DT>
 __global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ part, int splits, long long all, long long N, const typename Elem<DT>::T* __restrict__ bias,
                                                    typename Elem<DT>::T* __restrict__ y) {
@@ -606,6 +612,8 @@ __global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ par
 //   k_few       a workgroup owns 16*NT outputs of all rows; its eight waves take every eighth 128 bytes of W's rows straight into MFMA operands
 //               (W is read once, no LDS on its way), x comes from L2, and the waves' sums are added through LDS.  The low-rank term of
 //               an output is a dot of `rank` values in fp32, read in front of the loop, so that B's latency hides behind W's.
+// bf16, rank 16: one row x 4096 -> 4096 5.5 + 7.8 us (W at 4.3 TB/s); 48 rows x 4096 -> 8192 5.8 + 25 us (67 MB of W, 13 MB of B, and
+// 126 MB of x from L2).  The routed kernels take 56 us for the 48 rows: their tiles are 64 rows high and wait for one stage after the other.
 constexpr int FEW_WAVES = 8;
 static_assert(ANERF_FEW_ROWS == 64, "four blocks of 16 rows");
 
@@ -792,6 +800,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
 // take every fourth group of rows and are added through LDS, a quarter of the sums each.  What bounds it is the latency of Z's loads, so
 // the next turn's rows are on their way while a turn's products run, and two waves a SIMD are asked for (with one, whose registers then hold
 // more: rank 128, 8192 x (1024 + 1024) fp16, the whole backward 229 instead of 170 us).
+// 4096 x (2048 + 2048) bf16, 12 adapters of rank 16: 20 us; 24000 x (688 + 256) fp32, rank 8: 28 us (91 MB).
 // BY_RANK: part [piece][Rp][C] (operand order Z, V), else [piece][C][Rp] (V, Z): a lane ends with four values that lie together.
 constexpr int TG_WAVES = 4, TG_COLS = 64, TG_DEPTH = 2;
 
@@ -922,7 +931,8 @@ __global__ void __launch_bounds__(TG_WAVES * 64, 2) k_thin_grad(GradJobs G) {
   else thin_grad<DT, NJ, false>(G, J, bx, red);
 }
 
-// adds an adapter's pieces in their order; many pieces an adapter (ways = 4): wave w those of q = w mod 4, then the four sums.  BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.
+// adds an adapter's pieces in their order; many pieces an adapter (ways = 4): wave w those of q = w mod 4, then the four sums.
+// BY_RANK: out[i][j][c] (dA), else out[i][c][j] (dB).  Adapters without rows get zeros.  4096 x (2048 + 2048), 12 adapters of rank 16: 7 us.
 template <int DT>
 __global__ void __launch_bounds__(256) k_thin_grad_sum(GradJobs G) {
   typedef typename Elem<DT>::T E;
@@ -969,7 +979,8 @@ struct TransposeJobs {
   TransposeJob j[3];
 };
 
-// 64 x 64 values a workgroup through LDS, 16 bytes a lane on both sides where the rows allow it
+// 64 x 64 values a workgroup through LDS, 16 bytes a lane on both sides where the rows allow it.  HBM- and latency-bound: W 2048 x 2048
+// and twelve pairs of rank 16, bf16: 7.5 us.
 template <typename U>
 __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   constexpr int V = 16 / sizeof(U);
@@ -1013,7 +1024,8 @@ __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   }
 }
 
-// rows with zeros behind them up to a multiple of 128 bytes, 16-byte aligned: what k_main's direct loads want
+// rows with zeros behind them up to a multiple of 128 bytes, 16-byte aligned: what k_main's direct loads want.  HBM-bound: x 8192 x 4097 and
+// W 4096 x 4097 bf16 36 us (202 MB, 5.6 TB/s).
 struct PadJob {
   const void* in;
   void* out;

@@ -599,7 +599,8 @@ typedef struct AnerfAdapterIO {
   void* h;
 } AnerfAdapterIO;
 int64_t anerf_adapter_h_size(const AnerfAdapterIO* io);
-/* workspace: anerf_adapter_workspace_size bytes (0 unless the rows are few), 16-byte aligned. */
+/* workspace: anerf_adapter_workspace_size bytes of the same io (its pointers and strides count: unaligned rows are copied where outputs and
+ * rows are many, few tiles share their contraction; otherwise 0), 16-byte aligned. */
 int64_t anerf_adapter_workspace_size(const AnerfAdapterIO* io);
 int anerf_adapter_linear(const AnerfAdapterIO* io, void* workspace, int64_t ws_bytes, void* stream);
 /* The same for up to 64 rows (a decoding step), without a plan: groups [n_rows] int64 (wide != 0) or int32 holds every row's adapter, a value
