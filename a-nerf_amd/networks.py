@@ -217,7 +217,7 @@ class NeRF(nn.Module):
 
     def forward_batchify(self, inputs, chunk=1024 * 64, **kwargs):
         # the fused kernel tiles internally; `chunk` is accepted for signature compatibility (nerf.py:90-92)
-        return self.forward(inputs)
+        return self.forward(inputs, kwargs.get("subject_idxs"), kwargs.get("subject_weights"))
 
     def raw2outputs(self, raw, z_vals, rays_d, raw_noise_std=0, pytest=False, B=0.01, rgb_act=torch.sigmoid,
                     act_fn=F.relu, rgb_eps=0.001, **kwargs):

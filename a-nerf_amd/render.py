@@ -77,6 +77,7 @@ def render_path(render_poses, hwf, chunk, render_kwargs, centers=None, kp=None, 
     before the first frame, rays of a box are generated by k_gen_rays, the pose is passed ONCE (stride-0, no per-ray
     replication), the background composite + scatter into the H*W image is k_assemble, and the finished frames stay on
     the device until the end of the call: ONE D2H copy for all of them (per 2 GB of frames).
+    subject_idxs [F|1]: the subject of a frame, where the caster has adapters (RayCaster.set_adapters).
     H / W / focal may be per frame (sequences / arrays, as the h36m loader provides); kp [F|1,24,3], skts [F|1,24,4,4],
     cyls [F|1,5] (or None: derived from kp as kp_to_valid_rays does).  NaN disparities are zeroed (:139-140)."""
     from . import ops, synth
@@ -112,6 +113,8 @@ def render_path(render_poses, hwf, chunk, render_kwargs, centers=None, kp=None, 
     boxes = ops.cyl_bbox(cyls.to(torch.float64)[cyl_idx].contiguous(), c2w_all.to(torch.float64).contiguous(),
                          torch.tensor(hwf64, device=dev), torch.tensor(off, device=dev)).cpu().numpy()     # the one sync up front
     kw = {k: v for k, v in render_kwargs.items() if k not in ("use_viewdirs",)}
+    module = getattr(kw.get("ray_caster"), "module", kw.get("ray_caster"))
+    adapted = subject_idxs is not None and getattr(module, "network", None) is not None and module.network.adapters() is not None
     valid_idxs, bboxes, packed, shapes = [], [], [], []
     out_rgb, out_disp, out_acc = [None] * n_frames, [None] * n_frames, [None] * n_frames
     pending_bytes = 0
@@ -160,7 +163,8 @@ def render_path(render_poses, hwf, chunk, render_kwargs, centers=None, kp=None, 
             cam_i = pick(cams, i)
             ret = batchify_rays(rb, chunk, kp_batch=pick(kp, i), skts=pick(skts, i),
                                 cyls=cyl_i.expand(n, -1).contiguous(), bones=pick(bones, i),
-                                cams=None if cam_i is None else cam_i.expand(n).contiguous(), subject_idxs=None, **kw)
+                                cams=None if cam_i is None else cam_i.expand(n).contiguous(),
+                                subject_idxs=pick(subject_idxs, i) if adapted else None, **kw)
             rgb_img, disp_img, acc_img = ops.assemble_frame(ret["rgb_map"], ret["acc_map"], ret["disp_map"], vidx, rgb_img,
                                                             want_acc=ret_acc)
         parts = [rgb_img.reshape(-1), torch.nan_to_num(disp_img, nan=0.0).reshape(-1)] + ([acc_img.reshape(-1)] if ret_acc else [])
