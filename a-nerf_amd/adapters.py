@@ -153,9 +153,19 @@ class _AdapterFn(torch.autograd.Function):
         return dx, ddown, dup, None, None, None, None, None, None
 
 
-def _refuse(t, name, dim, x):
-    ops._rows_like(t, f"adapter_linear: {name}", None if t is x else x.device, None if t is x else x.dtype)
-    raise ValueError(f"adapter_linear: {name} must have {dim} dimensions, got {tuple(t.shape)}")
+def _check_tensors(x, weight, down, up, bias):
+    """raises what is wrong with them (asked for after the one-line test of adapter_linear failed)"""
+    ops._rows_like(x, "adapter_linear: x")
+    for t, name, dim in ((weight, "weight", 2), (down, "down", 3), (up, "up", 3), (bias, "bias", 1)):
+        if t is None and name == "bias":
+            continue
+        ops._rows_like(t, f"adapter_linear: {name}", x.device, x.dtype)
+        if t.dim() != dim:
+            raise ValueError(f"adapter_linear: {name} must have {dim} dimensions, got {tuple(t.shape)}")
+
+
+def _like(t, dtype, dev, dim):
+    return torch.is_tensor(t) and t.dtype is dtype and t.device == dev and t.ndim == dim
 
 
 def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
@@ -166,13 +176,12 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
     projection alone), the RowPlan of such indices (k = 1; worth keeping where several layers see the same rows), or plan.sorted()
     for dispatched rows.  scale: a number, or a float32 tensor [L].
     Gradients: x, A and B; weight and bias are frozen."""
-    for t, name, dim in ((x, "x", None), (weight, "weight", 2), (down, "down", 3), (up, "up", 3), (bias, "bias", 1)):
-        if t is None and name == "bias":
-            continue
-        if not (torch.is_tensor(t) and t.is_cuda and t.dtype in ops.ROW_DTYPES and t.dtype is x.dtype and t.device == x.device and (dim is None or t.dim() == dim)):
-            _refuse(t, name, dim, x)
-    dev, (N, K), (L, R, down_in), grads = x.device, weight.shape, down.shape, torch.is_grad_enabled()
-    if x.dim() < 1 or x.shape[-1] != K or down_in != K or up.shape != (L, N, R) or (bias is not None and bias.shape[0] != N):
+    dtype, dev = getattr(x, "dtype", None), getattr(x, "device", None)
+    if not (dtype in ops.ROW_DTYPES and x.is_cuda and _like(weight, dtype, dev, 2) and _like(down, dtype, dev, 3) and _like(up, dtype, dev, 3) and
+            (bias is None or _like(bias, dtype, dev, 1))):
+        _check_tensors(x, weight, down, up, bias)
+    (N, K), (L, R, down_in), grads, lead = weight.shape, down.shape, torch.is_grad_enabled(), x.shape[:-1]
+    if x.ndim < 1 or x.shape[-1] != K or down_in != K or up.shape != (L, N, R) or (bias is not None and bias.shape[0] != N):
         raise ValueError(f"adapter_linear: x {tuple(x.shape)}, weight {tuple(weight.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)}" +
                          ("" if bias is None else f", bias {tuple(bias.shape)}") + " do not fit together")
     if N < 1 or K < 1 or L < 1 or R < 1 or L > ops._lib.MAX_GROUPS or R > ops._lib.MAX_RANK:
@@ -187,18 +196,18 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
         if torch.is_grad_enabled() and scale.requires_grad:
             raise ValueError("adapter_linear: scale has no gradient")
         scale, scale_of = 1.0, scale.contiguous()
-    lead = x.shape[:-1]
-    flat = x.reshape(-1, K)
+    flat = x if x.ndim == 2 else x.reshape(-1, K)
     M = flat.shape[0]
     if torch.is_tensor(rows):
-        if tuple(rows.shape) != tuple(lead) and tuple(rows.shape) != (M,):
+        if rows.shape != lead and rows.shape != (M,):
             raise ValueError(f"adapter_linear: {tuple(rows.shape)} adapter indices for rows {tuple(lead)}")
         if rows.device != dev:
             raise ValueError(f"adapter_linear: indices on {rows.device}, rows on {dev}")
-        if rows.dtype not in (torch.int32, torch.int64):
+        if rows.dtype is not torch.int64 and rows.dtype is not torch.int32:
             raise TypeError(f"adapter_linear: adapter indices must be int32 / int64, got {rows.dtype}")
         few = M <= ops._lib.FEW_ROWS and not grads      # a decoding step: no plan, W streams through once
-        rows = rows.reshape(-1).contiguous() if few else route_rows(rows.reshape(-1), L)
+        rows = rows if rows.ndim == 1 else rows.reshape(-1)
+        rows = rows.contiguous() if few else route_rows(rows, L)
     elif not isinstance(rows, (RowPlan, SortedRows)):
         raise TypeError(f"adapter_linear: rows must be indices, a RowPlan or its sorted(), got {type(rows).__name__}")
     if flat.stride(1) != 1 or flat.stride(0) < K:
@@ -206,14 +215,17 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
     weight, down_, up_, bias = weight.contiguous(), down.contiguous(), up.contiguous(), None if bias is None else bias.contiguous()
     scale = float(scale)
     if torch.is_tensor(rows):
-        return ops._adapter_linear_few(flat, weight, down_, up_, rows, bias, scale, scale_of).reshape(lead + (N,))
+        y = ops._adapter_linear_few(flat, weight, down_, up_, rows, bias, scale, scale_of)
+        return y if x.ndim == 2 else y.reshape(lead + (N,))
     if rows.n_rows != M or rows.device != dev or rows.k != 1:
         raise ValueError(f"adapter_linear: a plan of {rows.n_rows} rows with {rows.k} group(s) each on {rows.device} for {M} rows on {dev}")
     if rows.n_groups < L:
         raise ValueError(f"adapter_linear: a plan of {rows.n_groups} groups for {L} adapters")
-    if not grads:
-        return ops._adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of)[0].reshape(lead + (N,))
-    return _AdapterFn.apply(flat, down_, up_, weight, bias, rows, scale, scale_of, _graph_of(x, down, up)).reshape(lead + (N,))
+    if grads:
+        y = _AdapterFn.apply(flat, down_, up_, weight, bias, rows, scale, scale_of, _graph_of(x, down, up))
+    else:
+        y = ops._adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of)[0]
+    return y if x.ndim == 2 else y.reshape(lead + (N,))
 
 
 LAYERS = [f"pts_linears.{i}" for i in range(8)] + ["alpha_linear", "feature_linear", "views_linears.0", "rgb_linear"]

@@ -959,21 +959,17 @@ class RowPlan:
         self.slot_ptr = self.source_ptr + 4 * ((self.pairs + 3) // 4 * 4)
         self.order_ptr = self.source_ptr
 
-    def _view(self, ptr, n):
-        at = (ptr - self.buf.data_ptr()) // 4
-        return self.buf[at:at + n]
-
     @property
     def offsets(self):
-        return self._view(self.offsets_ptr, self.n_groups + 1)
+        return self.buf.as_strided((self.n_groups + 1,), (1,))
 
     @property
     def source(self):
-        return self._view(self.source_ptr, self.pairs)
+        return self.buf.as_strided((self.pairs,), (1,), (self.source_ptr - self.offsets_ptr) // 4)
 
     @property
     def slot(self):
-        return self._view(self.slot_ptr, self.pairs).view(self.shape)
+        return self.buf.as_strided(self.shape, (self.k, 1)[:len(self.shape)], (self.slot_ptr - self.offsets_ptr) // 4)
 
     def sorted(self):
         """the plan of the DISPATCHED rows: n_rows * k of them, lying in group order already"""
@@ -1035,10 +1031,12 @@ def _row_weights(weights, plan):
 
 
 def _rows_2d(t, n, name, dev):
-    t = _rows_like(t, name, dev)
-    if t.dim() < 1 or t.shape[0] != n:
-        raise ValueError(f"{name}: {tuple(t.shape)} for a plan of {n} rows")
-    return t.contiguous(), math.prod(t.shape[1:])
+    if not (torch.is_tensor(t) and t.dtype in ROW_DTYPES and t.device == dev):
+        _rows_like(t, name, dev)
+    shape = t.shape
+    if len(shape) < 1 or shape[0] != n:
+        raise ValueError(f"{name}: {tuple(shape)} for a plan of {n} rows")
+    return t.contiguous(), shape[1] if len(shape) == 2 else math.prod(shape[1:])
 
 
 def dispatch_rows(x, plan, weights=None):
