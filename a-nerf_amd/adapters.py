@@ -15,12 +15,12 @@ Row types: float32, bfloat16, float16; sums are held in float32 and rounded once
 gradient is refused.
 """
 import math
+import threading
 import weakref
 
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
-from torch.utils.weak import WeakIdKeyDictionary
 
 from . import ops
 from .ops import RowPlan, SortedRows, route_rows  # noqa: F401
@@ -29,16 +29,16 @@ from .ops import RowPlan, SortedRows, route_rows  # noqa: F401
 # A leaf's gradient node belongs to the stream it was first used on, and lives as long as any graph that reaches the leaf.  While an
 # EAGER graph of a leaf is alive, a backward that is being captured makes autograd order the capturing stream against that other
 # stream -- which a capture does not allow, and the exception ends the process.  The calls below therefore know which of their graphs are
-# alive per leaf, and refuse such a backward with an exception that can be handled.
+# alive, and refuse such a backward with an exception that can be handled.
 class _Graph:
     """one call's graph: its leaves and the stream it was built on (alive while autograd holds the call's node)"""
     __slots__ = ("leaves", "stream", "__weakref__")
 
     def __init__(self, leaves):
-        self.leaves, self.stream = leaves, ops._stream().value
+        self.leaves, self.stream = leaves, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-_graphs = WeakIdKeyDictionary()     # leaf -> its living graphs
+_alive, _alive_lock = weakref.WeakSet(), threading.Lock()
 
 
 def _graph_of(*tensors):
@@ -46,11 +46,8 @@ def _graph_of(*tensors):
     if not leaves:
         return None
     graph = _Graph(leaves)
-    for t in leaves:
-        alive = _graphs.get(t)
-        if alive is None:
-            alive = _graphs[t] = weakref.WeakSet()
-        alive.add(graph)
+    with _alive_lock:
+        _alive.add(graph)
     return graph
 
 
@@ -61,10 +58,12 @@ def _capturing():
 def _check_capture(graph):
     if graph is None or not _capturing():
         return
-    for t in graph.leaves:
-        if any(other is not graph and other.stream != graph.stream for other in _graphs.get(t, ())):
-            raise RuntimeError("this backward is being captured while an eager graph of the same leaf tensor is alive (an output of an eager call that "
-                               "is still referenced): drop it before the capture")
+    mine = {id(t) for t in graph.leaves}
+    with _alive_lock:
+        others = list(_alive)
+    if any(other is not graph and other.stream != graph.stream and any(id(t) in mine for t in other.leaves) for other in others):
+        raise RuntimeError("this backward is being captured while an eager graph of the same leaf tensor is alive (an output of an eager call that "
+                           "is still referenced): drop it before the capture")
 
 
 def _once(backward):
