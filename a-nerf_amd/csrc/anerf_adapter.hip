@@ -4,7 +4,7 @@
 //     h[r] = s_i x[r] A_i^T,  u[r] = s_i g[r] B_i,  dx = g W + u A_i,  dA_i = sum_r u[r]^T x[r],  dB_i = sum_r g[r]^T h[r]
 // Rows are walked in the order of their adapter (positions p; order[p] = row, NULL = rows lie in that order already), adapter i
 // owning positions offsets[i] .. offsets[i+1]-1; the rows behind offsets[L] have no adapter.
-//   k_thin       h[p] = s_i x[order[p]] A_i^T: one workgroup a piece of 32 positions of one adapter
+//   k_thin       h[p] = s_i x[order[p]] A_i^T: one workgroup a piece of 16 or 32 positions of one adapter
 //   k_main       x W^T tile by tile; a tile starts with the low-rank term of the adapters whose positions it holds
 //   k_thin_grad  dA_i / dB_i as sums over pieces of an adapter's positions, k_thin_grad_sum adds the pieces in order
 //   k_few        up to 64 rows with an adapter index each, in any order
@@ -16,10 +16,12 @@
 namespace anerf {
 
 // ------------------------------------------------------------------------------------------------------------ h = s_i x A_i^T
-// HBM-bound on x.  The four waves split the contraction (every fourth 64-byte step), each holding all 32 rows x 16*NJ ranks of the
-// piece in MFMA accumulators, fed straight from memory: a row of A serves 32 rows of x, and nothing is read twice from HBM.
-// 65520 x 688 fp32, rank 8: 32 us, 5.6 TB/s; 8192 x 4096 bf16, 24 adapters of rank 32 (73 MB): 21 us.  Pieces of 16 rows read A twice as
-// often, 64 rows leave CUs idle at a few thousand rows.
+// HBM-bound on x.  The four waves split the contraction (every fourth 64-byte step), each holding all 16*MB rows x 16*NJ ranks of the
+// piece in MFMA accumulators, fed straight from memory: a row of A serves all rows of the piece, and nothing is read twice from HBM.
+// 65520 x 688 fp32, rank 8: 32 us, 5.6 TB/s; 8192 x 4096 bf16, 24 adapters of rank 32 (73 MB): 21 us where x was just
+// written, from HBM 33, with 16 rows a piece 35; 200 rows
+// x 4096 bf16: 13.7 us with 32 rows a piece, 10.2 with 16.  More waves a piece or deeper loads gain nothing: a few pieces are bound by
+// what one CU can load.
 // Kept as [position][Rp] fp32 (Rp = rank rounded up to 16, zeros behind the rank) for the gradient of B, and, for the 16-bit types, as what
 // k_main multiplies with: the nearest value hi and the rest lo, [hi of 16 ranks | lo of the same 16] per 16 ranks, which meet [B | B]
 // there -- h keeps 16 (bf16) or 21 (fp16) of its bits.  fp16's range does not hold every h: its rows are scaled first.
@@ -45,55 +47,55 @@ __device__ __forceinline__ int row_exponent(float big) {
   return big > 0.f && __builtin_isfinite(big) ? min(max(ilogbf(big), -100), 100) : 0;
 }
 
-constexpr int TH_ROWS = 32, TH_WAVES = 4, TH_DEPTH = 4;
+constexpr int TH_WAVES = 4, TH_DEPTH = 4;
 template <int V> struct Const { static constexpr int value = V; };
 template <bool C, typename A, typename B> struct Pick { typedef A T; };
 template <typename A, typename B> struct Pick<false, A, B> { typedef B T; };
 
-template <int DT, int NJ>
+template <int DT, int NJ, int MB>
 __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const int32_t* __restrict__ order,
                                                         const typename Elem<DT>::T* __restrict__ down, const int32_t* __restrict__ offsets,
                                                         int L, long long K, int R, int Rp, const float* __restrict__ scale_of, float scale,
                                                         float* __restrict__ h, typename Elem<DT>::T* __restrict__ split, float* __restrict__ factor) {
   typedef typename Elem<DT>::T E;
-  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
-  __shared__ f32x4 red[TH_WAVES][2 * NJ][64];
+  constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, TH_ROWS = 16 * MB;
+  __shared__ f32x4 red[TH_WAVES][MB * NJ][64];
   int a, p0, p1;
   if (!find_piece(offsets, L, TH_ROWS, blockIdx.x, a, p0, p1)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
   const int j0 = blockIdx.y * 16 * NJ;
   const float s_a = scale_of ? scale * scale_of[a] : scale;
   const E* A = down + (long long)a * R * K;
-  const E* xr[2];
+  const E* xr[MB];
   const E* ar[NJ];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
+  for (int m = 0; m < MB; ++m) {
     const int p = min(p0 + 16 * m + i, p1 - 1);      // rows behind the piece repeat its last one; their sums are not stored
     xr[m] = x + (long long)(order ? order[p] : p) * ldx;
   }
 #pragma unroll
   for (int n = 0; n < NJ; ++n) ar[n] = A + (long long)min(j0 + 16 * n + i, R - 1) * K;
-  f32x4 acc[2][NJ];
+  f32x4 acc[MB][NJ];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int n = 0; n < NJ; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   const long long steps = K / STEP;
   auto walk = [&](long long s0, auto depth) {       // `depth` steps of this wave, all their loads in front of the products
     constexpr int D = decltype(depth)::value;
-    u32x4 xv[D][2], av[D][NJ];
+    u32x4 xv[D][MB], av[D][NJ];
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const long long k = (s0 + d * TH_WAVES) * STEP + q * EPC;
 #pragma unroll
-      for (int m = 0; m < 2; ++m) xv[d][m] = load16(xr[m] + k);
+      for (int m = 0; m < MB; ++m) xv[d][m] = load16(xr[m] + k);
 #pragma unroll
       for (int n = 0; n < NJ; ++n) av[d][n] = load16(ar[n] + k);
     }
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < MB; ++m)
 #pragma unroll
         for (int n = 0; n < NJ; ++n)
 #pragma unroll
@@ -104,26 +106,26 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   for (; s < steps; s += TH_WAVES) walk(s, Const<1>());
   if (steps * STEP < K && wave == (int)(steps % TH_WAVES)) {
     const long long k = steps * STEP + q * EPC;
-    u32x4 xv[2], av[NJ];
+    u32x4 xv[MB], av[NJ];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) xv[m] = load_tail<DT>(xr[m], k, K);
+    for (int m = 0; m < MB; ++m) xv[m] = load_tail<DT>(xr[m], k, K);
 #pragma unroll
     for (int n = 0; n < NJ; ++n) av[n] = load_tail<DT>(ar[n], k, K);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int n = 0; n < NJ; ++n)
 #pragma unroll
         for (int e = 0; e < Elem<DT>::INSTR; ++e) acc[m][n] = Elem<DT>::mma(av[n], xv[m], acc[m][n], e);
   }
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int n = 0; n < NJ; ++n) red[wave][m * NJ + n][lane] = acc[m][n];
   __syncthreads();
   constexpr int LINE = 16 * NJ + 4;
   __shared__ float tile[TH_ROWS * LINE];            // the piece's h, row by row
-  for (int f = wave; f < 2 * NJ; f += TH_WAVES) {
+  for (int f = wave; f < MB * NJ; f += TH_WAVES) {
     f32x4 v = red[0][f][lane];
 #pragma unroll
     for (int w = 1; w < TH_WAVES; ++w) v += red[w][f][lane];
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   __syncthreads();
   // eight lanes a row, four ranks each and turn
   const int r = threadIdx.x >> 3, part = threadIdx.x & 7, p = p0 + r;
-  if (p >= p1) return;
+  if (r >= TH_ROWS || p >= p1) return;
   f32x4 v[(4 * NJ + 7) / 8];
   float big = 0.f;
 #pragma unroll
@@ -1146,7 +1148,8 @@ template <int DT>
 static int linear_t(const AnerfAdapterIO& A, long long ldw, void* ws, hipStream_t st) {
   typedef typename Elem<DT>::T E;
   const HLayout H = h_layout(A);
-  const long long pieces = pieces_bound(A.n_rows, A.n_adapters, TH_ROWS);
+  // pieces of 16 rows while there is at most one for a CU: what bounds few pieces is what one CU can load
+  const long long small = pieces_bound(A.n_rows, A.n_adapters, 16), pieces = small <= 256 ? small : pieces_bound(A.n_rows, A.n_adapters, 32);
   const int Rp = H.Rp;
   float* h = reinterpret_cast<float*>(A.h);
   E* split = reinterpret_cast<E*>(static_cast<char*>(A.h) + H.split);
@@ -1155,9 +1158,9 @@ static int linear_t(const AnerfAdapterIO& A, long long ldw, void* ws, hipStream_
     kernel<<<dim3((unsigned)pieces, parts), TH_WAVES * 64, 0, st>>>(static_cast<const E*>(A.x), A.x_stride, A.order, static_cast<const E*>(A.down), A.offsets,
                                                                   A.n_adapters, A.n_in, A.rank, Rp, A.scale_of, A.scale, h, split, factor);
   };
-  if (Rp <= 16) thin(k_thin<DT, 1>, 1);
-  else if (Rp <= 32) thin(k_thin<DT, 2>, 1);
-  else thin(k_thin<DT, 4>, (Rp + 63) / 64);
+  if (Rp <= 16) small <= 256 ? thin(k_thin<DT, 1, 1>, 1) : thin(k_thin<DT, 1, 2>, 1);
+  else if (Rp <= 32) small <= 256 ? thin(k_thin<DT, 2, 1>, 1) : thin(k_thin<DT, 2, 2>, 1);
+  else small <= 256 ? thin(k_thin<DT, 4, 1>, (Rp + 63) / 64) : thin(k_thin<DT, 4, 2>, (Rp + 63) / 64);
   if constexpr (DT == ANERF_F16) {
     if (A.y && Rp > 64) k_split_rows<<<(unsigned)((A.n_rows + 15) / 16), 256, 0, st>>>(h, A.offsets + A.n_adapters, Rp, split, factor);
   }
