@@ -485,20 +485,36 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 
   // ---- bias, rounding, store.  A lane holds four outputs of its row in each block.  fp32: 16 bytes, stored as they are
   if constexpr (F32) {
-    const float* bias = static_cast<const float*>(P.bias);
+    const float* bias = P.splits > 1 ? nullptr : static_cast<const float*>(P.bias);
+    f32x4 add[NI];
+    long long row[MI];
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const long long col = n0 + wn * TN + BS * n + 4 * q;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[n][e] = 0.f;
+      if (bias && col + 4 <= P.N) {
+        __builtin_memcpy(&add[n], bias + col, 16);
+      } else if (bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < P.N) add[n][e] = bias[col + e];
+      }
+    }
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
       const long long p = m0 + wm * TM + BS * m + i;
-      if (p >= P.M) continue;
-      const long long row = P.order ? (long long)P.order[p] : p;
-      float* yr = P.splits > 1 ? P.part + (part * P.M + row) * P.N : static_cast<float*>(P.y) + row * P.N;
+      row[m] = p < P.M ? (P.order ? (long long)P.order[p] : p) : -1;
+    }
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      if (row[m] < 0) continue;
+      float* yr = P.splits > 1 ? P.part + (part * P.M + row[m]) * P.N : static_cast<float*>(P.y) + row[m] * P.N;
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         const long long col = n0 + wn * TN + BS * n + 4 * q;
         f32x4 v = acc[m][n] + sum[m][n];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (bias && P.splits == 1 && col + e < P.N) v[e] += bias[col + e];
+        if (bias) v += add[n];
         if (col + 4 <= P.N) {
           store16(yr + col, __builtin_bit_cast(u32x4, v));
         } else {
@@ -520,14 +536,21 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     char* mine = reinterpret_cast<char*>(lds) + wave * (ROWS * LINE);
     const long long cw = n0 + wn * TN;
     const int r0 = lane / LPR, c = lane % LPR * PER;
-    float add[NI][4];
+    typedef E bias4 __attribute__((ext_vector_type(4)));
+    bias4 add[NI];
 #pragma unroll
-    for (int n = 0; n < NI; ++n)
+    for (int n = 0; n < NI; ++n) {
+      const long long col = cw + BS * n + 4 * q;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const long long col = cw + BS * n + 4 * q + e;
-        add[n][e] = bias && col < P.N ? (float)bias[col] : 0.f;
+      for (int e = 0; e < 4; ++e) add[n][e] = (E)0.f;
+      if (bias && col + 4 <= P.N) {
+        __builtin_memcpy(&add[n], bias + col, sizeof(bias4));
+      } else if (bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < P.N) add[n][e] = bias[col + e];
       }
+    }
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const long long pw = m0 + wm * TM + g * ROWS;
@@ -545,7 +568,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float v = acc[g * MG + m][n][e];
-            o[e] = (S)(bias ? v + add[n][e] : v);
+            o[e] = (S)(bias ? v + (float)add[n][e] : v);
           }
           *reinterpret_cast<four*>(mine + (BS * m + i) * LINE + (BS * n + 4 * q) * (int)sizeof(S)) = o;
         }
@@ -596,8 +619,12 @@ __global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ par
       v += w;
     }
     out4 o;
+    long long c = bias ? e % N : 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = (E)(bias ? v[k] + (float)bias[(e + k) % N] : v[k]);
+    for (int k = 0; k < 4; ++k) {
+      o[k] = (E)(bias ? v[k] + (float)bias[c] : v[k]);
+      c = c + 1 == N ? 0 : c + 1;
+    }
     __builtin_memcpy(y + e, &o, sizeof(o));
   } else {
     for (int k = 0; e + k < all; ++k) {
