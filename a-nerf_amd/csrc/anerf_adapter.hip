@@ -56,7 +56,8 @@ template <int DT, int NJ, int MB>
 __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>::T* __restrict__ x, long long ldx, const int32_t* __restrict__ order,
                                                         const typename Elem<DT>::T* __restrict__ down, const int32_t* __restrict__ offsets,
                                                         int L, long long K, int R, int Rp, const float* __restrict__ scale_of, float scale,
-                                                        float* __restrict__ h, typename Elem<DT>::T* __restrict__ split, float* __restrict__ factor) {
+                                                        float* __restrict__ h, typename Elem<DT>::T* __restrict__ split, float* __restrict__ factor,
+                                                        int32_t* __restrict__ owner) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, TH_ROWS = 16 * MB;
   __shared__ f32x4 red[TH_WAVES][MB * NJ][64];
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   // eight lanes a row, four ranks each and turn
   const int r = threadIdx.x >> 3, part = threadIdx.x & 7, p = p0 + r;
   if (r >= TH_ROWS || p >= p1) return;
+  if (part == 0 && j0 == 0) owner[p] = a;
   f32x4 v[(4 * NJ + 7) / 8];
   float big = 0.f;
 #pragma unroll
@@ -190,7 +192,8 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 // at any alignment.
 // Few tiles: `splits` workgroups share one, each with a contiguous part of the stages, and k_sum_parts adds their fp32 tiles.
 // The low-rank term comes first, behind the first stage's loads: for every adapter with positions in the tile h B_i^T is added to the
-// blocks of its rows; a block that two adapters share takes it by row (a NaN in one adapter stays with its rows).
+// blocks of its rows; a block that two adapters share takes it by row (a NaN in one adapter stays with its rows).  Waves with rows of many
+// adapters take it row by row.
 // fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set, so that no chain of
 // additions is longer than 8 * FOLD + K / (32 * FOLD).
 // Bound by the matrix units.  bf16, 8192 x 4096 -> 4096 with 24 adapters of rank 32: 245 us, 1140 TFLOP/s (without adapters, once the clocks
@@ -201,6 +204,8 @@ struct MainArgs {
   const int32_t *offsets, *order;
   const void* h;               // operand form of h: [M][Rp] fp32, [M][2 Rp] 16-bit
   const float* factor;         // fp16: power of two of every row of h
+  const float* h32;            // [M][Rp]
+  const int32_t* owner;        // the positions' adapters
   void* y;
   float* part;                 // splits > 1: fp32 [splits][M][N]
   long long ldx, ldw, K, N;
@@ -322,8 +327,84 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     const int last_col = (int)(P.N - 1 - c0 < TN ? P.N - 1 - c0 : TN);
     const int chunks = P.Rp / 16, row_bytes = P.Rp * 4;        // (two 16-bit values or one fp32 a rank)
     const char* hw = static_cast<const char*>(P.h) + (long long)w0 * row_bytes + 16 * q;
-    // the adapters 64 at a time; those that own positions of the tile
-    for (int b0 = 0; b0 < P.L; b0 += 64) {
+    int b0 = 0;                                                // of 64 adapters looked at together
+    if (P.L > 64) {                                            // first those that hold the tile's first position
+      const unsigned long long at = __ballot(64 * lane < P.L && P.offsets[min(64 * lane, P.L)] <= t0);
+      b0 = 64 * (63 - __builtin_clzll(at));
+    }
+    // A wave whose rows are of many adapters (64 rows may be of as many) would take them one after the other, 0.3 us each and 16 ranks.  It
+    // takes its rows' dots of `rank` fp32 values instead, whose loads do not wait for one another -- where B's rows are short enough for the
+    // first cache to serve them (bf16, rank 16, 1024 x 1024, 48 rows of 64 adapters: 26 -> 17 us; 256 rows x 2048 x 2048 of 500: 50 -> 36; with
+    // rank 64 the dots took twice the time).
+    bool one_by_one = false;
+    if constexpr (MI <= 4) {
+      constexpr int many = 3 * MI / 2 * NI;
+      if (P.R * (int)sizeof(E) <= 64) {
+        int count = 0;
+        for (int b = b0; b < P.L && count <= many; b += 64) {
+          const int ab = b + lane;
+          const int lo = ab < P.L ? P.offsets[ab] : 0, hi = ab < P.L ? P.offsets[ab + 1] : 0;
+          count += __popcll(__ballot(hi > lo && hi > w0 && lo < min(w0 + TM, t1)));
+          if (__builtin_amdgcn_readlane(hi, 63) >= min(w0 + TM, t1)) break;
+        }
+        one_by_one = count > many;
+      }
+      if (one_by_one) {
+        typedef E vec __attribute__((ext_vector_type(EPC)));
+#pragma unroll
+        for (int m0 = 0; m0 < MI; m0 += 2) {                   // two rows of a lane at a time
+          const E* br[2];
+          const float* hr[2];
+          bool has[2];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const int p = w0 + BS * (m0 + m) + i;
+            has[m] = p < kept;
+            br[m] = static_cast<const E*>(P.up) + (has[m] ? (long long)P.owner[p] * P.N : 0) * P.R;
+            hr[m] = P.h32 + (long long)(has[m] ? p : t0) * P.Rp;
+          }
+#pragma unroll
+          for (int n = 0; n < NI; ++n) {
+            long long at[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const long long col = c0 + BS * n + 4 * q + e;
+              at[e] = (col < P.N ? col : P.N - 1) * P.R;
+            }
+            f32x4 dot[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            int j = 0;
+            for (; j + EPC <= P.R; j += EPC) {
+              vec bv[2][4];
+              f32x4 hv[2][EPC / 4];
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bv[m][e] = __builtin_bit_cast(vec, load16(br[m] + at[e] + j));
+#pragma unroll
+                for (int k = 0; k < EPC / 4; ++k) hv[m][k] = __builtin_bit_cast(f32x4, load16(hr[m] + j + 4 * k));
+              }
+#pragma unroll
+              for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                  for (int k = 0; k < EPC; ++k) dot[m][e] = fmaf(hv[m][k / 4][k % 4], (float)bv[m][e][k], dot[m][e]);
+            }
+            for (; j < P.R; ++j)
+#pragma unroll
+              for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dot[m][e] = fmaf(hr[m][j], (float)br[m][at[e] + j], dot[m][e]);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m0 + m][n][e] = has[m] ? dot[m][e] : 0.f;
+          }
+        }
+      }
+    }
+    // the adapters that own positions of the tile, one after the other
+    for (; !one_by_one && b0 < P.L; b0 += 64) {
       const int ab = b0 + lane;
       const int lo = ab < P.L ? P.offsets[ab] : 0, hi = ab < P.L ? P.offsets[ab + 1] : 0;
       unsigned long long owners = __ballot(hi > lo && hi > t0 && lo < t1);
@@ -367,7 +448,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       }
       if (__builtin_amdgcn_readlane(hi, 63) >= t1) break;
     }
-    if constexpr (DT == ANERF_F16) {
+    if (DT == ANERF_F16 && !one_by_one) {
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
         const int p = w0 + BS * m + i;
@@ -1139,18 +1220,20 @@ static int launch_main(const MainArgs& P, hipStream_t st) {
   return run64();
 }
 
-// what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][2 Rp] (16-bit types) | factor [n_rows] (fp16); byte offsets
+// what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][2 Rp] (16-bit types) | factor [n_rows] (fp16) | the positions'
+// adapters [n_rows]; byte offsets
 struct HLayout {
   int Rp;
-  long long split, factor, bytes;
+  long long split, factor, owner, bytes;
 };
 static HLayout h_layout(const AnerfAdapterIO& A) {
   HLayout H;
   H.Rp = (A.rank + 15) / 16 * 16;
-  const long long part = A.n_rows * H.Rp * 4;
+  const long long part = A.n_rows * H.Rp * 4, line = (A.n_rows + 3) / 4 * 16;
   H.split = part;
   H.factor = A.dtype == ANERF_F32 ? part : 2 * part;
-  H.bytes = H.factor + (A.dtype == ANERF_F16 ? (A.n_rows + 3) / 4 * 16 : 0);
+  H.owner = H.factor + (A.dtype == ANERF_F16 ? line : 0);
+  H.bytes = H.owner + line;
   return H;
 }
 long long adapter_h_bytes(const AnerfAdapterIO& A) { return h_layout(A).bytes; }
@@ -1181,9 +1264,10 @@ static int linear_t(const AnerfAdapterIO& A, long long ldw, void* ws, hipStream_
   float* h = reinterpret_cast<float*>(A.h);
   E* split = reinterpret_cast<E*>(static_cast<char*>(A.h) + H.split);
   float* factor = reinterpret_cast<float*>(static_cast<char*>(A.h) + H.factor);
+  int32_t* owner = reinterpret_cast<int32_t*>(static_cast<char*>(A.h) + H.owner);
   auto thin = [&](auto kernel, int parts) {
     kernel<<<dim3((unsigned)pieces, parts), TH_WAVES * 64, 0, st>>>(static_cast<const E*>(A.x), A.x_stride, A.order, static_cast<const E*>(A.down), A.offsets,
-                                                                  A.n_adapters, A.n_in, A.rank, Rp, A.scale_of, A.scale, h, split, factor);
+                                                                  A.n_adapters, A.n_in, A.rank, Rp, A.scale_of, A.scale, h, split, factor, owner);
   };
   if (Rp <= 16) small <= 256 ? thin(k_thin<DT, 1, 1>, 1) : thin(k_thin<DT, 1, 2>, 1);
   else if (Rp <= 32) small <= 256 ? thin(k_thin<DT, 2, 1>, 1) : thin(k_thin<DT, 2, 2>, 1);
@@ -1195,7 +1279,7 @@ static int linear_t(const AnerfAdapterIO& A, long long ldw, void* ws, hipStream_
   if (rc || !A.y) return rc;       // (the gradient of A alone needs h only)
   const void* operand = split;
   if constexpr (DT == ANERF_F32) operand = h;
-  MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, A.y, static_cast<float*>(ws), A.x_stride, ldw, A.n_in, A.n_out,
+  MainArgs P = {A.x, A.weight, A.bias, A.up, A.offsets, A.order, operand, factor, h, owner, A.y, static_cast<float*>(ws), A.x_stride, ldw, A.n_in, A.n_out,
                 A.n_rows, A.n_adapters, A.rank, Rp, split_of(DT, A.n_rows, A.n_in, A.n_out)};
   if (const long long Kp = padded_width(A, ldw)) {
     char* w = static_cast<char*>(ws);

@@ -908,3 +908,23 @@ def test_an_adapted_render_and_its_backward_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), r
+
+
+@pytest.mark.parametrize("M,L,R,dt", [(200, 64, 8, "bf16"), (200, 150, 16, "fp32"), (333, 700, 5, "fp16"), (130, 1024, 32, "bf16"), (129, 1000, 1, "fp32"), (2100, 900, 16, "fp16"),
+                                      (200, 64, 40, "bf16")])
+def test_rows_of_many_adapters(M, L, R, dt):
+    """tiles that hold about as many adapters as rows, the first and the last among them; NaN and infinity stay with their rows"""
+    K, N = 72, 200
+    d = on_the_device(M, K, N, L, R, DT[dt], M + L)
+    d["idx"][:3], d["idx"][-2:] = L - 1, 0
+    rows = torch.arange(M, device="cuda")
+    y, yb = oracle_rows(d, 0.5, DT[dt], rows)
+    run = lambda: ad.adapter_linear(d["x"], d["weight"], d["down"], d["up"], ad.route_rows(d["idx"], L), bias=d["bias"], scale=0.5)
+    plain = run()
+    within(plain, y, yb, DT[dt])
+    bad = d["idx"].unique()[1:].tolist()[::5]                       # a fifth of the adapters in use
+    for k, a in enumerate(bad):
+        d["up" if k % 2 else "down"][a] = float("nan") if k % 3 else float("inf")
+    hit = torch.isin(d["idx"], torch.tensor(bad, device="cuda"))
+    got = run()
+    assert torch.equal(got[~hit], plain[~hit]) and not got[hit].isfinite().all(1).any()
