@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(RT_THREADS) k_route_count(const I* __restrict_
 // Positions.  A wave owns a contiguous part of the workgroup's chunk: its counters start at (start of the group) + (pairs of the
 // group in earlier workgroups) + (in earlier waves), and it walks its part 64 pairs at a time in order.  hist == NULL: one
 // workgroup holds all pairs.  Latency-bound: two passes over the indices, everything else is in LDS.  66 pairs: 3 us; 65520 pairs of 16
-// groups: count 4.9 + place 5.2 us, of 128 groups place 9.5 us (the prefix over the workgroups' counts grows with groups x workgroups).
+// groups: count 4.9 + place 5.2 us, of 128 groups place 8.1 us (the prefix over the workgroups' counts grows with groups x workgroups).
 template <typename I>
 __global__ void __launch_bounds__(RT_THREADS) k_route_place(const I* __restrict__ idx, long long n, int G, int chunk, int bits,
                                                             const int32_t* __restrict__ hist, int32_t* __restrict__ offsets,
@@ -74,10 +74,15 @@ __global__ void __launch_bounds__(RT_THREADS) k_route_place(const I* __restrict_
     const int nb = gridDim.x, parts = RT_THREADS / gp, my = tid / gp;
     for (int g = tid % gp; g < W; g += gp) {
       int all = 0, prev = 0;
-      for (int b = my; b < nb; b += parts) {
-        const int v = hist[(long long)b * W + g];
-        all += v;
-        prev += b < (int)blockIdx.x ? v : 0;
+      for (int b0 = my; b0 < nb; b0 += 8 * parts) {      // eight loads at a time (one after the other: 9.4 us with 128 groups)
+        int v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = b0 + u * parts < nb ? hist[(long long)(b0 + u * parts) * W + g] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          all += v[u];
+          prev += b0 + u * parts < (int)blockIdx.x ? v[u] : 0;
+        }
       }
       if (all) atomicAdd(&total[g], all);
       if (prev) atomicAdd(&before[g], prev);
