@@ -303,10 +303,10 @@ def encode_rows(net, kw, z):
     (encode_inputs, raycasters.py:476-577): what the training forward saves for its backward, columns put back, --freq_schedule factors
     and the frame-code column applied.  No gradient to the poses."""
     cfg, rays, dev = kw["cfg"], kw["ray_batch"], kw["ray_batch"].device
-    skts = ops._f32c(ops.first_row(kw["skts"]), "skts")
     n, s = z.shape
-    if skts.shape[0] not in (1, n) or tuple(skts.shape[1:]) != (cfg.n_joints, 4, 4):
-        raise ValueError(f"skts {tuple(skts.shape)} for {n} rays: expected [1 or {n}, {cfg.n_joints}, 4, 4]")
+    if kw["skts"].shape[0] not in (1, n) or tuple(kw["skts"].shape[1:]) != (cfg.n_joints, 4, 4):
+        raise ValueError(f"skts {tuple(kw['skts'].shape)} for {n} rays: expected [1 or {n}, {cfg.n_joints}, 4, 4]")
+    skts = ops._f32c(ops.first_row(kw["skts"]), "skts")
     codes = None if not net.use_framecode else net.framecodes.codes.weight.detach()
     cam = None if codes is None else kw["cam_idx"].reshape(-1).expand(n).contiguous()
     out = torch.empty(n * s, cfg.x_width, dtype=torch.float32, device=dev)
@@ -353,6 +353,8 @@ def render_rays_adapted(caster, kw, subject_idxs):
         raise NotImplementedError("subject_idxs with sample-point offsets (ray_noise_std > 0)")
     if not torch.is_tensor(subject_idxs) or subject_idxs.dtype not in (torch.int32, torch.int64) or subject_idxs.numel() not in (1, n):
         raise ValueError(f"subject_idxs: one int32 / int64 subject per ray, got {getattr(subject_idxs, 'shape', type(subject_idxs))} for {n} rays")
+    if caster.network.use_framecode and kw["cam_idx"] is None:
+        raise ValueError("subject_idxs: a network with frame codes needs cams")
     subject = subject_idxs.reshape(-1).to(kw["ray_batch"].device)
     kw = dict(kw, cyls=kw["cyls"].expand(n, 5))
 

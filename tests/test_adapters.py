@@ -928,3 +928,37 @@ def test_rows_of_many_adapters(M, L, R, dt):
     hit = torch.isin(d["idx"], torch.tensor(bad, device="cuda"))
     got = run()
     assert torch.equal(got[~hit], plain[~hit]) and not got[hit].isfinite().all(1).any()
+
+
+def test_backward_twice_and_no_gradient_of_a_gradient():
+    d = on_the_device(70, 40, 24, 3, 4, torch.float32, 6)
+    x, A, B = (d[k].requires_grad_() for k in ("x", "down", "up"))
+    w = torch.rand(70, 1, device="cuda").requires_grad_()
+    plan = ad.route_rows(d["idx"], 3)
+    y = ad.combine_rows(ad.adapter_linear(ad.dispatch_rows(x, plan), d["weight"], A, B, plan.sorted()), plan, w)
+    first = torch.autograd.grad(y, [x, A, B, w], d["g"], retain_graph=True)
+    again = torch.autograd.grad(y, [x, A, B, w], d["g"], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError):
+        again[0].sum().backward()
+    (dw,) = torch.autograd.grad(ad.combine_rows(ad.dispatch_rows(x.detach(), plan), plan, w), w, torch.ones(70, 40, device="cuda"))
+    kept = (d["idx"] >= 0).float()
+    # a sum of 40 values in fp32
+    assert float((dw[:, 0].double() - x.detach().double().sum(1) * kept).abs().max()) <= 48 * STEP * float(x.detach().abs().sum(1).max())
+
+
+def test_frame_codes_without_cams_are_refused():
+    raycaster = importlib.import_module("a-nerf_amd.raycaster")
+    mk = lambda: networks.NeRF(D=8, W=256, input_ch=360, input_ch_bones=72, input_ch_views=648, use_viewdirs=True, use_framecode=True, framecode_ch=16, n_framecodes=4)
+    ck = dict(cutoff=True, cutoff_dist=0.5, cutoff_inputs=True, cutoff_dim=24)
+    ev, eb, ed = (networks.get_embedder(7, 0, 24, cutoff_kwargs=dict(ck))[0], networks.get_embedder(0, 0, 72)[0],
+                  networks.get_embedder(4, 0, 72, cutoff_kwargs=dict(ck, dist_inputs=True))[0])
+    caster = raycaster.RayCaster(mk(), ev, eb, ed, network_fine=mk()).cuda().requires_grad_(False)
+    caster.set_adapters(ad.NetAdapters(caster.network, 2), ad.NetAdapters(caster.network_fine, 2))
+    args = dict(N_samples=8, kp_batch=torch.zeros(1, 24, 3, device="cuda"), cyls=torch.ones(4, 5, device="cuda"), N_importance=8,
+                subject_idxs=torch.zeros(4, dtype=torch.long, device="cuda"))
+    one = torch.eye(4, device="cuda").expand(1, 24, 4, 4)
+    with pytest.raises(ValueError, match="cams"):
+        caster(torch.rand(4, 11, device="cuda"), skts=one, **args)
+    with pytest.raises(ValueError, match="skts"):                                    # poses of two rays for four
+        caster(torch.rand(4, 11, device="cuda"), skts=one.expand(2, 24, 4, 4), cams=torch.zeros(4, device="cuda"), **args)
