@@ -122,3 +122,13 @@ def test_adapters_leave_the_networks_state_dict_alone():
     assert torch.equal(b.down("views_linears.0"), a.down("views_linears.0"))
     with pytest.raises(ValueError):
         networks.NeRF(input_ch=360, input_ch_bones=72, input_ch_views=648, use_viewdirs=True)(torch.zeros(2, 1080), subject_idxs=torch.zeros(2))
+
+
+def test_negative_row_strides_are_refused():
+    lib = _lib.load()
+    io = _io(x_stride=-64)
+    assert lib.anerf_adapter_workspace_size(ctypes.byref(io)) == E_SHAPE and lib.anerf_adapter_linear(ctypes.byref(io), P(9), 1 << 30, None) == E_SHAPE
+    assert lib.anerf_adapter_linear_few(ctypes.byref(io), P(10), 1, None) == E_SHAPE
+    g = _lib.AnerfAdapterGradIO()
+    g.g, g.g_stride, g.dx = P(11).value, -32, P(12).value
+    assert lib.anerf_adapter_backward(ctypes.byref(_io()), ctypes.byref(g), P(9), 1 << 30, None) == E_SHAPE
