@@ -206,7 +206,7 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
             raise TypeError(f"adapter_linear: adapter indices must be int32 / int64, got {rows.dtype}")
         few = M <= ops._lib.FEW_ROWS and not grads      # a decoding step: no plan, W streams through once
         rows = rows if rows.ndim == 1 else rows.reshape(-1)
-        rows = rows.contiguous() if few else route_rows(rows, L)
+        rows = rows.contiguous() if few else ops._route_rows(rows, M, 1, L)
     elif not isinstance(rows, (RowPlan, SortedRows)):
         raise TypeError(f"adapter_linear: rows must be indices, a RowPlan or its sorted(), got {type(rows).__name__}")
     if flat.stride(1) != 1 or flat.stride(0) < K:
@@ -223,7 +223,7 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
     if grads:
         y = _AdapterFn.apply(flat, down_, up_, weight, bias, rows, scale, scale_of, _graph_of(x, down, up))
     else:
-        y = ops._adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of)[0]
+        y = ops._adapter_linear(flat, weight, down_, up_, rows, bias, scale, scale_of, keep_h=False)[0]
     return y if x.ndim == 2 else y.reshape(lead + (N,))
 
 

@@ -1007,6 +1007,10 @@ def route_rows(groups, n_groups):
     n_groups = int(n_groups)
     if not 1 <= n_groups <= _lib.MAX_GROUPS:
         raise ValueError(f"route_rows: n_groups must be 1 .. {_lib.MAX_GROUPS}, got {n_groups}")
+    return _route_rows(groups, T, k, n_groups)
+
+
+def _route_rows(groups, T, k, n_groups):
     groups = groups.contiguous()
     n, lib = T * k, _lib.load()
     need = lib.anerf_route_rows_workspace_size(n, n_groups)
@@ -1136,15 +1140,18 @@ def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, 
     return _adapter_backward(g, x, weight, down, up, rows, h, scale, scale_of, want_dx, want_ddown, want_dup)
 
 
-def _adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=None):
+def _adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0, scale_of=None, keep_h=True):
     io, lib, dev = _adapter_io(x, weight, down, up, rows, bias, scale, scale_of), _lib.load(), x.device
     ref = C.byref(io)
     y = torch.empty(x.shape[0], weight.shape[0], dtype=x.dtype, device=dev)
-    h, _ = _workspace(lib.anerf_adapter_h_size, "anerf_adapter_h_size", dev, ref)
+    nh, need = lib.anerf_adapter_h_size(ref), lib.anerf_adapter_workspace_size(ref)
+    if nh < 0 or need < 0:
+        _lib.check(int(min(nh, need)), "anerf_adapter_h_size")
+    at = (nh + 15) // 16 * 16                                   # h alone where it is kept, else one buffer for both
+    h = torch.empty((nh if keep_h or need == 0 else at + need) // 4, dtype=torch.float32, device=dev)
+    ws = None if need == 0 else torch.empty(need // 4, dtype=torch.float32, device=dev) if keep_h else h
     io.y, io.h = y.data_ptr(), h.data_ptr()
-    need = lib.anerf_adapter_workspace_size(ref)
-    ws = torch.empty(need // 4, dtype=torch.float32, device=dev) if need > 0 else None
-    _launch(dev, lib.anerf_adapter_linear, "anerf_adapter_linear", ref, _ptr(ws), need)
+    _launch(dev, lib.anerf_adapter_linear, "anerf_adapter_linear", ref, None if ws is None else ws.data_ptr() + (0 if keep_h else at), need)
     return y, h
 
 
