@@ -62,13 +62,19 @@ class RayCaster(nn.Module):
 
     def set_adapters(self, adapters, adapters_fine=None):
         """adapters.NetAdapters of the coarse and of the fine network (None: detach both): render_rays(subject_idxs=...) then gives every ray
-        its subject's adapter.  They are not part of this module's parameters or checkpoint: save and step them by themselves."""
+        its subject's adapter.  They are not part of this module's parameters or checkpoint: save and step them by themselves.  Their
+        gradients are averaged over the ranks, and counted in the gradient norm, with this module's (step_parameters)."""
         if adapters is not None and self.network_fine is not None and self.network_fine is not self.network and adapters_fine is None:
             raise ValueError("set_adapters: this caster has a fine network, which needs adapters of its own")
         self.network.set_adapters(adapters)
         if self.network_fine is not None and self.network_fine is not self.network:
             self.network_fine.set_adapters(adapters_fine if adapters is not None else None)
         return self
+
+    def step_parameters(self):
+        """everything a training step through this caster gives gradients to: its own parameters and the attached adapters', each once"""
+        attached = [net.adapters() for net in (self.network, self.network_fine) if net is not None and net.adapters() is not None]
+        return list({id(p): p for m in [self, *attached] for p in m.parameters()}.values())
 
     @torch.no_grad()
     def forward_eval(self, *args, **kwargs):
@@ -339,12 +345,19 @@ class RayParallel(nn.Module):
         return self.module(*args, **kwargs)
 
     def sync_gradients(self, group=None):
-        """Average the gradients of every trainable parameter over the ranks with ONE all-reduce of a flat fp32 bucket
-        (parallel.GradBucket); call after loss.backward().  No-op in a single process."""
-        if getattr(self, "_bucket", None) is None:
+        """Average the gradients of every trainable parameter -- the caster's and its adapters' -- over the ranks with ONE all-reduce of
+        a flat fp32 bucket (parallel.GradBucket); call after loss.backward().  No-op in a single process."""
+        params = [p for p in self.step_parameters() if p.requires_grad]
+        bucket = getattr(self, "_bucket", None)
+        # (adapters may be attached or detached, parameters frozen, between two steps)
+        if bucket is None or len(bucket.params) != len(params) or any(a is not b for a, b in zip(bucket.params, params)):
             from .parallel import GradBucket
-            self._bucket = GradBucket([p for p in self.module.parameters() if p.requires_grad])
-        return self._bucket.all_reduce_mean(group)
+            bucket = self._bucket = GradBucket(params)
+        return bucket.all_reduce_mean(group)
+
+    def step_parameters(self):
+        of = getattr(self.module, "step_parameters", None)
+        return of() if of is not None else list(self.module.parameters())
 
 
 def get_grad_vars(args, ray_caster):

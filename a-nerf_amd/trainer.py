@@ -43,8 +43,10 @@ def decay_optimizer_lrate(lrate, lrate_decay, decay_rate, optimizer, global_step
 
 @torch.no_grad()
 def get_gradnorm(module):
-    """core/trainer.py:192-203 without its per-tensor `.item()`: (total_norm, avg_norm) as device scalars"""
-    sq = [p.grad.detach().float().pow(2).sum() for p in module.parameters() if p.grad is not None]
+    """core/trainer.py:192-203 without its per-tensor `.item()`: (total_norm, avg_norm) as device scalars.  A caster's adapters count with
+    its own parameters."""
+    of = getattr(module, "step_parameters", module.parameters)
+    sq = [p.grad.detach().float().pow(2).sum() for p in of() if p.grad is not None]
     if not sq:
         z = torch.zeros(())
         return z, z
