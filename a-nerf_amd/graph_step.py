@@ -20,7 +20,9 @@ Contract of `step_fn(i)` (the caller's iteration; i = the reference's iteration 
   * no host read of device data (`.item()`, `.cpu()`), no data-dependent host control flow;
   * the optimiser is a `FusedAdam` stepped with `i=i`; groups with `step_every > 1` (the pose cadence, trainer.py:476-478)
     get one graph per set of due groups;
-  * it returns a dict of tensors (loss, statistics): they live in the graph's pool and hold the last replay's values.
+  * it returns a dict of tensors (loss, statistics): they live in the graph's pool and hold the last replay's values.  step() hands
+    them out without their autograd graphs, eager iterations included; graphs of the same leaves that the caller builds and keeps
+    elsewhere must be dropped before a variant is captured.
 Not capturable here: `--freq_schedule` (its band factors are re-uploaded per iteration) -- `step()` falls back to the eager call
 for it, loudly once.
 
@@ -116,6 +118,19 @@ def _clear_sticky_hip_error():
 def ops_force_collectives():
     import os
     return os.environ.get("ANERF_FORCE_COLLECTIVES") == "1"
+
+
+def _values(out):
+    """the tensors of an iteration's results without their autograd graphs.  A caller that keeps the last result (a loss to print) would
+    keep the iteration's graph alive with it, and the gradient nodes of its leaves on the stream they were made on; a backward captured
+    beside those has to order the capturing stream against that other stream, which ends the process."""
+    if torch.is_tensor(out):
+        return out.detach()
+    if isinstance(out, dict):
+        return {k: _values(v) for k, v in out.items()}
+    if isinstance(out, (list, tuple)) and not hasattr(out, "_fields"):
+        return type(out)(_values(v) for v in out)
+    return out
 
 
 class StaticBatch:
@@ -237,7 +252,7 @@ class GraphedTrainStep:
             with ops.step_block(self.block):
                 ctx.__enter__()
                 entered = True
-                out = self.step_fn(i)
+                out = _values(self.step_fn(i))
                 ctx.__exit__(None, None, None)
                 entered = False
         except BaseException:
@@ -357,7 +372,7 @@ class GraphedTrainStep:
                 warnings.warn(f"GraphedTrainStep: running eagerly ({why})")
         if why is not None:
             self.eager_calls += 1
-            return self.step_fn(i)
+            return _values(self.step_fn(i))
         if self.block is None:
             self.block = ops.StepBlock(next(iter(self.opt.params)).device)
         due = tuple(self.opt._due(i)) if due is None else tuple(due)
@@ -366,18 +381,18 @@ class GraphedTrainStep:
         if hit is None:
             if gk in self.eager_only:
                 self.eager_calls += 1
-                return self.step_fn(i)
+                return _values(self.step_fn(i))
             if self.warm_each_key and gk not in self.warmed:
                 # first sight of this variant: its code path runs eagerly once (lazy one-off work must not fall inside a capture)
                 self.warmed.add(gk)
                 self.eager_calls += 1
-                return self.step_fn(i)
+                return _values(self.step_fn(i))
             try:
                 hit = self.graphs[gk] = self._capture(i, due)
             except Exception as e:
                 self._mark_eager_only(gk, e)
                 self.eager_calls += 1
-                return self.step_fn(i)
+                return _values(self.step_fn(i))
         g, out, fills = hit
         self._fill_block(i, due)
         self.block.write()
