@@ -362,6 +362,9 @@ class PoseOptLayer(nn.Module):
         if idxs is None:
             idxs = np.arange(len(self.pelvis))
         idxs = np.atleast_1d(np.asarray(idxs.cpu() if torch.is_tensor(idxs) else idxs))
+        # the last call's graph goes before this one's is built: kept through it, its gradient nodes (and the stream they were made on)
+        # would be the new graph's too, and a captured backward of a layer that is not attached would leave the capturing stream
+        self.last_unique = None
         if self.kp_map is None and len(self.rest_pose) == 1 and self.pelvis.is_cuda and getattr(self, "fused_batch", True):
             # single-view layer with one rest pose (surreal / mixamo / perfcap): the whole call is one launch each way
             pose_idx, inverse, uniq_host, counts = self._batch_index(idxs)
