@@ -210,6 +210,12 @@ SIGNATURES = {
     "anerf_rand_fill_dev": (C.c_int, [C.POINTER(AnerfRandJob), C.c_int32, C.c_void_p, C.c_int32, C.c_void_p]),
     "anerf_adam_step_dev": (C.c_int, [C.c_void_p] * 4 + [C.c_int64, C.c_float, C.c_float, C.c_float, C.c_void_p, C.c_int32, C.c_int32,
                                       C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "anerf_mlp_raw_train_dev": (C.c_int, [C.POINTER(AnerfConfig), C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
+                                          C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_int32, C.c_int32, C.c_void_p, C.POINTER(AnerfSaved), C.c_void_p]),
+    "anerf_encode_backward_dev": (C.c_int, [C.POINTER(AnerfConfig), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                            C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
+                                            C.c_void_p, C.c_void_p]),
     "anerf_route_rows_workspace_size": (C.c_int64, [C.c_int64, C.c_int32]),
     "anerf_route_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32] + [C.c_void_p] * 4 + [C.c_int64, C.c_void_p]),
     "anerf_dispatch_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,

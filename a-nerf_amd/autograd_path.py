@@ -65,15 +65,11 @@ class _MlpRawFn(torch.autograd.Function):
         skts = meta["skts"]
         stride = 0 if skts.shape[0] == 1 else 16 * cfg.n_joints
         codes = meta.get("codes")
-        cc = cfg.c()
-        b3 = meta.get("precision", "fp32") == "bf16x3"
-        packed, aux = meta["packed_b3"] if b3 else meta["packed"]
-        fwd = _lib.load().anerf_mlp_raw_train_b3 if b3 else _lib.load().anerf_mlp_raw_train
-        _lib.check(fwd(
-            C.byref(cc), _p(packed), _p(aux), _p(meta["rays"]), meta["rays"].shape[1], _p(z), _p(skts), stride,
-            _p(meta.get("cam")), _p(codes), 0 if codes is None else codes.shape[0], float(meta["tau_v"]),
-            float(meta["tau_d"]), _p(meta["cut_v"]), _p(meta["cut_d"]), n, s, _p(raw), C.byref(st), _stream()),
-            "anerf_mlp_raw_train")
+        prec = meta.get("precision", "fp32")
+        packed, aux = meta["packed_b3"] if prec == "bf16x3" else meta["packed"]
+        ops.mlp_raw_train(cfg, prec, packed, aux, meta["rays"], z, skts, stride, meta.get("cam"), codes, meta["tau_v"], meta["tau_d"], meta["cut_v"],
+                          meta["cut_d"], raw, st)
+        ctx.step = ops.active_step()          # the backward reads tau where the forward did
         ctx.meta, ctx.sv, ctx.T, ctx.P = meta, sv, T, P
         ctx.shapes = [tuple(p.shape) for p in params]
         return raw
@@ -122,10 +118,13 @@ class _MlpRawFn(torch.autograd.Function):
                 g_skts = torch.empty_like(skts)          # every element is written (row 3 as zeros) by k_pose_reduce
                 dyw = torch.empty(P, 72, dtype=torch.float32, device=dev)
                 dqw = torch.empty(P, 72, dtype=torch.float32, device=dev)
-                _lib.check(lib.anerf_encode_backward(
-                    C.byref(cc), _p(dx), _p(du), _p(rays), rays.shape[1], _p(z), _p(skts), 16 * cfg.n_joints,
-                    float(meta["tau_v"]), float(meta["tau_d"]), _p(meta["cut_v"]), _p(meta["cut_d"]), n, s, _p(dyw), _p(dqw),
-                    _p(g_skts), _stream()), "anerf_encode_backward")
+                tail = (_p(meta["cut_v"]), _p(meta["cut_d"]), n, s, _p(dyw), _p(dqw), _p(g_skts), _stream())
+                front = (C.byref(cc), _p(dx), _p(du), _p(rays), rays.shape[1], _p(z), _p(skts), 16 * cfg.n_joints)
+                if ctx.step is not None:
+                    rc = lib.anerf_encode_backward_dev(*front, C.c_void_p(ctx.step.ptr), *tail)
+                else:
+                    rc = lib.anerf_encode_backward(*front, float(meta["tau_v"]), float(meta["tau_d"]), *tail)
+                _lib.check(rc, "anerf_encode_backward")
             if need_codes:
                 codes = meta["codes"]
                 g_codes = torch.zeros_like(codes)
@@ -312,7 +311,6 @@ def encode_rows(net, kw, z):
     out = torch.empty(n * s, cfg.x_width, dtype=torch.float32, device=dev)
     packed, aux = net.packed(0)
     px, pu = (t.long() for t in perm_tables(cfg, dev))
-    cc = cfg.c()
     step = max(1, ENCODE_POINTS // s)
     for a in range(0, n, step):
         b = min(n, a + step)
@@ -326,10 +324,8 @@ def encode_rows(net, kw, z):
         sk = skts if skts.shape[0] == 1 else skts[a:b]
         # (the fused network's own output is not used: any code row will do for it, eval mode's extra mean-code row is not in this table)
         cm = None if cam is None else cam[a:b].clamp(0, codes.shape[0] - 1)
-        _lib.check(_lib.load().anerf_mlp_raw_train(
-            C.byref(cc), _p(packed), _p(aux), _p(rb), rays.shape[1], _p(zz), _p(sk), 0 if sk.shape[0] == 1 else 16 * cfg.n_joints, _p(cm), _p(codes),
-            0 if codes is None else codes.shape[0], float(kw["tau_v"]), float(kw["tau_d"]), _p(kw["cut_v"]), _p(kw["cut_d"]), b - a, s, _p(raw),
-            C.byref(st), _stream()), "anerf_mlp_raw_train")
+        ops.mlp_raw_train(cfg, "fp32", packed, aux, rb, zz, sk, 0 if sk.shape[0] == 1 else 16 * cfg.n_joints, cm, codes, kw["tau_v"], kw["tau_d"],
+                          kw["cut_v"], kw["cut_d"], raw, st)
         o = out[a * s:b * s]
         o[:, px] = x.view(T.p_pad, -1)[:P]
         o[:, cfg.dim_x + pu[:cfg.dim_d]] = u.view(T.p_pad, -1)[:P, :cfg.dim_d]

@@ -551,11 +551,11 @@ static int saved_ok(const AnerfSaved* s) {
   return s && s->h && s->f && s->g && s->x && s->u && s->p_pad > 0 && s->p_pad % 128 == 0;
 }
 
-int anerf_mlp_raw_train(const AnerfConfig* cfg, const float* packed, const float* aux, const float* rays,
-                        int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride,
-                        const float* cam_idx, const float* codes, int32_t n_codes, float tau_v, float tau_d,
-                        const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* raw,
-                        const AnerfSaved* saved, void* stream) {
+// tau_dev: {tau_v, tau_d} in device memory instead of the two values
+static int mlp_raw_train_impl(const AnerfConfig* cfg, const float* packed, const float* aux, const float* rays, int32_t ray_stride, const float* z_vals,
+                              const float* skts, int64_t skt_ray_stride, const float* cam_idx, const float* codes, int32_t n_codes, float tau_v,
+                              float tau_d, const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* raw,
+                              const AnerfSaved* saved, void* stream, const float* tau_dev) {
   AnerfLayout L;
   const int rc = anerf_layout(cfg, 0, &L);
   if (rc) return rc;
@@ -568,7 +568,16 @@ int anerf_mlp_raw_train(const AnerfConfig* cfg, const float* packed, const float
   if (skt_ray_stride != 0 && skt_ray_stride != 384) return set_error(ANERF_E_SHAPE, "mlp_raw_train: skt_ray_stride 0|384");
   return mlp_raw_entry(cfg, packed, aux, rays, ray_stride, z_vals, skts, skt_ray_stride, cam_idx, codes, n_codes, tau_v,
                        tau_d, cutoff_v, cutoff_d, nullptr, 0, (long long)n_rays * n_samples, n_rays, n_samples,
-                       L.n_stages, raw, false, saved, (hipStream_t)stream);
+                       L.n_stages, raw, false, saved, (hipStream_t)stream, nullptr, tau_dev);
+}
+
+int anerf_mlp_raw_train(const AnerfConfig* cfg, const float* packed, const float* aux, const float* rays,
+                        int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride,
+                        const float* cam_idx, const float* codes, int32_t n_codes, float tau_v, float tau_d,
+                        const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* raw,
+                        const AnerfSaved* saved, void* stream) {
+  return mlp_raw_train_impl(cfg, packed, aux, rays, ray_stride, z_vals, skts, skt_ray_stride, cam_idx, codes, n_codes, tau_v, tau_d, cutoff_v,
+                            cutoff_d, n_rays, n_samples, raw, saved, stream, nullptr);
 }
 
 int anerf_build_perm_tables_b3(const AnerfConfig* cfg, int32_t* perm_x, int32_t* perm_u) {
@@ -585,11 +594,10 @@ int anerf_build_perm_tables_b3(const AnerfConfig* cfg, int32_t* perm_x, int32_t*
   return ANERF_OK;
 }
 
-int anerf_mlp_raw_train_b3(const AnerfConfig* cfg, const float* packed, const float* aux, const float* rays,
-                           int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride,
-                           const float* cam_idx, const float* codes, int32_t n_codes, float tau_v, float tau_d,
-                           const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* raw,
-                           const AnerfSaved* saved, void* stream) {
+static int mlp_raw_train_b3_impl(const AnerfConfig* cfg, const float* packed, const float* aux, const float* rays, int32_t ray_stride,
+                                 const float* z_vals, const float* skts, int64_t skt_ray_stride, const float* cam_idx, const float* codes,
+                                 int32_t n_codes, float tau_v, float tau_d, const float* cutoff_v, const float* cutoff_d, int32_t n_rays,
+                                 int32_t n_samples, float* raw, const AnerfSaved* saved, void* stream, const float* tau_dev) {
   if (n_rays == 0) return ANERF_OK;
   AnerfLayout L;
   const int rc = anerf_layout(cfg, 3, &L);
@@ -603,7 +611,27 @@ int anerf_mlp_raw_train_b3(const AnerfConfig* cfg, const float* packed, const fl
   if (!saved_ok(saved) || saved->p_pad < (int64_t)n_rays * n_samples) return set_error(ANERF_E_WORKSPACE, "mlp_raw_train_b3: AnerfSaved");
   return mlp_b3_entry(cfg, packed, aux, rays, ray_stride, z_vals, skts, skt_ray_stride, cam_idx, codes, n_codes, tau_v, tau_d,
                       cutoff_v, cutoff_d, (long long)n_rays * n_samples, n_rays, n_samples, L.n_stages, raw, saved,
-                      (hipStream_t)stream);
+                      (hipStream_t)stream, nullptr, tau_dev);
+}
+
+int anerf_mlp_raw_train_b3(const AnerfConfig* cfg, const float* packed, const float* aux, const float* rays,
+                           int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride,
+                           const float* cam_idx, const float* codes, int32_t n_codes, float tau_v, float tau_d,
+                           const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* raw,
+                           const AnerfSaved* saved, void* stream) {
+  return mlp_raw_train_b3_impl(cfg, packed, aux, rays, ray_stride, z_vals, skts, skt_ray_stride, cam_idx, codes, n_codes, tau_v, tau_d,
+                               cutoff_v, cutoff_d, n_rays, n_samples, raw, saved, stream, nullptr);
+}
+
+int anerf_mlp_raw_train_dev(const AnerfConfig* cfg, int32_t precision, const float* packed, const float* aux, const float* rays,
+                            int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride, const float* cam_idx,
+                            const float* codes, int32_t n_codes, const AnerfStepBlock* block, const float* cutoff_v, const float* cutoff_d,
+                            int32_t n_rays, int32_t n_samples, float* raw, const AnerfSaved* saved, void* stream) {
+  if (!block) return set_error(ANERF_E_NULL, "mlp_raw_train_dev: NULL block");
+  if (precision != 0 && precision != 1) return set_error(ANERF_E_CONFIG, "mlp_raw_train_dev: precision 0|1");
+  return (precision == 1 ? mlp_raw_train_b3_impl : mlp_raw_train_impl)(cfg, packed, aux, rays, ray_stride, z_vals, skts, skt_ray_stride, cam_idx,
+                                                                      codes, n_codes, 0.f, 0.f, cutoff_v, cutoff_d, n_rays, n_samples, raw,
+                                                                      saved, stream, &block->tau_v);
 }
 
 int anerf_composite_backward(const AnerfConfig* cfg, const float* raw, const float* z_vals, const float* rays,
@@ -811,10 +839,10 @@ int anerf_input_grads_b3(const AnerfConfig* cfg, const float* packed_i, const fl
   return mlp_bwd_in_b3_entry(packed_i, dz, dzv, dx, du, n_points, p_pad, L.n_stages, u_width(cfg), (hipStream_t)stream);
 }
 
-int anerf_encode_backward(const AnerfConfig* cfg, const float* dx, const float* du, const float* rays,
-                          int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride, float tau_v,
-                          float tau_d, const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples,
-                          float* dy_ws, float* dq_ws, float* dskts, void* stream) {
+static int encode_backward_impl(const AnerfConfig* cfg, const float* dx, const float* du, const float* rays, int32_t ray_stride,
+                                const float* z_vals, const float* skts, int64_t skt_ray_stride, float tau_v, float tau_d, const float* cutoff_v,
+                                const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* dy_ws, float* dq_ws, float* dskts, void* stream,
+                                const float* tau_dev) {
   if (!config_ok(cfg)) return set_error(ANERF_E_CONFIG, "unsupported AnerfConfig");
   if (!dx || !du || !rays || !z_vals || !skts || !cutoff_v || !cutoff_d || !dy_ws || !dq_ws || !dskts)
     return set_error(ANERF_E_NULL, "encode_backward: NULL pointer");
@@ -822,7 +850,24 @@ int anerf_encode_backward(const AnerfConfig* cfg, const float* dx, const float* 
   if (n_rays == 0) return ANERF_OK;
   return launch_encode_bwd(cfg->multires_views, dx, du, u_width(cfg), rays, ray_stride, z_vals, skts, skt_ray_stride, tau_v,
                            tau_d, cutoff_v, cutoff_d, n_rays, n_samples, dy_ws, dq_ws, dskts, false, (hipStream_t)stream, nullptr,
-                           cfg->cutoff_bones);
+                           cfg->cutoff_bones, tau_dev);
+}
+
+int anerf_encode_backward(const AnerfConfig* cfg, const float* dx, const float* du, const float* rays,
+                          int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride, float tau_v,
+                          float tau_d, const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples,
+                          float* dy_ws, float* dq_ws, float* dskts, void* stream) {
+  return encode_backward_impl(cfg, dx, du, rays, ray_stride, z_vals, skts, skt_ray_stride, tau_v, tau_d, cutoff_v, cutoff_d, n_rays, n_samples, dy_ws,
+                              dq_ws, dskts, stream, nullptr);
+}
+
+int anerf_encode_backward_dev(const AnerfConfig* cfg, const float* dx, const float* du, const float* rays, int32_t ray_stride,
+                              const float* z_vals, const float* skts, int64_t skt_ray_stride, const AnerfStepBlock* block,
+                              const float* cutoff_v, const float* cutoff_d, int32_t n_rays, int32_t n_samples, float* dy_ws, float* dq_ws,
+                              float* dskts, void* stream) {
+  if (!block) return set_error(ANERF_E_NULL, "encode_backward_dev: NULL block");
+  return encode_backward_impl(cfg, dx, du, rays, ray_stride, z_vals, skts, skt_ray_stride, 0.f, 0.f, cutoff_v, cutoff_d, n_rays, n_samples, dy_ws, dq_ws,
+                              dskts, stream, &block->tau_v);
 }
 
 int anerf_code_grads(const AnerfConfig* cfg, const float* du, const float* cam_idx, int32_t n_rays, int32_t n_samples,

@@ -250,6 +250,25 @@ class step_block:
         _active_step = self.prev
 
 
+def active_step():
+    """the StepBlock that per-step scalars go through now, or None"""
+    return _active_step
+
+
+def mlp_raw_train(cfg, precision, packed, aux, rays, z, skts, skt_stride, cam, codes, tau_v, tau_d, cut_v, cut_d, raw, saved):
+    """anerf_mlp_raw_train ("fp32") / anerf_mlp_raw_train_b3 ("bf16x3") over rays x depths z [N,S]; inside `with step_block(blk)` tau is the
+    block's"""
+    b3, cc, (n, s) = precision == "bf16x3", cfg.c(), z.shape
+    front = (_p(packed), _p(aux), _p(rays), rays.shape[1], _p(z), _p(skts), skt_stride, _p(cam), _p(codes), 0 if codes is None else codes.shape[0])
+    back = (_p(cut_v), _p(cut_d), n, s, _p(raw), C.byref(saved), _stream())
+    lib = _lib.load()
+    if _active_step is not None:
+        rc = lib.anerf_mlp_raw_train_dev(C.byref(cc), int(b3), *front, C.c_void_p(_active_step.ptr), *back)
+    else:
+        rc = (lib.anerf_mlp_raw_train_b3 if b3 else lib.anerf_mlp_raw_train)(C.byref(cc), *front, float(tau_v), float(tau_d), *back)
+    _lib.check(rc, "anerf_mlp_raw_train")
+
+
 class DeviceRng:
     """Counter-based generator behind anerf_rand_fill: (key, offset) on the host, one launch per `fill`.  Stands where the
     reference calls torch.rand / torch.randn on the device (ray_utils.py:171-180,240-246; nerf.py:176-182;

@@ -363,7 +363,7 @@ typedef struct AnerfProfile {
 #define ANERF_MAX_ADAM_GROUPS 4
 typedef struct AnerfStepBlock {          /* DEVICE memory, 16-byte aligned; written only by anerf_step_block_write */
   uint64_t rng_seed, rng_offset;         /* anerf_rand_fill_dev                                                     */
-  float tau_v, tau_d;                    /* AnerfForwardIO.step (adjacent: the kernels read them as a pair)         */
+  float tau_v, tau_d;                    /* AnerfForwardIO.step, *_dev (adjacent: the kernels read them as a pair)   */
   float adam_step_size[ANERF_MAX_ADAM_GROUPS];    /* lr / (1 - beta1^step)                                          */
   float adam_sqrt_bc2[ANERF_MAX_ADAM_GROUPS];     /* sqrt(1 - beta2^step)                                           */
   float adam_grad_scale[ANERF_MAX_ADAM_GROUPS];   /* 1/world after a summed all-reduce, else 1                      */
@@ -387,6 +387,17 @@ int anerf_rand_fill_dev(const struct AnerfRandJob* jobs, int32_t n_jobs, const A
 int anerf_adam_step_dev(float* params, float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float beta1, float beta2, float eps,
                         const AnerfStepBlock* block, int32_t group, int32_t zero_grads, int32_t n_tensors, float* partials,
                         float* norms2, void* stream);
+/* The staged passes with tau_v / tau_d taken from the block: anerf_mlp_raw_train (precision 0) or anerf_mlp_raw_train_b3 (precision 1), and
+ * anerf_encode_backward. */
+int anerf_mlp_raw_train_dev(const AnerfConfig* cfg, int32_t precision, const float* packed, const float* aux,
+                            const float* rays, int32_t ray_stride, const float* z_vals,
+                            const float* skts, int64_t skt_ray_stride, const float* cam_idx,
+                            const float* codes, int32_t n_codes, const AnerfStepBlock* block, const float* cutoff_v, const float* cutoff_d,
+                            int32_t n_rays, int32_t n_samples, float* raw, const AnerfSaved* saved, void* stream);
+int anerf_encode_backward_dev(const AnerfConfig* cfg, const float* dx, const float* du, const float* rays,
+                              int32_t ray_stride, const float* z_vals, const float* skts, int64_t skt_ray_stride,
+                              const AnerfStepBlock* block, const float* cutoff_v, const float* cutoff_d,
+                              int32_t n_rays, int32_t n_samples, float* dy_ws, float* dq_ws, float* dskts, void* stream);
 
 typedef struct AnerfForwardIO {
   const float *packed_c, *aux_c, *packed_f, *aux_f;
