@@ -124,12 +124,22 @@ class Trainer:
         n_rays = int(batch["target_s"].shape[0])
         # the key holds everything a captured graph has frozen: sizes, phase flags, the pose layout, and the ADDRESSES of the
         # static inputs (an entry that changes shape / dtype or flips tensor <-> None gets another graph, not a stale buffer)
-        key = (n_rays, popt_detach, no_pose) + (layer.stage_batch(kp_idx) if layer is not None else ()) + (self._static.identity(sb),)
+        key = (n_rays, popt_detach, no_pose) + (layer.stage_batch(kp_idx) if layer is not None else ()) + (self._static.identity(sb),) + self._attached()
         only = 0 if (no_pose and len(f.param_groups) > 1) else None
         self._cur = (sb, kp_idx, popt_detach, no_pose)
         out = self._gs.step(i, key=key, due=f._due(i, only))
         self._cur = None
         return self._finish_iteration(out["loss_dict"], out["stats"], out["optim"], out["alpha"], global_step)
+
+    def _attached(self):
+        """graph key: the adapters that the caster renders with (they may be exchanged or detached between two steps).  Those that a key names
+        are kept, so that no other module takes their place in memory"""
+        caster = self.render_kwargs_train["ray_caster"]
+        caster = getattr(caster, "module", caster)
+        ads = [net.adapters() for net in (caster.network, caster.network_fine) if net is not None]
+        keep = self.__dict__.setdefault("_key_adapters", {})
+        keep.update({id(a): a for a in ads if a is not None})
+        return tuple(None if a is None else id(a) for a in ads)
 
     def _finish_iteration(self, loss_dict, stats, optim_stats, alpha, global_step):
         """the host-side tail of an iteration (trainer.py:262-277): learning-rate decay, tau / alpha schedules, the stats dict"""
