@@ -20,6 +20,7 @@ import weakref
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -124,7 +125,13 @@ def combine_rows(z, plan, weights=None):
 
 
 def _needs_grad(t, w=None):
-    return torch.is_grad_enabled() and (torch.is_tensor(t) and t.requires_grad or torch.is_tensor(w) and w.requires_grad)
+    return _forward_mode() or torch.is_grad_enabled() and (torch.is_tensor(t) and t.requires_grad or torch.is_tensor(w) and w.requires_grad)
+
+
+def _forward_mode():
+    """inside a level of forward-mode differentiation, whose dual tensors need not require a gradient (and which no_grad does not switch
+    off): a call goes through its autograd function there, which refuses tangents instead of losing them"""
+    return forward_ad._current_level >= 0
 
 
 def _check_plan(plan, name):
@@ -187,7 +194,7 @@ def adapter_linear(x, weight, down, up, rows, bias=None, scale=1.0):
         raise ValueError(f"adapter_linear: 1 .. {ops._lib.MAX_GROUPS} adapters of rank 1 .. {ops._lib.MAX_RANK} and no empty side, got {tuple(down.shape)}")
     if grads and (weight.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("adapter_linear: weight and bias are frozen beside adapters (requires_grad_(False) them, or detach)")
-    grads = grads and (x.requires_grad or down.requires_grad or up.requires_grad)
+    grads = grads and (x.requires_grad or down.requires_grad or up.requires_grad) or _forward_mode()
     scale_of = None
     if torch.is_tensor(scale):
         if scale.dtype != torch.float32 or scale.device != dev or tuple(scale.shape) != (L,):

@@ -1,4 +1,5 @@
-"""Adapters in training: gradients over several ranks (CPU, gloo), captured steps whose schedule moves tau."""
+"""Adapters in training: gradients over several ranks (CPU, gloo), captured steps whose schedule moves tau, forward
+mode."""
 import importlib
 import os
 import sys
@@ -12,6 +13,7 @@ import torch.multiprocessing as mp
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 ad = importlib.import_module("a-nerf_amd.adapters")
 networks = importlib.import_module("a-nerf_amd.networks")
+ops = importlib.import_module("a-nerf_amd.ops")
 raycaster = importlib.import_module("a-nerf_amd.raycaster")
 trainer = importlib.import_module("a-nerf_amd.trainer")
 
@@ -118,7 +120,7 @@ def test_the_staged_passes_in_a_captured_step_follow_tau(form):
     """GraphedTrainStep over the passes that are composed one by one -- an adapted render, and the staged route of a plain one (with pose
     gradients too) -- while the schedule moves tau and the learning rate every iteration: bit for bit the eager steps"""
     import test_graph_step as tg
-    optim, ops = importlib.import_module("a-nerf_amd.optim"), importlib.import_module("a-nerf_amd.ops")
+    optim = importlib.import_module("a-nerf_amd.optim")
     graph_step, render_mod = importlib.import_module("a-nerf_amd.graph_step"), importlib.import_module("a-nerf_amd.render")
     dev, n_rays, n_iter = torch.device("cuda"), 96, 7
     runs = []
@@ -173,7 +175,7 @@ def test_the_staged_passes_in_a_captured_step_follow_tau(form):
 
 def test_the_dev_forms_of_the_staged_passes_refuse():
     import ctypes
-    lib_mod, ops = importlib.import_module("a-nerf_amd._lib"), importlib.import_module("a-nerf_amd.ops")
+    lib_mod = importlib.import_module("a-nerf_amd._lib")
     lib, cc, P = lib_mod.load(), ops.PathConfig().c(), ctypes.c_void_p(0x7F0000001000)          # never read: every call returns before its launch
     sv = lib_mod.AnerfSaved(P, P, P, P, P, 128)
     fwd = lambda prec=0, block=P, packed=P, saved=sv, s=16: lib.anerf_mlp_raw_train_dev(ctypes.byref(cc), prec, packed, P, P, 11, P, P, 0, None, None, 0, block, P, P, 4, s,
@@ -183,3 +185,38 @@ def test_the_dev_forms_of_the_staged_passes_refuse():
     assert fwd(2) == -1
     bwd = lambda block=P, dx=P, stride=384, n=4: lib.anerf_encode_backward_dev(ctypes.byref(cc), dx, P, P, 11, P, P, stride, block, P, P, n, 16, P, P, P, None)
     assert bwd(block=None) == -3 and bwd(dx=None) == -3 and bwd(stride=0) == -2 and bwd(n=0) == 0
+
+
+def _plan_stub():
+    buf = torch.zeros(64, dtype=torch.int32)
+    return ops.RowPlan(buf, 4, 1, 3, (4,))
+
+
+def test_forward_mode_is_refused_not_dropped(monkeypatch):
+    """a dual tensor does not `require grad`: its tangent must not vanish (the launches are stubbed: nothing is computed)"""
+    import torch.autograd.forward_ad as fw
+    calls = []
+    monkeypatch.setattr(ops, "dispatch_rows", lambda x, plan, w=None: calls.append(1) or torch.zeros(4, 8))
+    monkeypatch.setattr(ops, "combine_rows", lambda z, plan, w=None: calls.append(1) or torch.zeros(4, 8))
+    monkeypatch.setattr(ops, "_adapter_linear", lambda *a, **k: calls.append(1) or (torch.zeros(4, 6), torch.zeros(4, 16)))
+    monkeypatch.setattr(ops, "_adapter_linear_few", lambda *a, **k: calls.append(1) or torch.zeros(4, 6))
+    monkeypatch.setattr(ops, "_route_rows", lambda *a: _plan_stub())
+    monkeypatch.setattr(ad, "_check_tensors", lambda *a: None)                   # (tensors on the CPU are refused there)
+    plan, r = _plan_stub(), torch.randn
+    x, w, W, A, B, b, s = r(4, 8), r(4, 1), r(6, 8), r(3, 2, 8), r(3, 6, 2), r(6), torch.ones(3)
+    idx = torch.zeros(4, dtype=torch.long)
+    lin = lambda **k: ad.adapter_linear(**{**dict(x=x, weight=W, down=A, up=B, rows=plan, bias=b, scale=s), **k})
+    with fw.dual_level():
+        d = lambda t: fw.make_dual(t, torch.ones_like(t))
+        cases = [lambda: ad.dispatch_rows(d(x), plan), lambda: ad.combine_rows(d(x), plan), lambda: ad.combine_rows(x, plan, d(w))]
+        for rows in (plan, idx):
+            cases += [lambda k=k, t=t, rows=rows: lin(rows=rows, **{k: d(t)}) for k, t in (("x", x), ("weight", W), ("down", A), ("up", B), ("bias", b), ("scale", s))]
+        for i, f in enumerate(cases):
+            for grad in (True, False):                                           # no_grad does not switch forward mode off
+                with pytest.raises((NotImplementedError, RuntimeError)), torch.set_grad_enabled(grad):
+                    f()
+                    pytest.fail(f"case {i} answered without its tangent", pytrace=False)
+        # and calls without a tangent run there as anywhere
+        n = len(calls)
+        ad.dispatch_rows(x, plan), ad.combine_rows(x, plan, w), lin(), lin(rows=idx)
+        assert len(calls) == n + 4
