@@ -30,23 +30,39 @@ from .ops import RowPlan, SortedRows, route_rows  # noqa: F401
 # A leaf's gradient node belongs to the stream it was first used on, and lives as long as any graph that reaches the leaf.  While an
 # EAGER graph of a leaf is alive, a backward that is being captured makes autograd order the capturing stream against that other
 # stream -- which a capture does not allow, and the exception ends the process.  The calls below therefore know which of their graphs are
-# alive, and refuse such a backward with an exception that can be handled.
+# alive, and refuse such a backward with an exception that can be handled.  (Graphs that hold none of these calls they do not know.)
 class _Graph:
-    """one call's graph: its leaves and the stream it was built on (alive while autograd holds the call's node)"""
-    __slots__ = ("leaves", "stream", "__weakref__")
+    """one call's graph: the leaves among its arguments, the nodes behind the others, and the stream it was built on (alive while autograd
+    holds the call's node)"""
+    __slots__ = ("leaves", "nodes", "stream", "__weakref__")
 
-    def __init__(self, leaves):
-        self.leaves, self.stream = leaves, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    def __init__(self, asking):
+        self.leaves, self.nodes = [t for t in asking if t.is_leaf], [t.grad_fn for t in asking if not t.is_leaf]
+        self.stream = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+    def reach(self):
+        """ids of all leaves that the graph gives gradients to (walked where a capture asks for it only)"""
+        ids, seen, todo = {id(t) for t in self.leaves}, {}, list(self.nodes)
+        while todo:
+            node = todo.pop()
+            if node is None or node in seen:
+                continue
+            seen[node] = True
+            leaf = getattr(node, "variable", None)
+            if leaf is not None:
+                ids.add(id(leaf))
+            todo += [n for n, _ in node.next_functions]
+        return ids
 
 
 _alive, _alive_lock = weakref.WeakSet(), threading.Lock()
 
 
 def _graph_of(*tensors):
-    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
-    if not leaves:
+    asking = [t for t in tensors if t is not None and t.requires_grad]
+    if not asking:
         return None
-    graph = _Graph(leaves)
+    graph = _Graph(asking)
     with _alive_lock:
         _alive.add(graph)
     return graph
@@ -59,10 +75,10 @@ def _capturing():
 def _check_capture(graph):
     if graph is None or not _capturing():
         return
-    mine = {id(t) for t in graph.leaves}
     with _alive_lock:
-        others = list(_alive)
-    if any(other is not graph and other.stream != graph.stream and any(id(t) in mine for t in other.leaves) for other in others):
+        others = [other for other in _alive if other is not graph and other.stream != graph.stream]
+    mine = graph.reach() if others else ()
+    if any(not mine.isdisjoint(other.reach()) for other in others):
         raise RuntimeError("this backward is being captured while an eager graph of the same leaf tensor is alive (an output of an eager call that "
                            "is still referenced): drop it before the capture")
 

@@ -115,6 +115,45 @@ def test_a_captured_step_belongs_to_the_adapters_it_was_captured_with(monkeypatc
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("form", ["cast", "stacked", "rows", "weights", "dispatched", "chain"])
+def test_the_capture_guard_sees_leaves_behind_other_operations(form, monkeypatch):
+    """a captured backward beside a living eager graph is refused also where the leaf is not an argument itself: master weights cast to the
+    rows' type, parameters stacked, rows of a trained layer in front.  The capture is only claimed: a real one would end the process without it"""
+    r = lambda *s: torch.randn(*s, device="cuda")
+    idx, W = torch.arange(8, device="cuda") % 2, r(16, 32)
+    A, B, lin, w = r(2, 4, 32).requires_grad_(), r(2, 16, 4).requires_grad_(), r(32, 32).requires_grad_(), r(8, 1).requires_grad_()
+    x, plan = r(8, 32), ad.route_rows(idx, 2)
+    other = r(2, 4, 32).requires_grad_()
+
+    def call():
+        if form == "cast":
+            return ad.adapter_linear(x.bfloat16(), W.bfloat16(), A.bfloat16(), B.bfloat16(), idx)
+        if form == "stacked":
+            return ad.adapter_linear(x, W, torch.stack([A[0] * 2, A[1]]), torch.cat([B[:1], B[1:]]), plan)
+        if form == "rows":
+            return ad.adapter_linear(torch.relu(x @ lin), W, A.detach(), B.detach(), idx)
+        if form == "weights":
+            return ad.combine_rows(x, plan, torch.sigmoid(w))
+        if form == "dispatched":
+            return ad.dispatch_rows((x @ lin) * 2, plan)
+        return ad.adapter_linear(ad.adapter_linear(x, r(32, 32), A * 1.0, r(2, 32, 4), idx), W, A.detach(), B.detach(), idx)
+
+    alive = call()
+    unrelated = ad.adapter_linear(x, W, other * 1.0, B.detach(), idx)              # lives on, shares no leaf
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = call()
+        monkeypatch.setattr(ad, "_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            y.float().sum().backward()
+        del alive
+        call().float().sum().backward()
+    side.synchronize()
+    assert unrelated.requires_grad
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("form", ["adapters", "staged", "staged bf16x3", "staged poses"])
 def test_the_staged_passes_in_a_captured_step_follow_tau(form):
     """GraphedTrainStep over the passes that are composed one by one -- an adapted render, and the staged route of a plain one (with pose
