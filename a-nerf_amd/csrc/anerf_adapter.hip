@@ -22,29 +22,40 @@ namespace anerf {
 // written, from HBM 33, with 16 rows a piece 35; 200 rows
 // x 4096 bf16: 13.7 us with 32 rows a piece, 10.2 with 16.  More waves a piece or deeper loads gain nothing: a few pieces are bound by
 // what one CU can load.
-// Kept as [position][Rp] fp32 (Rp = rank rounded up to 16, zeros behind the rank) for the gradient of B, and, for the 16-bit types, as what
-// k_main multiplies with: the nearest value hi and the rest lo, [hi of 16 ranks | lo of the same 16] per 16 ranks, which meet [B | B]
-// there -- h keeps 16 (bf16) or 21 (fp16) of its bits.  fp16's range does not hold every h: its rows are scaled first.
+// Kept as [position][Rp] fp32 (Rp = rank rounded up to 16, zeros behind the rank) for the gradient of B, and, for the 16-bit types, as what k_main
+// multiplies with: h as a sum of three (bf16) or two (fp16) values, each the nearest one to what the others leave, [first of 32 ranks | second |
+// third] per 32 ranks (16 where there are no more), which meet the same 32 ranks of B one after the other.  They hold the 24 bits of h, 23 in
+// fp16, whose range does not hold every h: its rows are scaled first.
+// (bf16 by two values, 16 bits of h: rank 32, 8192 x 4096 -> 4096 the same, rank 128, 8192 x 1024 -> 1024 1.5 of 57 us less)
+template <int DT> constexpr int pieces_of = DT == ANERF_BF16 ? 3 : DT == ANERF_F16 ? 2 : 1;
+// ranks and values of a row's operand form: where 16 ranks are all, two pieces of them lie in what a product contracts, and zeros beside an odd one
+__host__ __device__ constexpr int split_ranks(int Rp) { return Rp > 16 ? (Rp + 31) / 32 * 32 : 16; }
+template <int DT>
+__host__ __device__ constexpr int split_width(int Rp) { return Rp > 16 ? pieces_of<DT> * split_ranks(Rp) : (pieces_of<DT> + 1) / 2 * 32; }
 
 // ranks j .. j+3 of a row
-template <typename E>
-__device__ __forceinline__ void store_split(f32x4 v, E* row, int j) {
+template <int DT>
+__device__ __forceinline__ void store_split(f32x4 v, typename Elem<DT>::T* row, int j, int Rp) {
+  typedef typename Elem<DT>::T E;
   typedef E four __attribute__((ext_vector_type(4)));
-  four hi, lo;
+  const int W = Rp > 16 ? 32 : 16;
+  E* o = row + pieces_of<DT> * (j & -W) + (j & (W - 1));
+  if (pieces_of<DT> == 3 && W == 16) *reinterpret_cast<four*>(o + 48) = four{(E)0.f, (E)0.f, (E)0.f, (E)0.f};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    hi[e] = (E)v[e];
-    const float rest = v[e] - (float)hi[e];
-    lo[e] = __builtin_isfinite((float)hi[e]) ? (E)rest : (E)0.f;       // (infinity and NaN are carried by hi alone)
+  for (int p = 0; p < pieces_of<DT>; ++p) {
+    four piece;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      piece[e] = (E)v[e];
+      v[e] -= (float)piece[e];
+    }
+    *reinterpret_cast<four*>(o + W * p) = piece;
   }
-  E* o = row + 2 * (j & ~15) + (j & 15);
-  *reinterpret_cast<four*>(o) = hi;
-  *reinterpret_cast<four*>(o + 16) = lo;
 }
 
-// a row of h is divided by the power of two that brings its largest value into [1, 2); rows of zeros, infinities and NaN stay
+// a row of h is divided by the power of two that brings its largest value into [2^14, 2^15); rows of zeros, infinities and NaN stay
 __device__ __forceinline__ int row_exponent(float big) {
-  return big > 0.f && __builtin_isfinite(big) ? min(max(ilogbf(big), -100), 100) : 0;
+  return big > 0.f && __builtin_isfinite(big) ? max(ilogbf(big) - 14, -100) : 0;
 }
 
 constexpr int TH_WAVES = 4, TH_DEPTH = 4;
@@ -139,32 +150,34 @@ __global__ void __launch_bounds__(TH_WAVES * 64) k_thin(const typename Elem<DT>:
   if (part == 0 && j0 == 0) owner[p] = a;
   f32x4 v[(4 * NJ + 7) / 8];
   float big = 0.f;
+  const int end = DT == ANERF_F32 ? Rp : split_ranks(Rp);
 #pragma unroll
   for (int t = 0; t < (4 * NJ + 7) / 8; ++t) {
     const int j = 4 * (part + 8 * t);
-    if (j >= 16 * NJ || j0 + j >= Rp) continue;
+    if (j >= 16 * NJ || j0 + j >= end) continue;
     v[t] = *reinterpret_cast<const f32x4*>(tile + r * LINE + j);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[t][e] = j0 + j + e < R ? v[t][e] * s_a : 0.f;          // ranks of the padding: zero
       big = fmaxf(big, fabsf(v[t][e]));
     }
-    *reinterpret_cast<f32x4*>(h + (long long)p * Rp + j0 + j) = v[t];
+    if (j0 + j < Rp) *reinterpret_cast<f32x4*>(h + (long long)p * Rp + j0 + j) = v[t];
   }
-  if constexpr (DT == ANERF_F32) return;
-  if (DT == ANERF_F16 && gridDim.y > 1) return;                // (k_split_rows needs the whole row)
-  float shrink = 1.f;
-  if constexpr (DT == ANERF_F16) {
+  if constexpr (DT != ANERF_F32) {
+    if (DT == ANERF_F16 && gridDim.y > 1) return;              // (k_split_rows needs the whole row)
+    float shrink = 1.f;
+    if constexpr (DT == ANERF_F16) {
 #pragma unroll
-    for (int d = 4; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d));
-    const int e = row_exponent(big);
-    shrink = ldexpf(1.f, -e);
-    if (part == 0) factor[p] = ldexpf(1.f, e);
-  }
+      for (int d = 4; d; d >>= 1) big = fmaxf(big, __shfl_xor(big, d));
+      const int e = row_exponent(big);
+      shrink = ldexpf(1.f, -e);
+      if (part == 0) factor[p] = ldexpf(1.f, e);
+    }
 #pragma unroll
-  for (int t = 0; t < (4 * NJ + 7) / 8; ++t) {
-    const int j = 4 * (part + 8 * t);
-    if (j < 16 * NJ && j0 + j < Rp) store_split<E>(v[t] * shrink, split + (long long)p * 2 * Rp, j0 + j);
+    for (int t = 0; t < (4 * NJ + 7) / 8; ++t) {
+      const int j = 4 * (part + 8 * t);
+      if (j < 16 * NJ && j0 + j < end) store_split<DT>(v[t] * shrink, split + (long long)p * split_width<DT>(Rp), j0 + j, Rp);
+    }
   }
 }
 
@@ -181,7 +194,10 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
   const int e = row_exponent(big);
   if (i == 0) factor[p] = ldexpf(1.f, e);
   const float down = ldexpf(1.f, -e);
-  for (int j = 4 * i; j < Rp; j += 64) store_split<_Float16>(*reinterpret_cast<const f32x4*>(r + j) * down, split + (long long)p * 2 * Rp, j);
+  for (int j = 4 * i; j < split_ranks(Rp); j += 64) {
+    const f32x4 v = j < Rp ? *reinterpret_cast<const f32x4*>(r + j) * down : f32x4{0.f, 0.f, 0.f, 0.f};
+    store_split<ANERF_F16>(v, split + (long long)p * split_width<ANERF_F16>(Rp), j, Rp);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ y = x W^T ...
@@ -202,7 +218,7 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 struct MainArgs {
   const void *x, *w, *bias, *up;
   const int32_t *offsets, *order;
-  const void* h;               // operand form of h: [M][Rp] fp32, [M][2 Rp] 16-bit
+  const void* h;               // operand form of h: [M][Rp] fp32, [M][split_width] 16-bit
   const float* factor;         // fp16: power of two of every row of h
   const float* h32;            // [M][Rp]
   const int32_t* owner;        // the positions' adapters
@@ -325,7 +341,10 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
     const int w0 = t0 + wm * TM;                               // the wave's first position and output
     const long long c0 = n0 + wn * TN;
     const int last_col = (int)(P.N - 1 - c0 < TN ? P.N - 1 - c0 : TN);
-    const int chunks = P.Rp / 16, row_bytes = P.Rp * 4;        // (two 16-bit values or one fp32 a rank)
+    // a product contracts 64 bytes of h's row: 16 fp32 ranks; a piece of 32 ranks of a 16-bit type, or, where 16 are all, two pieces of them
+    const bool wide = DT != ANERF_F32 && P.Rp > 16;
+    const int times = wide ? pieces_of<DT> : (pieces_of<DT> + 1) / 2;      // products with the same ranks of B
+    const int row_bytes = DT == ANERF_F32 ? P.Rp * 4 : 2 * split_width<DT>(P.Rp);
     const char* hw = static_cast<const char*>(P.h) + (long long)w0 * row_bytes + 16 * q;
     int b0 = 0;                                                // of 64 adapters looked at together
     if (P.L > 64) {                                            // first those that hold the tile's first position
@@ -411,18 +430,23 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
       while (owners) {
         const int l = __builtin_ctzll(owners);
         owners &= owners - 1;
-        const int r0 = max(__builtin_amdgcn_readlane(lo, l) - w0, 0), r1 = min(__builtin_amdgcn_readlane(hi, l) - w0, TM);
+        int r0 = max(__builtin_amdgcn_readlane(lo, l) - w0, 0), r1 = min(__builtin_amdgcn_readlane(hi, l) - w0, TM);
         if (r0 >= r1) continue;                                // none of this wave's
         const E* bw = static_cast<const E*>(P.up) + ((long long)(b0 + l) * P.N + c0) * P.R;
-        for (int c = 0; c < chunks; ++c) {
-          const int j = 16 * c + (DT == ANERF_F32 ? 4 * q : 8 * (q & 1));
-          u32x4 bf[NI], hf[MI];
+        int j = DT == ANERF_F32 ? 4 * q : wide ? 8 * q : 8 * (q & 1);
+        u32x4 bf[NI];
+        for (int at = 0, s = 0; at < row_bytes; at += 64) {
+          const char* hs = hw + at;
+          asm volatile("" : "+s"(r0), "+s"(r1));               // (tests of the blocks are not kept across the loop: registers)
+          u32x4 hf[MI];
+          if (s == 0) {
 #pragma unroll
-          for (int n = 0; n < NI; ++n) bf[n] = load_tail<DT>(bw + min(BS * n + i, last_col) * P.R, j, P.R);
+            for (int n = 0; n < NI; ++n) bf[n] = load_tail<DT>(bw + min(BS * n + i, last_col) * P.R, j, P.R);
+          }
 #pragma unroll
           for (int m = 0; m < MI; ++m) {
             const int r = min(max(BS * m + i, r0), r1 - 1);
-            hf[m] = *reinterpret_cast<const u32x4*>(hw + r * row_bytes + 64 * c);
+            hf[m] = *reinterpret_cast<const u32x4*>(hs + r * row_bytes);
           }
 #pragma unroll
           for (int m = 0; m < MI; ++m) {
@@ -444,6 +468,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
               }
             }
           }
+          if (++s == times) s = 0, j += DT == ANERF_F32 ? 16 : 32;
         }
       }
       if (__builtin_amdgcn_readlane(hi, 63) >= t1) break;
@@ -1220,7 +1245,7 @@ static int launch_main(const MainArgs& P, hipStream_t st) {
   return run64();
 }
 
-// what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][2 Rp] (16-bit types) | factor [n_rows] (fp16) | the positions'
+// what k_thin leaves, in one buffer: h fp32 [n_rows][Rp] | operand form [n_rows][split_width] (16-bit types) | factor [n_rows] (fp16) | the positions'
 // adapters [n_rows]; byte offsets
 struct HLayout {
   int Rp;
@@ -1231,7 +1256,7 @@ static HLayout h_layout(const AnerfAdapterIO& A) {
   H.Rp = (A.rank + 15) / 16 * 16;
   const long long part = A.n_rows * H.Rp * 4, line = (A.n_rows + 3) / 4 * 16;
   H.split = part;
-  H.factor = A.dtype == ANERF_F32 ? part : 2 * part;
+  H.factor = A.dtype == ANERF_F32 ? part : part + A.n_rows * 2 * (A.dtype == ANERF_BF16 ? split_width<ANERF_BF16>(H.Rp) : split_width<ANERF_F16>(H.Rp));
   H.owner = H.factor + (A.dtype == ANERF_F16 ? line : 0);
   H.bytes = H.owner + line;
   return H;

@@ -1,0 +1,83 @@
+"""GPU: the bits that the low-rank term keeps, in every form of the product."""
+import importlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ad = importlib.import_module("a-nerf_amd.adapters")
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def same_kind(got, want):
+    """NaN where NaN, the same infinity where infinite, equal where finite"""
+    got, want = got.detach().double().cpu(), want.double().cpu()
+    ok = (got == want) | (got.isnan() & want.isnan())
+    assert ok.all(), (int((~ok).sum()), ok.numel(), got[~ok][:6].tolist(), want[~ok][:6].tolist(), (~ok).nonzero()[:6].tolist())
+
+
+def exact_data(M, K, N, L, R, dtype):
+    """every product and every sum a small whole number: h picks single values of x (1 .. 8, -8 .. -1 and some 0), so that its nearest value in 16
+    bits is h itself; the shared projection is 0"""
+    gen = torch.Generator().manual_seed(M + R)
+    x = torch.randint(-8, 9, (M, K), generator=gen).to(dtype)
+    x[::7] = 0                                                      # rows whose h is zero: 0 * infinity is NaN
+    down = torch.zeros(L, R, K)
+    for a in range(L):
+        down[a, torch.arange(R), torch.randperm(K, generator=gen)[:R]] = 1
+    up = torch.randint(-2, 3, (L, N, R), generator=gen).to(dtype)
+    idx = torch.randint(-1, L, (M,), generator=gen)
+    return x, torch.zeros(N, K, dtype=dtype), down.to(dtype), up, idx
+
+
+def term(x, down, up, idx, scale):
+    """s (x A^T) B^T term by term in 64 bits, so that infinities meet as the definition has them"""
+    out = torch.zeros(x.shape[0], up.shape[1], dtype=torch.float64)
+    for r, i in enumerate(idx.tolist()):
+        if i >= 0:
+            h = scale * (x[r].double()[None] * down[i].double()).sum(-1)
+            out[r] = (h[None] * up[i].double()).sum(-1)
+    return out
+
+
+@pytest.mark.parametrize("M,L", [(200, 1), (200, 100), (40, 1), (700, 2)])
+def test_the_low_rank_term_keeps_what_fp32_holds(M, L):
+    """h of two ranks: 256 + 1 + 2^-8 + 2^-12 and 256 + 1 + 2^-8, whose difference is 2^-12.  Every partial sum in any order is a multiple of 2^-12
+    below 2^10, so fp32 sums are exact and so is the answer; two values of 8 bits each do not hold the first."""
+    K, N, R = 16, 64, 16
+    x = torch.zeros(M, K).bfloat16()
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3] = 256, 1, 2.0 ** -8, 2.0 ** -12
+    down = torch.zeros(L, R, K).bfloat16()
+    down[:, 0, :4], down[:, 1, :3] = 1, 1
+    up = torch.zeros(L, N, R).bfloat16()
+    up[:, :, 0], up[:, :, 1] = 1, -1
+    idx = torch.arange(M) % L
+    W = torch.zeros(N, K).bfloat16()
+    got = ad.adapter_linear(x.cuda(), W.cuda(), down.cuda(), up.cuda(), idx.cuda())
+    same_kind(got, torch.full((M, N), 2.0 ** -12))
+    # the gradient of x: the same numbers through A^T and B^T
+    xz = torch.zeros(M, N, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    y = ad.adapter_linear(xz, W.t().contiguous().cuda(), up.transpose(1, 2).contiguous().cuda(), down.transpose(1, 2).contiguous().cuda(), idx.cuda())
+    (gx,) = torch.autograd.grad(y, xz, x.cuda())
+    same_kind(gx, torch.full((M, N), 2.0 ** -12))
+
+
+@pytest.mark.parametrize("R", [1, 16, 17, 33, 40, 48, 49, 65, 80, 100, 130])
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_whole_numbers_of_every_rank(R, dt):
+    """h, u, the low-rank term and the gradients of A and B as sums of whole numbers below 2^24: exact in fp32 in any order, rounded once"""
+    M, K, N, L = 150, 136, 90, 3
+    x, W, down, up, idx = exact_data(M, K, N, L, R, DT[dt])
+    g = torch.randint(-2, 3, (M, N), generator=torch.Generator().manual_seed(R)).to(DT[dt])
+    want = term(x, down, up, idx, 1.0)
+    dA, dB = torch.zeros(L, R, K, dtype=torch.float64), torch.zeros(L, N, R, dtype=torch.float64)
+    dx = torch.zeros(M, K, dtype=torch.float64)
+    for i in range(L):
+        r = (idx == i).nonzero()[:, 0]
+        u = g[r].double() @ up[i].double()
+        dx[r], dA[i], dB[i] = u @ down[i].double(), u.t() @ x[r].double(), g[r].double().t() @ (x[r].double() @ down[i].double().t())
+    xd, A, B = x.cuda().requires_grad_(), down.cuda().requires_grad_(), up.cuda().requires_grad_()
+    y = ad.adapter_linear(xd, W.cuda(), A, B, idx.cuda())
+    for got, ref in zip([y, *torch.autograd.grad(y, [xd, A, B], g.cuda())], (want, dx, dA, dB)):
+        same_kind(got, ref.to(DT[dt]))
