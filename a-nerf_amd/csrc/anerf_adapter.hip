@@ -47,7 +47,7 @@ __device__ __forceinline__ void store_split(f32x4 v, typename Elem<DT>::T* row, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       piece[e] = (E)v[e];
-      v[e] -= (float)piece[e];
+      v[e] -= (float)piece[e];                                 // (behind an infinity: NaN; k_main takes h itself where that shows)
     }
     *reinterpret_cast<four*>(o + W * p) = piece;
   }
@@ -480,6 +480,38 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM
         const float f = p < kept ? P.factor[p] : 1.f;
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] *= f;
+      }
+    }
+    // An infinite value of h or B has met pieces of the other's values there, zeros and ones of either sign among them, and infinity times 0
+    // is NaN.  Values that are not finite are therefore taken again, from h itself.
+    if constexpr (DT != ANERF_F32) {
+      float zero = 0.f;
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) zero = fmaf(acc[m][n][e], 0.f, zero);
+      if (!one_by_one && __any(!(zero == 0.f))) {
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+          const int p = w0 + BS * m + i;
+          const bool has = p < kept;
+          const E* br = static_cast<const E*>(P.up) + (has ? (long long)P.owner[p] * P.N : 0) * P.R;
+          const float* hr = P.h32 + (long long)(has ? p : t0) * P.Rp;
+#pragma unroll
+          for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (!has || __builtin_isfinite(acc[m][n][e])) continue;
+              const long long col = c0 + BS * n + 4 * q + e;
+              const E* b = br + (col < P.N ? col : P.N - 1) * P.R;
+              float dot = 0.f;
+#pragma unroll 1
+              for (int j = 0; j < P.R; ++j) dot = fmaf(hr[j], (float)b[j], dot);
+              acc[m][n][e] = dot;
+            }
+        }
       }
     }
   }

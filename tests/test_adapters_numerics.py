@@ -1,4 +1,4 @@
-"""GPU: the bits that the low-rank term keeps, in every form of the product."""
+"""GPU: infinities in adapters, and the bits that the low-rank term keeps, in every form of the product."""
 import importlib
 
 import pytest
@@ -39,6 +39,47 @@ def term(x, down, up, idx, scale):
             h = scale * (x[r].double()[None] * down[i].double()).sum(-1)
             out[r] = (h[None] * up[i].double()).sum(-1)
     return out
+
+
+FORMS = [(200, 2, 8), (200, 2, 20), (700, 3, 33), (40, 2, 8), (200, 100, 8), (130, 60, 40)]       # few adapters a tile, few rows, a tile of many adapters
+
+
+@pytest.mark.parametrize("M,L,R", FORMS)
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_infinite_entries_give_infinities(M, L, R, dt):
+    K, N = 64, 90
+    x, W, down, up, idx = exact_data(M, K, N, L, R, DT[dt])
+    inf = float("inf")
+    up[:, 3, 0], up[:, 50, R - 1], up[0, 7] = inf, -inf, inf        # one entry of a row of B, the last rank, a whole row
+    up[L - 1, 11, 0], up[L - 1, 11, 1] = inf, -inf
+    want = term(x, down, up, idx, 0.5)
+    assert want.isinf().any() and want.isnan().any() and want.isfinite().any()
+    c = [t.cuda() for t in (x, W, down, up)]
+    same_kind(ad.adapter_linear(*c, idx.cuda(), scale=0.5), want)
+    # the gradient of x is the same product the other way round, with the roles of A and B changed
+    xz = torch.zeros(M, N, dtype=DT[dt], device="cuda").requires_grad_()
+    y = ad.adapter_linear(xz, W.t().contiguous().cuda(), up.transpose(1, 2).contiguous().cuda(), down.transpose(1, 2).contiguous().cuda(), idx.cuda(), scale=0.5)
+    (gx,) = torch.autograd.grad(y, xz, x.cuda())
+    same_kind(gx, want)
+
+
+@pytest.mark.parametrize("M", [40, 200])
+def test_an_infinite_rank_beside_ranks_beyond_fp16(M):
+    """h of one rank is infinite, of the others past 65504: infinity plus finite numbers is infinity"""
+    K, N, R = 32, 48, 4
+    x, down = torch.full((M, K), 2.0 ** 10).half(), torch.zeros(1, R, K).half()
+    down[0, 0, 0], down[0, 1, 1], down[0, 2, 2] = float("inf"), 2.0 ** 10, -(2.0 ** 11)
+    up = torch.zeros(1, N, R).half()
+    up[0, :, 0], up[0, :, 1], up[0, :, 2], up[0, :, 3] = 1, -1, 1, 1
+    up[0, ::2, 0] = -1
+    idx = torch.zeros(M, dtype=torch.long)
+    h = torch.tensor([float("inf"), 2.0 ** 20, -(2.0 ** 21), 0.0], dtype=torch.float64)
+    # (0 * infinity in the sum over K would be NaN: x is nowhere 0)
+    want = (h[None] * up[0].double()).sum(-1)[None].expand(M, N)
+    assert want.isinf().all()
+    # columns of A that are 0 meet finite x only; A's infinity meets x = 1024
+    got = ad.adapter_linear(x.cuda(), torch.zeros(N, K).half().cuda(), down.cuda(), up.cuda(), idx.cuda())
+    same_kind(got, want)
 
 
 @pytest.mark.parametrize("M,L", [(200, 1), (200, 100), (40, 1), (700, 2)])
