@@ -1370,16 +1370,20 @@ int anerf_combine_rows_backward(const void* dy, const void* z, int32_t dtype, co
   return launch_rows(2, dtype, dy, z, weights, slot, kept, n_rows, k, width, dz, dweights, static_cast<hipStream_t>(stream));
 }
 
+constexpr int64_t ADAPTER_MAX_BLOCKS = INT64_C(1) << 24;
+static int64_t blocks64(int64_t rows, int64_t cols) { return (rows + 63) / 64 * ((cols + 63) / 64); }
+
 static int adapter_check(const AnerfAdapterIO* a) {
   if (!a) return set_error(ANERF_E_NULL, "adapter: null io");
   if (a->dtype != ANERF_F32 && a->dtype != ANERF_BF16 && a->dtype != ANERF_F16) return set_error(ANERF_E_CONFIG, "adapter: unknown element type");
   if (a->n_adapters < 1 || a->n_adapters > ROWS_MAX_GROUPS) return set_error(ANERF_E_SHAPE, "adapter: n_adapters must be 1 .. 1024");
   if (a->rank < 1 || a->rank > ANERF_MAX_RANK) return set_error(ANERF_E_SHAPE, "adapter: rank must be 1 .. 1024");
-  const int64_t lim = INT64_C(1) << 31, side = INT64_C(1) << 24;      // (tiles, pieces and byte offsets stay inside their integers)
+  const int64_t side = INT64_C(1) << 24;      // (tiles, pieces and byte offsets stay inside their integers)
   if (a->n_in < 1 || a->n_out < 1 || a->n_in > side || a->n_out > side) return set_error(ANERF_E_SHAPE, "adapter: n_in / n_out must be 1 .. 2^24");
-  if (a->n_rows < 0 || a->n_rows >= lim) return set_error(ANERF_E_SHAPE, "adapter: the number of rows must be 0 .. 2^31 - 1");
+  if (a->n_rows < 0 || a->n_rows >= INT64_C(1) << 28) return set_error(ANERF_E_SHAPE, "adapter: the number of rows must be 0 .. 2^28 - 1");
   if (a->x_stride < 0) return set_error(ANERF_E_SHAPE, "adapter: x_stride must not be negative");
-  if (((a->n_rows + 63) / 64) * ((a->n_out + 63) / 64) >= lim || ((a->n_rows + 63) / 64) * ((a->n_in + 63) / 64) >= lim)
+  // a launch has fewer than 2^32 work items, and a workgroup 256 of them
+  if (blocks64(a->n_rows, a->n_out) >= ADAPTER_MAX_BLOCKS || blocks64(a->n_rows, a->n_in) >= ADAPTER_MAX_BLOCKS)
     return set_error(ANERF_E_SHAPE, "adapter: too many output tiles for one launch");
   return ANERF_OK;
 }
@@ -1415,13 +1419,22 @@ int anerf_adapter_linear_few(const AnerfAdapterIO* a, const void* groups, int32_
   return launch_adapter_few(*a, groups, wide, static_cast<hipStream_t>(stream));
 }
 
-int64_t anerf_adapter_backward_workspace_size(const AnerfAdapterIO* a) {
+// the backward also transposes the weight and the adapters, 64 x 64 values a workgroup
+static int adapter_backward_check(const AnerfAdapterIO* a) {
   const int rc = adapter_check(a);
+  if (rc) return rc;
+  if (blocks64(a->n_out, a->n_in) + a->n_adapters * (blocks64(a->rank, a->n_in) + blocks64(a->n_out, a->rank)) >= ADAPTER_MAX_BLOCKS)
+    return set_error(ANERF_E_SHAPE, "adapter: weight and adapters too large to transpose in one launch");
+  return ANERF_OK;
+}
+
+int64_t anerf_adapter_backward_workspace_size(const AnerfAdapterIO* a) {
+  const int rc = adapter_backward_check(a);
   return rc ? rc : adapter_backward_workspace(*a);
 }
 
 int anerf_adapter_backward(const AnerfAdapterIO* a, const AnerfAdapterGradIO* g, void* workspace, int64_t ws_bytes, void* stream) {
-  const int rc = adapter_check(a);
+  const int rc = adapter_backward_check(a);
   if (rc) return rc;
   if (!g) return set_error(ANERF_E_NULL, "adapter_backward: null gradients");
   if (g->g_stride < 0) return set_error(ANERF_E_SHAPE, "adapter_backward: g_stride must not be negative");

@@ -183,7 +183,7 @@ int launch_route(const void* idx, int wide, long long n, int G, int32_t* offsets
 // One wave a row t: its k slots sit in the lanes, and the row is read once and written k times.  16 bytes a lane and access; the
 // elements behind the last whole 16 bytes of a row go one by one.  HBM-bound: T*D read + T*k*D written.  65520 x 1080 fp32: 111 us,
 // 5.1 TB/s; 8192 x 2048 bf16 to 8 places each: 65 us, 4.7 TB/s.
-constexpr int RW_WAVES = 4, RW_BATCH = 4;
+constexpr int RW_WAVES = 4, RW_BATCH = 4, RW_MAX_X = 1 << 23;
 
 template <int DT, bool WEIGHTED>
 __global__ void __launch_bounds__(RW_WAVES * 64) k_rows_out(const typename Elem<DT>::T* __restrict__ x, const float* __restrict__ w,
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(RW_WAVES * 64) k_rows_out(const typename Elem<
   constexpr int EPC = Elem<DT>::EPC;
   typedef E vec __attribute__((ext_vector_type(EPC)));
   const int lane = threadIdx.x & 63;
-  const long long t = (long long)blockIdx.x * RW_WAVES + (threadIdx.x >> 6);
+  const long long t = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RW_WAVES + (threadIdx.x >> 6);
   if (t >= T) return;
   const int kept = *end;
   const int myslot = lane < k ? slot[t * k + lane] : 0;
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(RW_WAVES * 64) k_rows_back(const typename Elem
   constexpr int EPC = Elem<DT>::EPC;
   typedef E vec __attribute__((ext_vector_type(EPC)));
   const int lane = threadIdx.x & 63;
-  const long long t = (long long)blockIdx.x * RW_WAVES + (threadIdx.x >> 6);
+  const long long t = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RW_WAVES + (threadIdx.x >> 6);
   if (t >= T) return;
   const int kept = *end;
   const int myslot = lane < k ? slot[t * k + lane] : 0;
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(RW_WAVES * 64) k_rows_back_grad(const typename
   constexpr int EPC = Elem<DT>::EPC;
   typedef E vec __attribute__((ext_vector_type(EPC)));
   const int lane = threadIdx.x & 63;
-  const long long t = (long long)blockIdx.x * RW_WAVES + (threadIdx.x >> 6);
+  const long long t = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * RW_WAVES + (threadIdx.x >> 6);
   if (t >= T) return;
   const int kept = *end;
   const int myslot = lane < k ? slot[t * k + lane] : 0;
@@ -344,7 +344,9 @@ template <int DT>
 static int launch_rows_t(int op, const void* a, const void* b, const float* w, const int32_t* slot, const int32_t* end, long long T, int k,
                          long long D, void* out, float* dw, hipStream_t st) {
   typedef typename Elem<DT>::T E;
-  const dim3 grid((unsigned)((T + RW_WAVES - 1) / RW_WAVES)), block(RW_WAVES * 64);
+  // (a launch has fewer than 2^32 work items along x: 2^25 rows)
+  const long long blocks = (T + RW_WAVES - 1) / RW_WAVES, along_x = blocks < RW_MAX_X ? blocks : RW_MAX_X;
+  const dim3 grid((unsigned)along_x, (unsigned)((blocks + along_x - 1) / along_x)), block(RW_WAVES * 64);
   const E* in = static_cast<const E*>(a);
   E* o = static_cast<E*>(out);
   if (op == 0) {

@@ -598,7 +598,8 @@ int anerf_combine_rows_backward(const void* dy, const void* z, int32_t dtype, co
  *   x [n_rows][n_in] rows x_stride elements apart, weight [n_out][n_in], bias [n_out] or NULL, down [n_adapters][rank][n_in] (A),
  *   up [n_adapters][n_out][rank] (B), y [n_rows][n_out], all of dtype; h: anerf_adapter_h_size bytes, 16-byte aligned, written: s_i x A_i^T
  *   by position in fp32 [n_rows][rank rounded up to 16], and behind it the forms the products use (kept for the backward).  Sums in fp32, one
- *   rounding at the end. */
+ *   rounding at the end.  n_adapters, rank <= 1024; n_rows < 2^28, n_in, n_out <= 2^24, and fewer than 2^24 tiles of 64 x 64 in y and in dx, for the
+ *   gradients also in weight, down and up together: more is refused (ANERF_E_SHAPE). */
 typedef struct AnerfAdapterIO {
   int32_t dtype, n_adapters, rank;
   float scale;
