@@ -354,9 +354,24 @@ def render_rays_adapted(caster, kw, subject_idxs):
     subject = subject_idxs.reshape(-1).to(kw["ray_batch"].device)
     kw = dict(kw, cyls=kw["cyls"].expand(n, 5))
 
+    def rays(a, b, zz):
+        skts, cam = kw["skts"], kw["cam_idx"]
+        part = dict(kw, ray_batch=kw["ray_batch"][a:b], skts=skts[a:b] if skts.shape[0] == n else skts,
+                    cam_idx=cam if cam is None or cam.numel() == 1 else cam.reshape(-1)[a:b])
+        return part, zz[a:b], subject.expand(n)[a:b, None].expand(b - a, zz.shape[1])
+
     def mlp(net, zz):
-        idx = subject.reshape(-1, 1).expand(n, zz.shape[1]).reshape(-1)
-        return net(encode_rows(net, kw, zz), subject_idxs=idx).view(n, zz.shape[1], 4)
+        if torch.is_grad_enabled() or zz.numel() <= ENCODE_POINTS:
+            part, z, idx = rays(0, n, zz)
+            return net(encode_rows(net, part, z).view(n, zz.shape[1], -1), subject_idxs=idx)
+        # without gradients: rays are independent, and no more of them are encoded at once than ENCODE_POINTS holds (4 KB a point, and again in group
+        # order, and the layers' inputs; rows past 4 GB would also leave the layers' faster loads)
+        raw, step = torch.empty(n, zz.shape[1], 4, dtype=torch.float32, device=zz.device), max(1, ENCODE_POINTS // zz.shape[1])
+        for a in range(0, n, step):
+            b = min(n, a + step)
+            part, z, idx = rays(a, b, zz)
+            raw[a:b] = net(encode_rows(net, part, z).view(b - a, zz.shape[1], -1), subject_idxs=idx)
+        return raw
     return _staged(caster, kw, mlp)
 
 

@@ -63,3 +63,52 @@ def test_more_rows_than_work_items_along_one_axis():
     assert torch.equal(dw, torch.where(kept, x.float().square().sum(1, keepdim=True), 0.0))
     del xs, z, dz, dw
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["poses", "one pose", "codes"])
+def test_a_large_render_holds_a_piece_of_its_points(form, monkeypatch):
+    """an adapted render without gradients: the encoded rows of the whole call are never in memory together, and the picture is that of the
+    whole call (a row's sums may be taken in another order: the bar of the other pictures)"""
+    networks, raycaster = importlib.import_module("a-nerf_amd.networks"), importlib.import_module("a-nerf_amd.raycaster")
+    autograd_path, ad, synth = (importlib.import_module("a-nerf_amd." + m) for m in ("autograd_path", "adapters", "synth"))
+    n, S, Ni, dev = 600, 64, 16, "cuda"
+    codes = form == "codes"
+    kw = dict(use_framecode=True, framecode_ch=16, n_framecodes=6) if codes else {}
+    ck = dict(cutoff=True, cutoff_dist=0.5, cutoff_inputs=True, cutoff_dim=24)
+    nets = []
+    for seed in (11, 12):
+        nets.append(networks.NeRF(D=8, W=256, input_ch=360, input_ch_bones=72, input_ch_views=648, use_viewdirs=True, **kw))
+        nets[-1].load_state_dict({k: torch.tensor(v) for k, v in synth.make_net_params(seed, **(dict(framecode_ch=16, n_codes=6) if codes else {})).items()})
+    ev, eb, ed = (networks.get_embedder(7, 0, 24, cutoff_kwargs=dict(ck))[0], networks.get_embedder(0, 0, 72)[0],
+                  networks.get_embedder(4, 0, 72, cutoff_kwargs=dict(ck, dist_inputs=True))[0])
+    caster = raycaster.RayCaster(nets[0], ev, eb, ed, network_fine=nets[1]).to(dev).requires_grad_(False).eval()
+    torch.manual_seed(1)
+    ads = [ad.NetAdapters(net, 3, rank=4) for net in nets]
+    with torch.no_grad():
+        for a in ads:
+            for name in ad.LAYERS:
+                a.up(name).normal_(0, 0.05)
+    caster.set_adapters(*ads)
+    ro, rd, kp, skts, bones, cyls, _ = synth.scene_batch(n, [0, 1, 2], H=128, W=128, focal=150.0, ray_seed=3, per_ray_pose=True)
+    t = lambda v: torch.tensor(v, dtype=torch.float32, device=dev)
+    pipeline = importlib.import_module("a-nerf_amd.pipeline")
+    rb = pipeline.make_ray_batch(t(ro), t(rd))
+    one = form == "one pose"
+    cut = lambda v: t(v)[:1] if one else t(v)
+    subjects = torch.arange(n, device=dev) % 4
+    cams = (torch.arange(n, device=dev) % 7 - 1).float() if codes else None             # -1: the mean code
+    call = lambda: caster(rb, N_samples=S, kp_batch=cut(kp), skts=cut(skts), cyls=cut(cyls), cams=cams, subject_idxs=subjects, N_importance=Ni,
+                          preproc_kwargs={"density_scale": 1.0})
+    whole = call()
+    monkeypatch.setattr(autograd_path, "ENCODE_POINTS", 5000)                            # 78 rays of the first pass, 62 of the second
+    call()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    parts = call()
+    # one copy of all encoded rows of the second pass alone
+    assert torch.cuda.max_memory_allocated() - before < n * (S + Ni) * 1080 * 4
+    for k in ("rgb_map", "acc_map", "rgb0"):
+        assert float((whole[k] - parts[k]).abs().max()) < 1e-4, k
+    assert float(whole["acc_map"].max()) > 0.1
