@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 // The low-rank term comes first, behind the first stage's loads: for every adapter with positions in the tile h B_i^T is added to the
 // blocks of its rows; a block that two adapters share takes it by row (a NaN in one adapter stays with its rows).  Waves with rows of many
 // adapters take it row by row.
-// fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set, so that no chain of
-// additions is longer than 8 * FOLD + K / (32 * FOLD).
+// fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set.  An instruction adds its four
+// products one after the other, so that a chain has Rp (the low-rank term, in the first) + 32 * FOLD + K / (32 * FOLD) additions at most.
 // Bound by the matrix units.  bf16, 8192 x 4096 -> 4096 with 24 adapters of rank 32: 245 us, 1140 TFLOP/s (without adapters, once the clocks
 // allow it, 1305; a plain product of that shape by the BLAS 1300 .. 1380); fp32, 65536 x 688 -> 256: 182 us, 127 TFLOP/s (the BLAS 135),
 // 8192 x 4096 -> 4096: 147 TFLOP/s of the 150 that it reaches.
@@ -232,7 +232,7 @@ struct MainArgs {
 constexpr int FOLD = 16;
 
 template <int DT, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
-__global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) k_main(MainArgs P) {
+__global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_main(MainArgs P) {
   typedef typename Elem<DT>::T E;
   constexpr int EPC = Elem<DT>::EPC, KB = 8 * EPC;        // elements of a 128-byte row piece
   constexpr int NW = WM * WN;
