@@ -122,3 +122,48 @@ def test_whole_numbers_of_every_rank(R, dt):
     y = ad.adapter_linear(xd, W.cuda(), A, B, idx.cuda())
     for got, ref in zip([y, *torch.autograd.grad(y, [xd, A, B], g.cuda())], (want, dx, dA, dB)):
         same_kind(got, ref.to(DT[dt]))
+
+
+STEP = 2.0 ** -23
+
+
+def within(got, want, bound, dt):
+    """|got - want| <= bound + half a step of the result (the smallest normal number's below it)"""
+    got, want = got.double(), want.double()
+    tol = bound + torch.finfo(dt).eps / 2 * (want.abs() + bound) + torch.finfo(dt).tiny
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.numel(), float((got - want).abs()[bad].max()), bad.nonzero()[:4].tolist())
+
+
+# rows x inputs -> outputs, adapters, rank: large tiles in the gradient of x, as they lie and from padded copies; pieces of 128 rows and more, which
+# the gradients of A and B walk in several turns and add in four ways; as many adapters as leave a workgroup several turns of their sums
+MANY = [(4100, 2050, 2060, 5, 16), (4099, 2048, 2056, 12, 16), (24001, 688, 256, 3, 8), (3000, 640, 520, 1000, 16), (5003, 1032, 1000, 6, 128), (9001, 264, 4104, 2, 40)]
+
+
+@pytest.mark.parametrize("M,K,N,L,R", MANY)
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_gradients_of_many_rows(M, K, N, L, R, dt):
+    """all three gradients against 64 bits on the device.  Tolerances are counted: a sum of n products in fp32 is off by (n + 2) * 2^-23 of the
+    products' magnitudes at most, sums of sums by their own bound times the factor besides, h and u lose 2^-23 of themselves as pieces"""
+    dtype, scale = DT[dt], 0.75
+    gen = torch.Generator(device="cuda").manual_seed(M + N)
+    mk = lambda *s, f=1.0: (torch.randn(*s, generator=gen, device="cuda") * f).to(dtype)
+    x, W, A, B, g = mk(M, K), mk(N, K, f=K ** -0.5), mk(L, R, K, f=K ** -0.5), mk(L, N, R, f=R ** -0.5), mk(M, N)
+    idx = torch.randint(-1, L, (M,), generator=gen, device="cuda")
+    xd, Ad, Bd = (t.clone().requires_grad_() for t in (x, A, B))
+    y = ad.adapter_linear(xd, W, Ad, Bd, idx, scale=scale)
+    gx, gA, gB = torch.autograd.grad(y, [xd, Ad, Bd], g)
+    del y, xd, Ad, Bd
+    x, W, A, B, g = (t.double() for t in (x, W, A, B, g))
+    dx, dxb = g @ W, (N + R + 4) * STEP * (g.abs() @ W.abs())
+    for i in range(L):
+        r = (idx == i).nonzero()[:, 0]
+        n = len(r)
+        xi, gi, a, b = x[r], g[r], A[i], B[i]
+        h, hb = xi @ a.t(), (K + 2) * STEP * (xi.abs() @ a.abs().t())
+        u, ub = gi @ b, (N + 2) * STEP * (gi.abs() @ b.abs())
+        dx[r] += scale * u @ a
+        dxb[r] += scale * (ub + (N + R + 5) * STEP * u.abs()) @ a.abs()
+        within(gA[i], scale * u.t() @ xi, scale * (ub + (n + 5) * STEP * u.abs()).t() @ xi.abs(), dtype)
+        within(gB[i], scale * gi.t() @ h, scale * gi.abs().t() @ (hb + (n + 5) * STEP * h.abs()), dtype)
+    within(gx, dx, dxb, dtype)
