@@ -1154,7 +1154,7 @@ def adapter_backward(g, x, weight, down, up, rows, h, scale=1.0, scale_of=None, 
     if g.shape != (x.shape[0], weight.shape[0]) or not (g.stride(1) == 1 or g.shape[1] == 1):
         raise ValueError(f"adapter_backward: g {tuple(g.shape)} with strides {g.stride()} for y {(x.shape[0], weight.shape[0])}")
     need = _lib.load().anerf_adapter_h_size(C.byref(_adapter_io(x, weight, down, up, rows, None, scale, scale_of)))
-    if h.device != x.device or not h.is_contiguous() or h.numel() * h.element_size() < need:
+    if not torch.is_tensor(h) or h.device != x.device or not h.is_contiguous() or h.numel() * h.element_size() < need:
         raise ValueError("adapter_backward: h must be what adapter_linear returned for these rows")
     return _adapter_backward(g, x, weight, down, up, rows, h, scale, scale_of, want_dx, want_ddown, want_dup)
 

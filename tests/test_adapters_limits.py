@@ -1,5 +1,6 @@
 """The largest sizes: row calls past 2^32 work items, and what the adapter calls refuse (CPU: before any launch)."""
 import ctypes
+import gc
 import importlib
 
 import pytest
@@ -8,6 +9,15 @@ import torch
 _lib = importlib.import_module("a-nerf_amd._lib")
 E_SHAPE = -2
 P = lambda k: ctypes.c_void_p(0x7F0000000000 + 0x1000 * k)          # never read: every call returns before its launch
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_back_what_the_allocator_cached():
+    """other tests account for single allocations: blocks of this module's sizes would serve them instead of fresh ones"""
+    yield
+    gc.collect()
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
 
 
 def _io(**kw):
@@ -37,6 +47,16 @@ def test_launches_of_too_many_work_items_are_refused():
     assert size(lib.anerf_adapter_backward_workspace_size, n_adapters=1024, rank=1, n_in=2 ** 19, n_out=1) > 0
     io = _io(n_rows=2 ** 28)
     assert lib.anerf_adapter_linear(ctypes.byref(io), P(9), 1 << 62, None) == E_SHAPE
+
+
+@pytest.mark.gpu
+def test_the_backward_wants_what_the_forward_returned():
+    ops = importlib.import_module("a-nerf_amd.ops")
+    x, W, A, B = (torch.zeros(*s, device="cuda") for s in ((80, 32), (24, 32), (3, 4, 32), (3, 24, 4)))
+    plan = ops.route_rows(torch.zeros(80, dtype=torch.long, device="cuda"), 3)
+    for h in (None, [1.0], torch.zeros(4, device="cuda"), torch.zeros(80, 64)):
+        with pytest.raises(ValueError, match="h must be"):
+            ops.adapter_backward(torch.zeros(80, 24, device="cuda"), x, W, A, B, plan, h)
 
 
 @pytest.mark.gpu

@@ -1,4 +1,5 @@
 """GPU: infinities in adapters, and the bits that the low-rank term keeps, in every form of the product."""
+import gc
 import importlib
 
 import pytest
@@ -8,6 +9,15 @@ pytestmark = pytest.mark.gpu
 
 ad = importlib.import_module("a-nerf_amd.adapters")
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_back_what_the_allocator_cached():
+    """other tests account for single allocations: blocks of this module's sizes would serve them instead of fresh ones"""
+    yield
+    gc.collect()
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
 
 
 def same_kind(got, want):

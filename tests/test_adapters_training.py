@@ -1,5 +1,6 @@
 """Adapters in training: gradients over several ranks (CPU, gloo), captured steps whose schedule moves tau, forward
 mode."""
+import gc
 import importlib
 import os
 import sys
@@ -16,6 +17,15 @@ networks = importlib.import_module("a-nerf_amd.networks")
 ops = importlib.import_module("a-nerf_amd.ops")
 raycaster = importlib.import_module("a-nerf_amd.raycaster")
 trainer = importlib.import_module("a-nerf_amd.trainer")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_back_what_the_allocator_cached():
+    """other tests account for single allocations: blocks of this module's sizes would serve them instead of fresh ones"""
+    yield
+    gc.collect()
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
 
 
 def small_caster(single=False):
@@ -259,3 +269,46 @@ def test_forward_mode_is_refused_not_dropped(monkeypatch):
         n = len(calls)
         ad.dispatch_rows(x, plan), ad.combine_rows(x, plan, w), lin(), lin(rows=idx)
         assert len(calls) == n + 4
+
+
+@pytest.mark.gpu
+def test_adapters_train_through_the_graphed_trainer():
+    """Trainer.enable_graph over attached adapters and a FusedAdam of them, tau and the learning rate scheduled by the trainer itself, an exchange
+    of the adapters in the middle: bit for bit the eager trainer"""
+    import numpy as np
+    import test_trajectory as tj
+    synth, optim = importlib.import_module("a-nerf_amd.synth"), importlib.import_module("a-nerf_amd.optim")
+    case, dev = tj.CASES["surreal"], torch.device("cuda")
+    args = tj.ref_args(case["args"])
+    args.cutoff_step, args.cutoff_rate = 1, 1.05                                   # tau = 20 * 1.05 ^ (i / 1000): 500 steps of fp32 an iteration
+    data_attrs = {"skel_type": tj.Skel, "near": 0.0, "far": 1.0, "n_views": tj.N_POSES, "hwf": (512, 512, 600.0),
+                  "joint_coords": np.tile(np.eye(3, dtype=np.float32), (24, 1, 1))}
+    runs = []
+    for graphed in (False, True):
+        torch.manual_seed(5)
+        rk_train, rk_test, _, _, _, _ = raycaster.create_raycaster(args, data_attrs, device=dev)
+        caster = rk_test["ray_caster"]
+        for net, seed in ((caster.network, case["seeds"][0]), (caster.network_fine, case["seeds"][1])):
+            net.load_state_dict({k: torch.tensor(v) for k, v in synth.make_net_params(seed, args.multires, args.multires_views, 0, tj.N_POSES).items()})
+        caster.train().requires_grad_(False)
+        caster._rng = ops.DeviceRng(seed=77, stream_id=1)
+        sets = [[ad.NetAdapters(net, 3, rank=4) for net in (caster.network, caster.network_fine)] for _ in range(2)]
+        opt = optim.FusedAdam([p for ads in sets for a in ads for p in a.parameters()], lr=1e-3)
+        opt.materialize()
+        tr = trainer.Trainer(args, data_attrs, opt, None, rk_train, rk_test, popt_kwargs=None, device=dev)
+        if graphed:
+            tr.enable_graph(eager_steps=1)
+        batch = tj._batch(case, dev)
+        n = case["n"]
+        losses = []
+        for i in range(1, 13):
+            caster.set_adapters(*sets[0 if i <= 4 or i > 8 else 1])
+            batch["subject_idxs"] = (torch.arange(n, device=dev) * i) % 4
+            loss, _ = tr.train_batch(batch, i=i, global_step=i)
+            losses.append(loss["total_loss"].detach().clone())
+        torch.cuda.synchronize()
+        runs.append((losses, opt.flat.clone(), tr, caster))
+    (e, ef, _, ec), (g, gf, tr, gc_) = runs
+    assert not tr._gs.eager_only and tr._gs.captures == 2 and tr._gs.replays >= 8, (tr._gs.eager_only, tr._gs.captures, tr._gs.replays)
+    assert all(torch.equal(a, b) for a, b in zip(e, g)) and torch.equal(ef, gf) and len({float(v) for v in e}) == 12
+    assert gc_.embed_fn.get_tau() == ec.embed_fn.get_tau() == float(np.float32(20.0 * 1.05 ** 0.012))
