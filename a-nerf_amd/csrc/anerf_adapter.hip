@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(256) k_split_rows(const float* __restrict__ h,
 // adapters take it row by row.
 // fp32 sums of long rows are kept in two levels: every FOLD stages the accumulators are added to a second set.  An instruction adds its four
 // products one after the other, so that a chain has Rp (the low-rank term, in the first) + 32 * FOLD + K / (32 * FOLD) additions at most.
-// Bound by the matrix units.  bf16, 8192 x 4096 -> 4096 with 24 adapters of rank 32: 245 us, 1140 TFLOP/s (without adapters, once the clocks
-// allow it, 1305; a plain product of that shape by the BLAS 1300 .. 1380); fp32, 65536 x 688 -> 256: 182 us, 127 TFLOP/s (the BLAS 135),
-// 8192 x 4096 -> 4096: 147 TFLOP/s of the 150 that it reaches.
+// Bound by the matrix units.  In a trace, in turn with a library's plain product of the same rows (us with adapters, without, the library): bf16,
+// 8192 x 4096 -> 4096, 24 adapters of rank 32: 269 (1020 TFLOP/s; in a loop of its own 239), 243, 195; 4096 x 2048 -> 2048, 12 of rank 16: 41, 35, 33;
+// fp32, 65520 x 688 -> 256, 16 of rank 8: 214 (108 TFLOP/s; rows in order 211), 205, 203; 24000 x 688 -> 256: 87, 75, 94;
+// 8192 x 4096 -> 4096, 24 of rank 32: 1901 (145 TFLOP/s), 1873, 1830.
 struct MainArgs {
   const void *x, *w, *bias, *up;
   const int32_t *offsets, *order;
@@ -779,8 +780,9 @@ __global__ void __launch_bounds__(256) k_sum_parts(const float* __restrict__ par
 //   k_few       a workgroup owns 16*NT outputs of all rows; its eight waves take every eighth 128 bytes of W's rows straight into MFMA operands
 //               (W is read once, no LDS on its way), x comes from L2, and the waves' sums are added through LDS.  The low-rank term of
 //               an output is a dot of `rank` values in fp32, read in front of the loop, so that B's latency hides behind W's.
-// bf16, rank 16: one row x 4096 -> 4096 5.5 + 7.8 us (W at 4.3 TB/s); 48 rows x 4096 -> 8192 5.8 + 25 us (67 MB of W, 13 MB of B, and
-// 126 MB of x from L2).  The routed kernels take 56 us for the 48 rows: their tiles are 64 rows high and wait for one stage after the other.
+// bf16, rank 16: one row x 4096 -> 4096 5.7 + 8.0 us (W at 4.2 TB/s); 48 rows x 4096 -> 8192 5.6 + 25 us (67 MB of W, 13 MB of B, and
+// 126 MB of x from L2).  The routed kernels take 42 us for the 48 rows, plan included, and catch up where rows are many and outputs few: 64 rows x
+// 4096 -> 1024 26.9 us here, 25.7 there (fp32 45.8, 40.7), 4096 -> 4096 27.8 and 36.8, 1024 -> 1024 10.8 and 19.0: the limit is 64 rows.
 constexpr int FEW_WAVES = 8;
 static_assert(ANERF_FEW_ROWS == 64, "four blocks of 16 rows");
 
