@@ -351,13 +351,18 @@ def render_rays_adapted(caster, kw, subject_idxs):
         raise ValueError(f"subject_idxs: one int32 / int64 subject per ray, got {getattr(subject_idxs, 'shape', type(subject_idxs))} for {n} rays")
     if caster.network.use_framecode and kw["cam_idx"] is None:
         raise ValueError("subject_idxs: a network with frame codes needs cams")
+    # (before the rays are cut into pieces, whose size could agree with a wrong number by chance)
+    if kw["skts"].shape[0] not in (1, n):
+        raise ValueError(f"skts {tuple(kw['skts'].shape)} for {n} rays: one pose, or one per ray")
+    if caster.network.use_framecode and kw["cam_idx"].numel() not in (1, n):
+        raise ValueError(f"cams {tuple(kw['cam_idx'].shape)} for {n} rays: one, or one per ray")
     subject = subject_idxs.reshape(-1).to(kw["ray_batch"].device)
     kw = dict(kw, cyls=kw["cyls"].expand(n, 5))
 
     def rays(a, b, zz):
         skts, cam = kw["skts"], kw["cam_idx"]
         part = dict(kw, ray_batch=kw["ray_batch"][a:b], skts=skts[a:b] if skts.shape[0] == n else skts,
-                    cam_idx=cam if cam is None or cam.numel() == 1 else cam.reshape(-1)[a:b])
+                    cam_idx=cam if cam is None or cam.numel() != n else cam.reshape(-1)[a:b])
         return part, zz[a:b], subject.expand(n)[a:b, None].expand(b - a, zz.shape[1])
 
     def mlp(net, zz):

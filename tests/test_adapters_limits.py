@@ -132,3 +132,10 @@ def test_a_large_render_holds_a_piece_of_its_points(form, monkeypatch):
     for k in ("rgb_map", "acc_map", "rgb0"):
         assert float((whole[k] - parts[k]).abs().max()) < 1e-4, k
     assert float(whole["acc_map"].max()) > 0.1
+    # as many poses or cameras as a piece of the second pass has rays are not one per ray
+    bad = dict(N_samples=S, kp_batch=cut(kp), skts=cut(skts), cyls=cut(cyls), cams=cams, subject_idxs=subjects, N_importance=Ni)
+    with pytest.raises(ValueError, match="skts"):
+        caster(rb, **{**bad, "skts": t(skts)[:5000 // S]})
+    if codes:
+        with pytest.raises(ValueError, match="cams"):
+            caster(rb, **{**bad, "cams": cams[:5000 // S]})
