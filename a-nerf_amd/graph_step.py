@@ -128,8 +128,10 @@ def _values(out):
         return out.detach()
     if isinstance(out, dict):
         return {k: _values(v) for k, v in out.items()}
-    if isinstance(out, (list, tuple)) and not hasattr(out, "_fields"):
-        return type(out)(_values(v) for v in out)
+    if isinstance(out, tuple) and hasattr(out, "_fields"):
+        return type(out)(*map(_values, out))
+    if isinstance(out, (list, tuple)):
+        return type(out)(map(_values, out))
     return out
 
 

@@ -73,8 +73,11 @@ class RayCaster(nn.Module):
 
     def step_parameters(self):
         """everything a training step through this caster gives gradients to: its own parameters and the attached adapters', each once"""
-        attached = [net.adapters() for net in (self.network, self.network_fine) if net is not None and net.adapters() is not None]
-        return list({id(p): p for m in [self, *attached] for p in m.parameters()}.values())
+        return list({id(p): p for m in [self, *self.attached_adapters()] if m is not None for p in m.parameters()}.values())
+
+    def attached_adapters(self):
+        """adapters of the coarse and of the fine network, None where there are none"""
+        return [net.adapters() if isinstance(net, NeRF) else None for net in (self.network, self.network_fine)]
 
     @torch.no_grad()
     def forward_eval(self, *args, **kwargs):

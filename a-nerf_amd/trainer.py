@@ -136,7 +136,7 @@ class Trainer:
         are kept, so that no other module takes their place in memory"""
         caster = self.render_kwargs_train["ray_caster"]
         caster = getattr(caster, "module", caster)
-        ads = [net.adapters() for net in (caster.network, caster.network_fine) if net is not None]
+        ads = caster.attached_adapters() if hasattr(caster, "attached_adapters") else []
         keep = self.__dict__.setdefault("_key_adapters", {})
         keep.update({id(a): a for a in ads if a is not None})
         return tuple(None if a is None else id(a) for a in ads)

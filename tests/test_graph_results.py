@@ -1,6 +1,7 @@
 """CPU: nothing that outlives an iteration holds its autograd graph (one that lives through the next capture ends the process there)."""
 import importlib
 import types
+import typing
 import weakref
 
 import torch
@@ -23,6 +24,11 @@ class _Token:
     pass
 
 
+class _Named(typing.NamedTuple):
+    y: torch.Tensor
+    n: int
+
+
 def test_results_of_eager_iterations_hold_no_graph():
     w = torch.ones(3, requires_grad=True)
     alive = []
@@ -33,7 +39,7 @@ def test_results_of_eager_iterations_hold_no_graph():
         y = _Probe.apply(w, token)
         loss = (y * i).sum()
         loss.backward()
-        return {"loss": loss, "more": {"maps": [y, (y + 1,)], "n": i, "none": None}}
+        return {"loss": loss, "more": {"maps": [y, (y + 1,)], "n": i, "none": None, "named": _Named(y, i)}}
 
     emb = types.SimpleNamespace()
     for kw in (dict(enabled=False), dict(eager_steps=5)):
@@ -42,7 +48,7 @@ def test_results_of_eager_iterations_hold_no_graph():
         assert alive[-1]() is None                                             # the iteration's graph is gone although its results live
         tensors = [out["loss"], out["more"]["maps"][0], out["more"]["maps"][1][0]]
         assert not any(t.requires_grad for t in tensors) and float(out["loss"]) == 6.0 and torch.equal(tensors[2], torch.full((3,), 2.0))
-        assert out["more"]["n"] == 2 and out["more"]["none"] is None
+        assert out["more"]["n"] == 2 and out["more"]["none"] is None and type(out["more"]["named"]) is _Named and not out["more"]["named"].y.requires_grad
 
 
 def test_the_pose_layer_drops_its_last_graph_before_it_builds_the_next(monkeypatch):
