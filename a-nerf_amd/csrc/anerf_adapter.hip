@@ -18,7 +18,7 @@ namespace anerf {
 // ------------------------------------------------------------------------------------------------------------ h = s_i x A_i^T
 // HBM-bound on x.  The four waves split the contraction (every fourth 64-byte step), each holding all 16*MB rows x 16*NJ ranks of the
 // piece in MFMA accumulators, fed straight from memory: a row of A serves all rows of the piece, and nothing is read twice from HBM.
-// 65520 x 688 fp32, rank 8: 32 us, 5.6 TB/s; 8192 x 4096 bf16, 24 adapters of rank 32 (73 MB): 21 us where x was just
+// 65520 x 688 fp32, rank 8: 32 us, 5.6 TB/s; 8192 x 4096 bf16, 24 adapters of rank 32 (73 MB): 23 us where x was just
 // written, from HBM 33, with 16 rows a piece 35; 200 rows
 // x 4096 bf16: 13.7 us with 32 rows a piece, 10.2 with 16.  More waves a piece or deeper loads gain nothing: a few pieces are bound by
 // what one CU can load.
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN <= 64 * 64 ? 4 : 2) k_ma
               const E* b = br + (col < P.N ? col : P.N - 1) * P.R;
               float dot = 0.f;
 #pragma unroll 1
-              for (int j = 0; j < P.R; ++j) dot = fmaf(hr[j], (float)b[j], dot);
+              for (int j = 0; j < P.R && dot == dot; ++j) dot = fmaf(hr[j], (float)b[j], dot);      // (NaN stays NaN)
               acc[m][n][e] = dot;
             }
         }
@@ -969,7 +969,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_few(const typename Elem<DT>:
 // take every fourth group of rows and are added through LDS, a quarter of the sums each.  What bounds it is the latency of Z's loads, so
 // the next turn's rows are on their way while a turn's products run, and two waves a SIMD are asked for (with one, whose registers then hold
 // more: rank 128, 8192 x (1024 + 1024) fp16, the whole backward 229 instead of 170 us).
-// 4096 x (2048 + 2048) bf16, 12 adapters of rank 16: 20 us; 24000 x (688 + 256) fp32, rank 8: 28 us (91 MB).
+// 4096 x (2048 + 2048) bf16, 12 adapters of rank 16: 18 us; 24000 x (688 + 256) fp32, rank 8: 27 us (91 MB).
 // BY_RANK: part [piece][Rp][C] (operand order Z, V), else [piece][C][Rp] (V, Z): a lane ends with four values that lie together.
 constexpr int TG_WAVES = 4, TG_COLS = 64, TG_DEPTH = 2;
 
@@ -1149,7 +1149,7 @@ struct TransposeJobs {
 };
 
 // 64 x 64 values a workgroup through LDS, 16 bytes a lane on both sides where the rows allow it.  HBM- and latency-bound: W 2048 x 2048
-// and twelve pairs of rank 16, bf16: 7.5 us.
+// and twelve pairs of rank 16, bf16: 6.6 us.
 template <typename U>
 __global__ void __launch_bounds__(256) k_transpose(TransposeJobs J) {
   constexpr int V = 16 / sizeof(U);
